@@ -41,7 +41,7 @@ def build_ref() -> bool:
     """Compile _ref/libmpref.so (the reference CPU engine) and, once the product
     libraries exist, _ref/cow_test_b200 (the reference's cow_test.cpp on the B200
     drop-in runner) when the reference sources are present."""
-    if not os.path.isdir(REFERENCE):
+    if not os.path.isfile(os.path.join(REFERENCE, "src", "core", "tensor.cpp")):  # absent, or an empty mount point
         return os.path.exists(REF_SO)
     targets = ["ref"]
     if os.path.exists(os.path.join(os.path.dirname(HERE), "tinyinfer_b200", "libmpb200_host.so")):
