@@ -248,6 +248,137 @@ int mp_paged_attention_prefill(const float* q, const float* keys, const float* v
                                int32_t count, float* out, void* stream);
 int mp_paged_attention_status(void* stream);
 
+/* ---------------------------------------------------------------- 8-bit paged KV cache
+ * Operators on a paged K/V cache held in 8 bits, with one scale for each block of
+ * block_tokens tokens, kv head and K or V (no counterpart in the reference; a quarter
+ * of its FP32 cache's bytes). They stand beside the FP32 cache's operators above,
+ * on caller device buffers:
+ *   mp_kv8_append             rotates q and k, quantises k and v into the pages;
+ *   mp_kv8_attention_decode   one query row per sequence over the pages;
+ *   mp_kv8_attention_prefill  causal attention of packed chunks of rows.
+ * A value is code * scale. Codes are INT8 (-127..127) or E4M3 (bytes of the 8-bit
+ * float with 4 exponent and 3 mantissa bits, largest 448). The append chooses scales
+ * that are powers of two; the attentions take any finite scale.
+ *
+ * All arrays are device memory of the current device unless stated, and the metadata
+ * (tables, lengths, row_offsets, starts) is read by the kernels only: no call copies
+ * to the device, synchronises or allocates, so every call can be captured into a
+ * graph and replayed with other metadata in the same buffers. Calls that share a
+ * workspace must not overlap. A null or misaligned pointer, a pointer that is not
+ * memory of the current device, and sizes outside the stated ranges are refused with
+ * MP_ERR_INVALID (a geometry without a kernel with MP_ERR_UNSUPPORTED) before
+ * anything is queued. What only the device can see goes to `device_error`
+ * (optional, caller-owned device word, zeroed by the caller; mp_kv8_status reads
+ * and clears it): bit 1 = a block id outside [0, max_blocks), metadata outside its
+ * table, or a position outside the rotation tables; bit 2 = a copy wait expired;
+ * bit 4 = an appended value was NaN or infinite, or the scale of a block that already
+ * held tokens was no power of two. */
+#define MP_KV8_INT8 0
+#define MP_KV8_E4M3 1
+#define MP_TYPE_F32 0
+#define MP_TYPE_BF16 1
+#define MP_ROPE_HALF 0        /* pairs (i, i + rotary_dim / 2), the reference's */
+#define MP_ROPE_INTERLEAVED 1 /* pairs (2i, 2i + 1) */
+
+typedef struct {
+    void* pages;          /* [max_blocks][kv_heads][2][block_tokens][head_dim] codes, 0 = K, 1 = V; 16-byte aligned */
+    float* scales;        /* [max_blocks][kv_heads][2]; 8-byte aligned */
+    int64_t page_stride;  /* bytes from a block to the next: a multiple of 16, >= kv_heads * 2 * block_tokens * head_dim */
+    int64_t scale_stride; /* floats from a block's scales to the next block's: even, >= 2 * kv_heads */
+    int32_t format;       /* MP_KV8_INT8 or MP_KV8_E4M3 */
+    int32_t kv_heads;     /* 1 .. 256 */
+    int32_t head_dim;     /* 64 or 128 */
+    int32_t block_tokens; /* a multiple of 16, 16 .. 256 */
+    int32_t max_blocks;
+} mp_kv8_cache;
+
+/* Rows of `count` sequences, packed: sequence i's rows are row_offsets[i] ..
+ * row_offsets[i + 1] - 1 (row_offsets[0] = 0, nondecreasing; a sequence may have none),
+ * at positions starts[i], starts[i] + 1, ...; `rows` is the number of rows that the
+ * buffers hold: rows at or past row_offsets[count] are neither read nor written. A
+ * row is heads (q) or kv_heads (k, v) x head_dim values of `type`; strides count
+ * values between rows (a fused q | k | v projection: three pointers, one stride), with
+ * 16-byte aligned rows.
+ *
+ * Every row's k is rotated by its position, and k and v go to slot position %
+ * block_tokens of block tables[i][position / block_tokens]. With q, the rotated q goes
+ * to q_out (which may be q itself). Rotation of a pair (a, b): (a cos - b sin, b cos
+ * + a sin) with row `position` of cos / sin ([max_positions][rotary_dim / 2]), in 64
+ * bits, rounded once; dims at or past rotary_dim pass unrotated (rotary_dim 0: no
+ * rotation, cos and sin unused).
+ *
+ * The scale of a block written from its slot 0 on is the smallest power of two with
+ * which the largest new magnitude fits the format (at least 2^-100); what the block
+ * held is forgotten. A block that held tokens before (the first appended slot is past
+ * 0) keeps its scale if that suffices, else takes the larger one and its codes are
+ * rounded to it. A code is the nearest to value / scale, ties to even. An INT8 value
+ * is then off by at most half its block's scale when appended, and by less than one
+ * scale after any number of re-roundings (each scale is at least twice the one
+ * before). NaN is stored as 0 and infinity as the largest code, with the error bit.
+ * A block takes new rows from one sequence per call; slots past a sequence's last
+ * token keep their bytes. */
+typedef struct {
+    const void *q, *k, *v; /* q optional */
+    void* q_out;           /* with q */
+    int64_t q_stride, k_stride, v_stride, q_out_stride;
+    const float *cos, *sin;
+    const int32_t* tables;      /* [count][table_stride] block ids */
+    const int32_t* row_offsets; /* [count + 1] */
+    const int32_t* starts;      /* [count] */
+    int32_t type;               /* MP_TYPE_* of q, k, v, q_out */
+    int32_t heads;              /* query heads, a multiple of kv_heads */
+    int32_t rotary_dim;         /* a multiple of 8, 0 .. head_dim */
+    int32_t rope_layout;        /* MP_ROPE_* */
+    int32_t max_positions;
+    int32_t table_stride;
+    int32_t count; /* 1 .. 65536 */
+    int32_t rows;
+} mp_kv8_append_args;
+int mp_kv8_append(const mp_kv8_cache* cache, const mp_kv8_append_args* args, uint32_t* device_error, void* stream);
+
+/* out[i] = softmax(scale * q[i] K^T) V over tokens 0 .. lengths[i] - 1 of sequence i,
+ * query head h reading kv head h / (heads / kv_heads). A length of 0 gives a row of
+ * zeros. Sums, maxima and weights are FP32; products run on the tensor cores as FP16
+ * halves (FP32-level: the codes are exact in FP16, an FP32 query and weight is two
+ * halves). The rows' tokens are cut into equal runs over the device and joined. */
+typedef struct {
+    const void* q;
+    void* out;
+    int64_t q_stride, out_stride;
+    const int32_t* tables;
+    const int32_t* lengths; /* [count] */
+    void* workspace;        /* 16-byte aligned, mp_kv8_decode_workspace bytes, zeroed before its first use; left as the next call needs it */
+    size_t workspace_bytes;
+    int32_t type, heads, table_stride, count;
+    float scale;
+} mp_kv8_decode_args;
+size_t mp_kv8_decode_workspace(const mp_kv8_cache* cache, int32_t heads);
+int mp_kv8_attention_decode(const mp_kv8_cache* cache, const mp_kv8_decode_args* args, uint32_t* device_error,
+                            void* stream);
+
+/* Causal attention of packed chunks of rows (row_offsets, starts, rows as for the
+ * append): the row at position p attends to tokens 0 .. p of its sequence, which are in
+ * the pages already (the chunk's own rows among them: append first). */
+typedef struct {
+    const void* q;
+    void* out;
+    int64_t q_stride, out_stride;
+    const int32_t* tables;
+    const int32_t* row_offsets;
+    const int32_t* starts;
+    void* workspace; /* as for decode, of mp_kv8_prefill_workspace bytes */
+    size_t workspace_bytes;
+    int32_t type, heads, table_stride, count, rows;
+    float scale;
+} mp_kv8_prefill_args;
+size_t mp_kv8_prefill_workspace(const mp_kv8_cache* cache, int32_t heads);
+int mp_kv8_attention_prefill(const mp_kv8_cache* cache, const mp_kv8_prefill_args* args, uint32_t* device_error,
+                             void* stream);
+/* Synchronises `stream`, reads and clears *device_error: MP_OK, MP_ERR_BOUNDS,
+ * MP_ERR_TIMEOUT or MP_ERR_NONFINITE (the first that applies in the order timeout,
+ * bounds, nonfinite). */
+int mp_kv8_status(uint32_t* device_error, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

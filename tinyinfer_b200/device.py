@@ -58,6 +58,43 @@ class TailCopyRegionC(C.Structure):
     _fields_ = [(n, C.c_uint64) for n in ("destination", "source", "pitch", "width", "rows")]
 
 
+MP_KV8_INT8, MP_KV8_E4M3 = range(2)
+MP_TYPE_F32, MP_TYPE_BF16 = range(2)
+MP_ROPE_HALF, MP_ROPE_INTERLEAVED = range(2)
+
+
+class Kv8Cache(C.Structure):
+    """mp_kv8_cache: an 8-bit paged K/V cache in caller memory. Pointers are device addresses."""
+    _fields_ = [("pages", C.c_void_p), ("scales", C.c_void_p), ("page_stride", C.c_int64), ("scale_stride", C.c_int64),
+                ("format", C.c_int32), ("kv_heads", C.c_int32), ("head_dim", C.c_int32), ("block_tokens", C.c_int32),
+                ("max_blocks", C.c_int32)]
+
+
+class Kv8AppendArgs(C.Structure):
+    """mp_kv8_append_args; a serving loop over fixed buffers keeps one and calls with it every step."""
+    _fields_ = ([(n, C.c_void_p) for n in ("q", "k", "v", "q_out")] +
+                [(n, C.c_int64) for n in ("q_stride", "k_stride", "v_stride", "q_out_stride")] +
+                [(n, C.c_void_p) for n in ("cos", "sin", "tables", "row_offsets", "starts")] +
+                [(n, C.c_int32) for n in ("type", "heads", "rotary_dim", "rope_layout", "max_positions", "table_stride",
+                                          "count", "rows")])
+
+
+class Kv8DecodeArgs(C.Structure):
+    """mp_kv8_decode_args."""
+    _fields_ = [("q", C.c_void_p), ("out", C.c_void_p), ("q_stride", C.c_int64), ("out_stride", C.c_int64),
+                ("tables", C.c_void_p), ("lengths", C.c_void_p), ("workspace", C.c_void_p),
+                ("workspace_bytes", C.c_size_t), ("type", C.c_int32), ("heads", C.c_int32), ("table_stride", C.c_int32),
+                ("count", C.c_int32), ("scale", C.c_float)]
+
+
+class Kv8PrefillArgs(C.Structure):
+    """mp_kv8_prefill_args."""
+    _fields_ = [("q", C.c_void_p), ("out", C.c_void_p), ("q_stride", C.c_int64), ("out_stride", C.c_int64),
+                ("tables", C.c_void_p), ("row_offsets", C.c_void_p), ("starts", C.c_void_p), ("workspace", C.c_void_p),
+                ("workspace_bytes", C.c_size_t), ("type", C.c_int32), ("heads", C.c_int32), ("table_stride", C.c_int32),
+                ("count", C.c_int32), ("rows", C.c_int32), ("scale", C.c_float)]
+
+
 _lib = None
 
 
@@ -108,6 +145,13 @@ def library() -> C.CDLL:
                                                    C.c_int32, C.c_int32, C.c_void_p, C.c_int32, C.c_void_p,
                                                    C.c_void_p, C.c_int32, C.c_void_p, C.c_void_p]
         lib.mp_gemm_f32.argtypes = [C.c_void_p, C.c_void_p, C.c_void_p, C.c_int32, C.c_int32, C.c_int32, C.c_void_p]
+        for name, args in (("append", Kv8AppendArgs), ("attention_decode", Kv8DecodeArgs),
+                           ("attention_prefill", Kv8PrefillArgs)):
+            getattr(lib, "mp_kv8_" + name).argtypes = [C.POINTER(Kv8Cache), C.POINTER(args), C.c_void_p, C.c_void_p]
+        for name in ("mp_kv8_decode_workspace", "mp_kv8_prefill_workspace"):
+            getattr(lib, name).argtypes = [C.POINTER(Kv8Cache), C.c_int32]
+            getattr(lib, name).restype = C.c_size_t
+        lib.mp_kv8_status.argtypes = [C.c_void_p, C.c_void_p]
         _lib = lib
     return _lib
 
@@ -330,3 +374,35 @@ def gemm_f32(a_ptr: int, b_ptr: int, c_ptr: int, m: int, n: int, k: int, stream:
 
 def paged_attention_status(stream: int | None = None) -> int:
     return library().mp_paged_attention_status(stream)
+
+
+def kv8_append(cache: Kv8Cache, args: Kv8AppendArgs, device_error: int | None = None, stream: int | None = None) -> None:
+    """Rotate q and k, quantise k and v, write the 8-bit pages (see mp_kv8_append)."""
+    check(library().mp_kv8_append(cache, args, device_error, stream))
+
+
+def kv8_attention_decode(cache: Kv8Cache, args: Kv8DecodeArgs, device_error: int | None = None,
+                         stream: int | None = None) -> None:
+    """Attention of one query row per sequence over the 8-bit cache (see mp_kv8_attention_decode)."""
+    check(library().mp_kv8_attention_decode(cache, args, device_error, stream))
+
+
+def kv8_attention_prefill(cache: Kv8Cache, args: Kv8PrefillArgs, device_error: int | None = None,
+                          stream: int | None = None) -> None:
+    """Causal attention of packed chunks of rows over the 8-bit cache (see mp_kv8_attention_prefill)."""
+    check(library().mp_kv8_attention_prefill(cache, args, device_error, stream))
+
+
+def kv8_decode_workspace(cache: Kv8Cache, heads: int) -> int:
+    """Bytes of the decode attention's workspace for `heads` query heads."""
+    return library().mp_kv8_decode_workspace(cache, heads)
+
+
+def kv8_prefill_workspace(cache: Kv8Cache, heads: int) -> int:
+    """Bytes of the prefill attention's workspace for `heads` query heads."""
+    return library().mp_kv8_prefill_workspace(cache, heads)
+
+
+def kv8_status(device_error: int, stream: int | None = None) -> int:
+    """Synchronises `stream`, reads and clears the error word: an MP_* code (see mp_kv8_status)."""
+    return library().mp_kv8_status(device_error, stream)
