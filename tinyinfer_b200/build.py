@@ -29,7 +29,7 @@ COMMON = ["-O3", "-std=c++17", "-lineinfo", "-Xcompiler", "-fPIC", f"-I{INCLUDE}
 COMMON += os.environ.get("MPB_NVCC_FLAGS", "").split()
 
 DEVICE_SOURCES = ["attention.cu", "attention_shared.cu", "attention_prefill.cu", "tc_gemm.cu", "fused_ops.cu", "context.cu", "operator.cu", "operator_noalloc.cu",
-                  "kv8_api.cu", "kv8_append.cu", "kv8_decode.cu"]
+                  "kv8_api.cu", "kv8_append.cu", "kv8_decode.cu", "kv8_prefill.cu"]
 HOST_SOURCES = []  # filled in by host/ when present
 
 

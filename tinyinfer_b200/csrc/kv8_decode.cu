@@ -1,85 +1,382 @@
-// mp_kv8_attention_decode: one query row per sequence over the 8-bit paged cache.
+// mp_kv8_attention_decode: one query row per sequence over the 8-bit paged cache (sm_100a).
+//
+// Bound by HBM: a token costs 2 head_dim bytes per kv head and 4 head_dim flops per query
+// head. The work is cut into units of 16 tokens of one (row, kv head, up to 8 query heads)
+// item; all items' units, in order, are dealt out in equal runs to the warps of one CTA
+// per SM, however long the sequences are. The lengths are device memory, so every CTA adds
+// them up itself (a block scan) and finds where its warps' runs begin.
+//
+// A warp is a pipeline of its own: a ring of 2 to 6 units in shared memory that bulk copies fill
+// (K and V tiles of a page are one piece, so a 16-token page is one copy) and the warp-level
+// tensor ops of kv8_warp.cuh empty. 16 warps keep up to 192 KB in flight per SM, and no two
+// warps wait for one another before the end.
+//
+// An item that ends in a later run leaves partials (max, sum, outputs): a CTA's warps join theirs
+// through shared memory, CTAs through the workspace: the last CTA to arrive on the counter of
+// the CTA in which the item began joins them in CTA order (deterministic) and clears it.
 #include "kv8_warp.cuh"
 
 namespace mpb {
 namespace kv8 {
 namespace {
 
-constexpr int kThreads = 128;
+constexpr int kCtas = 148;
+constexpr int kSmemBytes = 227 * 1024;
+constexpr int kMinUnits = 2;  // fewest units of a run: smaller launches use fewer CTAs
 
-// One warp per (row, kv head, 8 query heads), token unit by token unit.
-template <class T, int F, int D, bool kPrefill>
-__global__ void __launch_bounds__(kThreads) row_kernel(const AttentionParams p) {
-    pdl_enter();
-    const int lane = threadIdx.x & 31;
-    const int group = p.heads / p.cache.kv_heads, subs = (group + 7) / 8;
-    const int64_t item = int64_t(blockIdx.x) * (kThreads / 32) + (threadIdx.x >> 5);
-    const int per = p.cache.kv_heads * subs;
-    const int row = int(item / per), kh = int(item % per) / subs, sub = int(item % per) % subs;
-    if (row >= p.rows) return;
-    const int bt = p.cache.block_tokens;
-    int seq = row, len;
-    if constexpr (kPrefill) {
-        int before = 0;
-        for (int i = lane; i < p.count; i += 32) before += p.row_offsets[i + 1] <= row;
-        seq = __reduce_add_sync(0xffffffffu, before);
-        if (seq >= p.count) return;
-        const int begin = p.row_offsets[seq], start = p.starts[seq];
-        const int64_t end = int64_t(start) + row - begin + 1;
-        if (row < begin || start < 0 || end > int64_t(p.table_stride) * bt) {
-            if (lane == 0) raise_error(p.error, kErrBounds);
-            return;
-        }
-        len = int(end);
-    } else {
-        len = p.lengths[row];
-        if (len < 0 || len > int64_t(p.table_stride) * bt) {
-            if (lane == 0) raise_error(p.error, kErrBounds);
-            len = 0;
-        }
-    }
-    const int h0 = kh * group + sub * 8, heads = min(8, group - sub * 8);
-    WarpRow<T, F, D> w;
-    w.begin(static_cast<const T*>(p.q) + row * p.q_stride + h0 * D, heads, p.scale, lane);
-    const int32_t* table = p.tables + int64_t(seq) * p.table_stride;
-    const int n = lane >> 2, c = lane & 3;
-    for (int t = 0; t < len; t += kUnit) {
-        const int block = block_id(p.cache, table, p.table_stride, t / bt, p.error);
-        const float2 s = *reinterpret_cast<const float2*>(p.cache.scales + block * p.cache.scale_stride + 2 * kh);
-        const unsigned char* kt = p.cache.pages + tile_offset(p.cache, block, kh, 0, D) + (t % bt) * D;
-        const unsigned char* vt = kt + bt * D;
-        uint4 k[D / 64][2], v[D / 64][2];
-#pragma unroll
-        for (int h = 0; h < D / 64; ++h)
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                k[h][i] = *reinterpret_cast<const uint4*>(kt + (8 * i + n) * D + h * 64 + c * 16);
-                v[h][i] = *reinterpret_cast<const uint4*>(vt + (8 * i + n) * D + h * 64 + c * 16);
-            }
-        w.step(k, v, s.x, s.y, min(kUnit, len - t), lane);
-    }
-    w.end();
-    w.write(static_cast<T*>(p.out) + row * p.out_stride + h0 * D, heads, lane);
+template <class T, int D>
+__host__ __device__ constexpr int warps_of() {
+    return D == 64 ? 16 : sizeof(T) == 2 ? 12 : 8;  // 128, 168 and 255 registers a thread
 }
 
-template <bool kPrefill>
-cudaError_t launch(const AttentionParams& p, int type, int format, int head_dim, cudaStream_t stream) {
-    const int64_t items = int64_t(p.rows) * p.cache.kv_heads * ((p.heads / p.cache.kv_heads + 7) / 8);
-    return dispatch(type, format, head_dim, [&](auto t, auto f, auto d) {
-        return launch_pdl(row_kernel<decltype(t), decltype(f)::value, decltype(d)::value, kPrefill>,
-                          dim3(unsigned((items + 3) / 4)), dim3(kThreads), 0, stream, p);
-    });
+struct Record {  // a partial of one warp, or none (units 0)
+    int64_t first;  // device-wide index of the item's first unit
+    int row, item, units;
+    int begins, ends;  // it holds the item's first / last unit
+};
+
+// Shared memory of a CTA; `heads` = partial rows (query heads of an item, up to 8).
+struct Layout {
+    int partials, records, meta, bars, misc, total, stages;
+};
+__host__ __device__ constexpr Layout layout_of(int warps, int heads, int head_dim) {
+    Layout l{};
+    const int stage = 2 * kUnit * head_dim;
+    const int partial = heads * (head_dim + 4) * 4;
+    const int fixed = warps * 2 * partial + warps * 2 * int(sizeof(Record)) + 1024;
+    int stages = (kSmemBytes - fixed) / (warps * (stage + 16));
+    stages = stages > 6 ? 6 : stages;
+    l.stages = stages;
+    l.partials = warps * stages * stage;
+    l.records = l.partials + warps * 2 * partial;
+    l.meta = l.records + warps * 2 * int(sizeof(Record));
+    l.bars = l.meta + warps * stages * 8;
+    l.misc = l.bars + warps * stages * 8;
+    l.total = l.misc + 1024;
+    return l;
+}
+static_assert(layout_of(12, 8, 128).stages >= 2 && layout_of(16, 8, 64).stages >= 4 && layout_of(8, 8, 128).stages >= 4);
+static_assert(layout_of(12, 8, 128).total <= kSmemBytes && layout_of(16, 1, 64).total <= kSmemBytes);
+
+// A partial row of one query head: head_dim outputs, then max and sum.
+template <int D>
+struct Joined {
+    float m = -INFINITY, l = 0.f, o[D / 4];
+    __device__ __forceinline__ void clear() {
+        m = -INFINITY, l = 0.f;
+#pragma unroll
+        for (int i = 0; i < D / 4; ++i) o[i] = 0.f;
+    }
+    // lane (n, c): head n, dims h * 64 + 16 c + 0 .. 15 of each half h
+    template <bool kGlobal>
+    __device__ __forceinline__ void add(const float* slot, int heads, int lane) {
+        const int n = lane >> 2, c = lane & 3;
+        if (n >= heads) return;
+        const float* row = slot + n * (D + 4);
+        float v[D / 4];
+#pragma unroll
+        for (int i = 0; i < D / 16; ++i) {
+            const float4* at = reinterpret_cast<const float4*>(row + (i >> 2) * 64 + c * 16 + (i & 3) * 4);
+            const float4 x = kGlobal ? __ldcg(at) : *at;  // other CTAs wrote it: from L2
+            v[4 * i] = x.x, v[4 * i + 1] = x.y, v[4 * i + 2] = x.z, v[4 * i + 3] = x.w;
+        }
+        const float2* tail = reinterpret_cast<const float2*>(row + D);
+        const float2 ml = kGlobal ? __ldcg(tail) : *tail;
+        const float top = fmaxf(m, ml.x);
+        const float a = m == top ? 1.f : ex2(m - top), b = ml.x == top ? 1.f : ex2(ml.x - top);
+        l = l * a + ml.y * b;
+        m = top;
+#pragma unroll
+        for (int i = 0; i < D / 4; ++i) o[i] = fmaf(o[i], a, v[i] * b);
+    }
+    __device__ __forceinline__ void store(float* slot, int heads, int lane) const {
+        const int n = lane >> 2, c = lane & 3;
+        if (n >= heads) return;
+        float* row = slot + n * (D + 4);
+#pragma unroll
+        for (int i = 0; i < D / 16; ++i)
+            *reinterpret_cast<float4*>(row + (i >> 2) * 64 + c * 16 + (i & 3) * 4) =
+                make_float4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
+        if (c == 0) *reinterpret_cast<float2*>(row + D) = make_float2(m, l);
+    }
+    template <class T>
+    __device__ __forceinline__ void write(T* out, int heads, int lane) const {
+        const int n = lane >> 2, c = lane & 3;
+        if (n >= heads) return;
+        const float r = l == 0.f ? 0.f : 1.f / l;
+#pragma unroll
+        for (int i = 0; i < D / 16; ++i)
+            store4(out + n * D + (i >> 2) * 64 + c * 16 + (i & 3) * 4, o[4 * i] * r, o[4 * i + 1] * r, o[4 * i + 2] * r,
+                   o[4 * i + 3] * r);
+    }
+};
+
+template <class T, int F, int D>
+__global__ void __launch_bounds__(warps_of<T, D>() * 32, 1) decode_kernel(const AttentionParams p) {
+    constexpr int kWarps = warps_of<T, D>(), kThreads = kWarps * 32, kStage = 2 * kUnit * D;
+    extern __shared__ __align__(128) unsigned char smem[];
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int group = p.heads / p.cache.kv_heads, subs = (group + 7) / 8, per = p.cache.kv_heads * subs;
+    const int slots = min(group, 8);  // partial rows
+    const Layout lay = layout_of(kWarps, slots, D);
+    const int partial = slots * (D + 4);
+    unsigned char* ring = smem + warp * lay.stages * kStage;
+    float* partials = reinterpret_cast<float*>(smem + lay.partials);
+    Record* records = reinterpret_cast<Record*>(smem + lay.records);
+    float2* meta = reinterpret_cast<float2*>(smem + lay.meta) + warp * lay.stages;
+    uint64_t* bars = reinterpret_cast<uint64_t*>(smem + lay.bars) + warp * lay.stages;
+    int64_t* scan = reinterpret_cast<int64_t*>(smem + lay.misc);                  // [kWarps + 1]
+    int* first = reinterpret_cast<int*>(scan + kWarps + 1);                       // [kWarps][3] row, item, unit
+    int* joins = first + 3 * kWarps;                                              // [2] CTAs to join, 0: none
+    if (lane == 0)
+        for (int i = 0; i < lay.stages; ++i) mbar_init(bars + i, 1);
+    if (lane < 2) records[2 * warp + lane].units = 0;
+    if (tid < 2) joins[tid] = 0;
+    fence_barrier_init();
+    pdl_enter();
+
+    // ---- units of all rows, and where this CTA's warps begin
+    const int bt = p.cache.block_tokens;
+    const int64_t longest = int64_t(p.table_stride) * bt;
+    const int share = (p.count + kThreads - 1) / kThreads;
+    const int r0 = min(tid * share, p.count), r1 = min(r0 + share, p.count);
+    auto tokens = [&](int row) {
+        const int n = p.lengths[row];
+        if (n >= 0 && n <= longest) return n;
+        raise_error(p.error, kErrBounds);
+        return 0;
+    };
+    int64_t mine = 0;
+    for (int r = r0; r < r1; ++r) mine += (tokens(r) + kUnit - 1) / kUnit;
+    int64_t before = mine;  // inclusive scan over the warp
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const int64_t x = __shfl_up_sync(0xffffffffu, before, o);
+        if (lane >= o) before += x;
+    }
+    if (lane == 31) scan[warp] = before;
+    before -= mine;
+    __syncthreads();
+    int64_t total = 0;
+    for (int w = 0; w < kWarps; ++w) {
+        if (w == warp) before += total;
+        total += scan[w];
+    }
+    total *= per;
+    const int64_t want = (total + kWarps * kMinUnits - 1) / (kWarps * kMinUnits);
+    const int ctas = int(want < int64_t(gridDim.x) ? want : int64_t(gridDim.x));
+    const int64_t workers = int64_t(ctas) * kWarps;
+    // where the run of each of the CTA's warps begins, and the next CTA's first (lane = warp)
+    const int64_t starts = total * (int64_t(blockIdx.x) * kWarps + min(lane, kWarps)) / (workers ? workers : 1);
+    auto cta_of = [&](int64_t unit) { return int(((unit + 1) * workers - 1) / total / kWarps); };
+    // rows without tokens
+    for (int r = blockIdx.x; r < p.count; r += gridDim.x)
+        if (tokens(r) == 0) {
+            T* out = static_cast<T*>(p.out) + r * p.out_stride;
+            for (int i = tid; i < p.heads * D / 4; i += kThreads) store4(out + 4 * i, 0.f, 0.f, 0.f, 0.f);
+        }
+    if (int(blockIdx.x) >= ctas) return;
+    for (int w = 0; w < kWarps; ++w) {
+        const int64_t g = __shfl_sync(0xffffffffu, starts, w);
+        if (g < before * per || g >= (before + mine) * per) continue;
+        int64_t x = before;
+        for (int r = r0; r < r1; ++r) {
+            const int u = (tokens(r) + kUnit - 1) / kUnit;
+            if (g < (x + u) * per) {
+                const int in = int(g - x * per);
+                first[3 * w] = r, first[3 * w + 1] = in / u, first[3 * w + 2] = in % u;
+                break;
+            }
+            x += u;
+        }
+    }
+    __syncthreads();
+
+    // ---- this warp's run
+    const int64_t begin = __shfl_sync(0xffffffffu, starts, warp);
+    const int run = int(__shfl_sync(0xffffffffu, starts, warp + 1) - begin);
+    if (run > 0) {
+        const int in_page = bt / kUnit;
+        // producer: the next unit to copy, and a window of 32 units' addresses and scales over the lanes
+        int c_row = first[3 * warp], c_item = first[3 * warp + 1], c_unit = first[3 * warp + 2];
+        int c_units = (tokens(c_row) + kUnit - 1) / kUnit, c_left = run, w_base = -32;
+        const unsigned char* w_at = nullptr;
+        float2 w_scale{};
+        auto issue = [&](int stage) {
+            if (c_left == 0) return;
+            if (c_unit >= w_base + 32) {
+                w_base = c_unit;
+                const int u = c_unit + lane;
+                if (u < c_units && lane < c_left) {
+                    const int kh = c_item / subs;
+                    const int block = block_id(p.cache, p.tables + int64_t(c_row) * p.table_stride, p.table_stride,
+                                               u / in_page, p.error);
+                    w_scale = *reinterpret_cast<const float2*>(p.cache.scales + block * p.cache.scale_stride + 2 * kh);
+                    w_at = p.cache.pages + tile_offset(p.cache, block, kh, 0, D) + (u % in_page) * (kUnit * D);
+                }
+            }
+            if (lane == c_unit - w_base) {
+                unsigned char* to = ring + stage * kStage;
+                meta[stage] = w_scale;
+                mbar_arrive_expect_tx(bars + stage, kStage);
+                if (in_page == 1) {
+                    bulk_copy_g2s(to, w_at, kStage, bars + stage);
+                } else {
+                    bulk_copy_g2s(to, w_at, kUnit * D, bars + stage);
+                    bulk_copy_g2s(to + kUnit * D, w_at + bt * D, kUnit * D, bars + stage);
+                }
+            }
+            --c_left;
+            if (++c_unit == c_units && c_left) {
+                c_unit = 0, w_base = -32;
+                if (++c_item == per) {
+                    c_item = 0;
+                    do c_units = (tokens(++c_row) + kUnit - 1) / kUnit;
+                    while (c_units == 0);
+                }
+            }
+        };
+        for (int s = 0; s < lay.stages; ++s) issue(s);
+        __syncwarp();
+
+        int row = first[3 * warp], item = first[3 * warp + 1], unit = first[3 * warp + 2];
+        int stage = 0, emitted = 0;
+        uint32_t phase = 0;
+        bool ok = true;
+        for (int done = 0; done < run;) {
+            const int len = tokens(row), units = (len + kUnit - 1) / kUnit;
+            const int last = min(units, unit + run - done), from = unit;
+            const int kh = item / subs, sub = item % subs;
+            const int h0 = kh * group + sub * 8, heads = min(8, group - sub * 8);
+            WarpRow<T, F, D> w;
+            w.begin(static_cast<const T*>(p.q) + row * p.q_stride + h0 * D, heads, p.scale, lane);
+            for (; unit < last; ++unit) {
+                if (ok && !mbar_wait_bounded(bars + stage, phase)) {
+                    ok = false;
+                    if (lane == 0) raise_error(p.error, kErrTimeout);
+                }
+                const unsigned char* at = ring + stage * kStage + (lane >> 2) * D + (lane & 3) * 16;
+                uint4 k[D / 64][2], v[D / 64][2];
+#pragma unroll
+                for (int h = 0; h < D / 64; ++h)
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        k[h][i] = *reinterpret_cast<const uint4*>(at + 8 * i * D + h * 64);
+                        v[h][i] = *reinterpret_cast<const uint4*>(at + (kUnit + 8 * i) * D + h * 64);
+                    }
+                const float2 s = meta[stage];
+                w.step(k, v, s.x, s.y, min(kUnit, len - unit * kUnit), lane);
+                __syncwarp();
+                issue(stage);
+                if (++stage == lay.stages) stage = 0, phase ^= 1;
+            }
+            w.end();
+            done += last - from;
+            if (from == 0 && last == units) {
+                w.write(static_cast<T*>(p.out) + row * p.out_stride + h0 * D, heads, lane);
+            } else {
+                Joined<D> j;
+                j.m = w.m, j.l = w.l;
+#pragma unroll
+                for (int i = 0; i < D / 8; ++i) j.o[2 * i] = w.o[i][0], j.o[2 * i + 1] = w.o[i][1];
+                j.store(partials + (2 * warp + emitted) * partial, slots, lane);
+                if (lane == 0)
+                    records[2 * warp + emitted] = {begin + done - last, row, item, units, from == 0, last == units};
+                ++emitted;
+            }
+            unit = 0;
+            if (done < run && ++item == per) {
+                item = 0;
+                do ++row;
+                while (tokens(row) == 0);
+            }
+        }
+    }
+    __syncthreads();
+
+    // ---- join the warps' partials: the warp of an item's first record in this CTA joins them
+    float* store = reinterpret_cast<float*>(static_cast<unsigned char*>(p.workspace) + kCtas * 4 + 48);
+    unsigned* counters = static_cast<unsigned*>(p.workspace);
+    auto same = [&](const Record& a, const Record& b) { return b.units && a.row == b.row && a.item == b.item; };
+    auto output = [&](const Record& r) {
+        return static_cast<T*>(p.out) + r.row * p.out_stride + (r.item / subs * group + r.item % subs * 8) * D;
+    };
+    auto heads_of = [&](const Record& r) { return min(8, group - r.item % subs * 8); };
+    for (int k = 0; k < 2; ++k) {
+        const int index = 2 * warp + k;
+        const Record r = records[index];
+        if (!r.units) continue;
+        int previous = index - 1;
+        while (previous >= 0 && !records[previous].units) --previous;
+        if (previous >= 0 && same(r, records[previous])) continue;
+        Joined<D> j;
+        j.clear();
+        int ends = 0;
+        for (int i = index; i < 2 * kWarps; ++i) {
+            if (!records[i].units) continue;
+            if (!same(r, records[i])) break;
+            j.template add<false>(partials + i * partial, slots, lane);
+            ends = records[i].ends;
+        }
+        if (r.begins && ends) {
+            j.write(output(r), heads_of(r), lane);
+            continue;
+        }
+        // 0: the item began in an earlier CTA, 1: it begins here
+        j.store(store + (int64_t(blockIdx.x) * 2 + r.begins) * partial, slots, lane);
+        __threadfence();
+        __syncwarp();
+        if (lane == 0) {
+            const int c0 = cta_of(r.first), n = cta_of(r.first + r.units - 1) - c0 + 1;
+            if (atomicAdd(counters + c0, 1u) == unsigned(n - 1)) {
+                counters[c0] = 0;
+                joins[r.begins] = n;
+                records[index].begins = c0 + 1;  // read back below as the joining record
+                first[r.begins] = index;
+            }
+            __threadfence();
+        }
+    }
+    __syncthreads();
+
+    // ---- join the CTAs' partials, all warps at once
+    float* level = reinterpret_cast<float*>(smem);  // the rings are empty
+    for (int k = 0; k < 2; ++k) {
+        const int n = joins[k];
+        if (n == 0) continue;
+        const Record r = records[first[k]];
+        const int c0 = r.begins - 1;
+        Joined<D> j;
+        j.clear();
+        for (int i = warp; i < n; i += kWarps) j.template add<true>(store + (int64_t(c0 + i) * 2 + (i == 0)) * partial, slots, lane);
+        j.store(level + warp * partial, slots, lane);
+        __syncthreads();
+        if (warp == 0) {
+            j.clear();
+            for (int i = 0; i < min(n, kWarps); ++i) j.template add<false>(level + i * partial, slots, lane);
+            j.write(output(r), heads_of(r), lane);
+        }
+        __syncthreads();
+    }
 }
 
 }  // namespace
 
-size_t decode_workspace(int, int) { return 256; }
-size_t prefill_workspace(int, int) { return 256; }
-cudaError_t launch_decode(const AttentionParams& p, int type, int format, int head_dim, cudaStream_t stream) {
-    return launch<false>(p, type, format, head_dim, stream);
+size_t decode_workspace(int group, int head_dim) {
+    return kCtas * 4 + 48 + size_t(kCtas) * 2 * (group < 8 ? group : 8) * (head_dim + 4) * 4;
 }
-cudaError_t launch_prefill(const AttentionParams& p, int type, int format, int head_dim, cudaStream_t stream) {
-    return launch<true>(p, type, format, head_dim, stream);
+
+cudaError_t launch_decode(const AttentionParams& p, int type, int format, int head_dim, cudaStream_t stream) {
+    return dispatch(type, format, head_dim, [&](auto t, auto f, auto d) {
+        using T = decltype(t);
+        constexpr int kDim = decltype(d)::value, kWarps = warps_of<T, kDim>();
+        auto kernel = decode_kernel<T, decltype(f)::value, kDim>;
+        const int group = p.heads / p.cache.kv_heads;
+        const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes);
+        if (e != cudaSuccess) return e;
+        return launch_pdl(kernel, dim3(kCtas), dim3(kWarps * 32), size_t(layout_of(kWarps, group < 8 ? group : 8, kDim).total),
+                          stream, p);
+    });
 }
 
 }  // namespace kv8
