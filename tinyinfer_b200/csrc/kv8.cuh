@@ -3,6 +3,7 @@
 // metadata. The layout is mp_kv8_cache's (miniprefix_b200.h): a block holds, per kv
 // head, a K tile and a V tile of [block_tokens][head_dim] bytes, each with one scale.
 #pragma once
+#include <cuda.h>
 #include <cuda_bf16.h>
 
 #include "common.cuh"
@@ -49,6 +50,10 @@ struct AttentionParams {
 cudaError_t launch_append(const AppendParams& p, int type, int format, int head_dim, cudaStream_t stream);
 cudaError_t launch_decode(const AttentionParams& p, int type, int format, int head_dim, cudaStream_t stream);
 cudaError_t launch_prefill(const AttentionParams& p, int type, int format, int head_dim, cudaStream_t stream);
+// Tensor map of the cache's pages for TMA boxes of `box_rows` token rows of one tile: the
+// dimensions are (dim, kv head x K/V x slot, block), rows land in shared memory with the
+// 64- or 128-byte swizzle of their length.
+cudaError_t page_map(const Cache& cache, int head_dim, int box_rows, CUtensorMap* map);
 size_t decode_workspace(int group, int head_dim);
 size_t prefill_workspace(int group, int head_dim);
 
@@ -63,6 +68,21 @@ cudaError_t dispatch(int type, int format, int head_dim, F f) {
                                      : by_dim(t, std::integral_constant<int, MP_KV8_E4M3>{});
     };
     return type == MP_TYPE_F32 ? by_format(float{}) : by_format(__nv_bfloat16{});
+}
+
+// Bulk tensor copy of one box of page_map: token rows from `row` on, of block `block`.
+__device__ __forceinline__ void load_box(void* dst, const CUtensorMap* map, int row, int block, uint64_t* bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(
+            smem_u32(dst)),
+        "l"(map), "r"(0), "r"(row), "r"(block), "r"(smem_u32(bar))
+        : "memory");
+}
+
+// 16-byte chunk at which a box's swizzle puts chunk `chunk` of token row `row`.
+template <int D>
+__device__ __forceinline__ int swizzled(int row, int chunk) {
+    return chunk ^ (D == 128 ? row & 7 : (row >> 1) & 3);
 }
 
 // Byte offset of the K (part 0) or V (part 1) tile of (block, kv head).
@@ -107,6 +127,21 @@ __device__ __forceinline__ void widen4(uint32_t w, uint32_t& lo, uint32_t& hi) {
     }
 }
 
+// The same for a word of codes a0 a1 b0 b1 (two dims of tokens a and b): (a0, b0), (a1, b1).
+template <int F>
+__device__ __forceinline__ void widen_pairs(uint32_t w, uint32_t& first, uint32_t& second) {
+    if constexpr (F == MP_KV8_INT8) {
+        const uint32_t u = w ^ 0x80808080u;
+        const __half2 off = __half2half2(__ushort_as_half(0x6480));
+        uint32_t a = __byte_perm(u, 0x64646464u, 0x4240), b = __byte_perm(u, 0x64646464u, 0x4341);
+        __half2 x = __hsub2(*reinterpret_cast<__half2*>(&a), off), y = __hsub2(*reinterpret_cast<__half2*>(&b), off);
+        first = *reinterpret_cast<uint32_t*>(&x);
+        second = *reinterpret_cast<uint32_t*>(&y);
+    } else {
+        widen4<F>(__byte_perm(w, 0, 0x3120), first, second);
+    }
+}
+
 // FP16 halves of two values, packed: hi = fp16(x), lo = fp16(x - hi). Callers scale
 // their values so that the largest are near 2^14: lo then keeps 11 bits of its own down
 // to values 2^-26 of the largest, and hi + lo is x within 2^-22 |x|.
@@ -146,6 +181,15 @@ __device__ __forceinline__ uint32_t transpose8x8(uint32_t a) {
     uint32_t d;
     asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(a));
     return d;
+}
+
+// Four 8 x 8 matrices of 16-bit elements from shared memory, transposed: lane l gives
+// the address of row l % 8 of matrix l / 8.
+__device__ __forceinline__ void load_transposed(uint32_t (&r)[4], uint32_t address) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                 : "r"(address)
+                 : "memory");
 }
 
 __device__ __forceinline__ void load4(const float* p, float (&v)[4]) {

@@ -1,14 +1,13 @@
 // mp_kv8_attention_decode: one query row per sequence over the 8-bit paged cache (sm_100a).
 //
 // Bound by HBM: a token costs 2 head_dim bytes per kv head and 4 head_dim flops per query
-// head. The work is cut into units of 16 tokens of one (row, kv head, up to 8 query heads)
+// head. The work is cut into units of 32 tokens of one (row, kv head, up to 8 query heads)
 // item; all items' units, in order, are dealt out in equal runs to the warps of one CTA
 // per SM, however long the sequences are. The lengths are device memory, so every CTA adds
 // them up itself (a block scan) and finds where its warps' runs begin.
 //
-// A warp is a pipeline of its own: a ring of 2 to 6 units in shared memory that bulk copies fill
-// (K and V tiles of a page are one piece, so a 16-token page is one copy) and the warp-level
-// tensor ops of kv8_warp.cuh empty. 16 warps keep up to 192 KB in flight per SM, and no two
+// A warp is a pipeline of its own: a ring of units in shared memory that tensor copies fill
+// (K and V tiles of a page are one piece, so a 16-token page is one box; its rows are swizzled against bank conflicts) and the warp-level tensor ops of kv8_warp.cuh empty. 16 warps keep up to 192 KB in flight per SM, and no two
 // warps wait for one another before the end.
 //
 // An item that ends in a later run leaves partials (max, sum, outputs): a CTA's warps join theirs
@@ -22,7 +21,7 @@ namespace {
 
 constexpr int kCtas = 148;
 constexpr int kSmemBytes = 227 * 1024;
-constexpr int kMinUnits = 2;  // fewest units of a run: smaller launches use fewer CTAs
+constexpr int kMinUnits = 4;  // units per warp before another CTA takes part: joining CTAs costs more
 
 template <class T, int D>
 __host__ __device__ constexpr int warps_of() {
@@ -41,21 +40,21 @@ struct Layout {
 };
 __host__ __device__ constexpr Layout layout_of(int warps, int heads, int head_dim) {
     Layout l{};
-    const int stage = 2 * kUnit * head_dim;
+    const int stage = 2 * kUnit * head_dim;  // [tile][K, V][16 tokens][head_dim]
     const int partial = heads * (head_dim + 4) * 4;
     const int fixed = warps * 2 * partial + warps * 2 * int(sizeof(Record)) + 1024;
-    int stages = (kSmemBytes - fixed) / (warps * (stage + 16));
-    stages = stages > 6 ? 6 : stages;
+    int stages = (kSmemBytes - fixed) / (warps * (stage + kTiles * 8 + 8));
+    stages = stages > 3 ? 3 : stages;
     l.stages = stages;
     l.partials = warps * stages * stage;
     l.records = l.partials + warps * 2 * partial;
     l.meta = l.records + warps * 2 * int(sizeof(Record));
-    l.bars = l.meta + warps * stages * 8;
+    l.bars = l.meta + warps * stages * kTiles * 8;
     l.misc = l.bars + warps * stages * 8;
     l.total = l.misc + 1024;
     return l;
 }
-static_assert(layout_of(12, 8, 128).stages >= 2 && layout_of(16, 8, 64).stages >= 4 && layout_of(8, 8, 128).stages >= 4);
+static_assert(layout_of(12, 8, 128).stages >= 1 && layout_of(16, 8, 64).stages >= 2 && layout_of(8, 8, 128).stages >= 2);
 static_assert(layout_of(12, 8, 128).total <= kSmemBytes && layout_of(16, 1, 64).total <= kSmemBytes);
 
 // A partial row of one query head: head_dim outputs, then max and sum.
@@ -67,7 +66,7 @@ struct Joined {
 #pragma unroll
         for (int i = 0; i < D / 4; ++i) o[i] = 0.f;
     }
-    // lane (n, c): head n, dims h * 64 + 16 c + 0 .. 15 of each half h
+    // lane (n, c): head n, dims 16 i + 4 c + 0 .. 3
     template <bool kGlobal>
     __device__ __forceinline__ void add(const float* slot, int heads, int lane) {
         const int n = lane >> 2, c = lane & 3;
@@ -76,7 +75,7 @@ struct Joined {
         float v[D / 4];
 #pragma unroll
         for (int i = 0; i < D / 16; ++i) {
-            const float4* at = reinterpret_cast<const float4*>(row + (i >> 2) * 64 + c * 16 + (i & 3) * 4);
+            const float4* at = reinterpret_cast<const float4*>(row + 16 * i + 4 * c);
             const float4 x = kGlobal ? __ldcg(at) : *at;  // other CTAs wrote it: from L2
             v[4 * i] = x.x, v[4 * i + 1] = x.y, v[4 * i + 2] = x.z, v[4 * i + 3] = x.w;
         }
@@ -95,7 +94,7 @@ struct Joined {
         float* row = slot + n * (D + 4);
 #pragma unroll
         for (int i = 0; i < D / 16; ++i)
-            *reinterpret_cast<float4*>(row + (i >> 2) * 64 + c * 16 + (i & 3) * 4) =
+            *reinterpret_cast<float4*>(row + 16 * i + 4 * c) =
                 make_float4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
         if (c == 0) *reinterpret_cast<float2*>(row + D) = make_float2(m, l);
     }
@@ -106,15 +105,16 @@ struct Joined {
         const float r = l == 0.f ? 0.f : 1.f / l;
 #pragma unroll
         for (int i = 0; i < D / 16; ++i)
-            store4(out + n * D + (i >> 2) * 64 + c * 16 + (i & 3) * 4, o[4 * i] * r, o[4 * i + 1] * r, o[4 * i + 2] * r,
+            store4(out + n * D + 16 * i + 4 * c, o[4 * i] * r, o[4 * i + 1] * r, o[4 * i + 2] * r,
                    o[4 * i + 3] * r);
     }
 };
 
 template <class T, int F, int D>
-__global__ void __launch_bounds__(warps_of<T, D>() * 32, 1) decode_kernel(const AttentionParams p) {
+__global__ void __launch_bounds__(warps_of<T, D>() * 32, 1)
+    decode_kernel(const AttentionParams p, const __grid_constant__ CUtensorMap pages) {
     constexpr int kWarps = warps_of<T, D>(), kThreads = kWarps * 32, kStage = 2 * kUnit * D;
-    extern __shared__ __align__(128) unsigned char smem[];
+    extern __shared__ __align__(1024) unsigned char smem[];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int group = p.heads / p.cache.kv_heads, subs = (group + 7) / 8, per = p.cache.kv_heads * subs;
     const int slots = min(group, 8);  // partial rows
@@ -123,7 +123,7 @@ __global__ void __launch_bounds__(warps_of<T, D>() * 32, 1) decode_kernel(const 
     unsigned char* ring = smem + warp * lay.stages * kStage;
     float* partials = reinterpret_cast<float*>(smem + lay.partials);
     Record* records = reinterpret_cast<Record*>(smem + lay.records);
-    float2* meta = reinterpret_cast<float2*>(smem + lay.meta) + warp * lay.stages;
+    float2* meta = reinterpret_cast<float2*>(smem + lay.meta) + warp * lay.stages * kTiles;
     uint64_t* bars = reinterpret_cast<uint64_t*>(smem + lay.bars) + warp * lay.stages;
     int64_t* scan = reinterpret_cast<int64_t*>(smem + lay.misc);                  // [kWarps + 1]
     int* first = reinterpret_cast<int*>(scan + kWarps + 1);                       // [kWarps][3] row, item, unit
@@ -196,43 +196,45 @@ __global__ void __launch_bounds__(warps_of<T, D>() * 32, 1) decode_kernel(const 
     const int64_t begin = __shfl_sync(0xffffffffu, starts, warp);
     const int run = int(__shfl_sync(0xffffffffu, starts, warp + 1) - begin);
     if (run > 0) {
-        const int in_page = bt / kUnit;
-        // producer: the next unit to copy, and a window of 32 units' addresses and scales over the lanes
+        const int in_page = bt / kTile;
+        // producer: the next unit to copy, and a window of 32 tiles (block, row, scales) over the lanes
         int c_row = first[3 * warp], c_item = first[3 * warp + 1], c_unit = first[3 * warp + 2];
-        int c_units = (tokens(c_row) + kUnit - 1) / kUnit, c_left = run, w_base = -32;
-        const unsigned char* w_at = nullptr;
+        int c_len = tokens(c_row), c_left = run, w_base = -32;
+        int w_block = 0, w_at = 0;
         float2 w_scale{};
         auto issue = [&](int stage) {
             if (c_left == 0) return;
-            if (c_unit >= w_base + 32) {
-                w_base = c_unit;
-                const int u = c_unit + lane;
-                if (u < c_units && lane < c_left) {
+            if (kTiles * c_unit >= w_base + 32) {
+                w_base = kTiles * c_unit;
+                const int tile = w_base + lane;
+                w_scale = make_float2(0.f, 0.f);
+                if (tile * kTile < c_len && lane < kTiles * c_left) {
                     const int kh = c_item / subs;
-                    const int block = block_id(p.cache, p.tables + int64_t(c_row) * p.table_stride, p.table_stride,
-                                               u / in_page, p.error);
-                    w_scale = *reinterpret_cast<const float2*>(p.cache.scales + block * p.cache.scale_stride + 2 * kh);
-                    w_at = p.cache.pages + tile_offset(p.cache, block, kh, 0, D) + (u % in_page) * (kUnit * D);
+                    w_block = block_id(p.cache, p.tables + int64_t(c_row) * p.table_stride, p.table_stride, tile / in_page,
+                                       p.error);
+                    w_scale = *reinterpret_cast<const float2*>(p.cache.scales + w_block * p.cache.scale_stride + 2 * kh);
+                    w_at = kh * 2 * bt + tile % in_page * kTile;
                 }
             }
-            if (lane == c_unit - w_base) {
-                unsigned char* to = ring + stage * kStage;
-                meta[stage] = w_scale;
-                mbar_arrive_expect_tx(bars + stage, kStage);
-                if (in_page == 1) {
-                    bulk_copy_g2s(to, w_at, kStage, bars + stage);
-                } else {
-                    bulk_copy_g2s(to, w_at, kUnit * D, bars + stage);
-                    bulk_copy_g2s(to + kUnit * D, w_at + bt * D, kUnit * D, bars + stage);
+            const int mine = lane + w_base - kTiles * c_unit;  // this lane's tile of the unit, if it has one
+            const bool both = (kTiles * c_unit + 1) * kTile < c_len;
+            if (mine == 0) mbar_arrive_expect_tx(bars + stage, both ? kStage : kStage / 2);
+            __syncwarp();
+            if (mine == 0 || mine == 1) {
+                meta[kTiles * stage + mine] = w_scale;
+                if (mine == 0 || both) {
+                    unsigned char* to = ring + stage * kStage + mine * (kStage / 2);
+                    load_box(to, &pages, w_at, w_block, bars + stage);
+                    if (in_page > 1) load_box(to + kTile * D, &pages, w_at + bt, w_block, bars + stage);
                 }
             }
             --c_left;
-            if (++c_unit == c_units && c_left) {
+            if (++c_unit * kUnit >= c_len && c_left) {
                 c_unit = 0, w_base = -32;
                 if (++c_item == per) {
                     c_item = 0;
-                    do c_units = (tokens(++c_row) + kUnit - 1) / kUnit;
-                    while (c_units == 0);
+                    do c_len = tokens(++c_row);
+                    while (c_len == 0);
                 }
             }
         };
@@ -240,6 +242,8 @@ __global__ void __launch_bounds__(warps_of<T, D>() * 32, 1) decode_kernel(const 
         __syncwarp();
 
         int row = first[3 * warp], item = first[3 * warp + 1], unit = first[3 * warp + 2];
+        const int k_row = WarpRow<T, F, D>::token(0, lane >> 2);                    // and 8 rows on
+        const int v_row = WarpRow<T, F, D>::token((lane >> 3) & 1, lane & 7);       // this lane's matrix row
         int stage = 0, emitted = 0;
         uint32_t phase = 0;
         bool ok = true;
@@ -255,17 +259,21 @@ __global__ void __launch_bounds__(warps_of<T, D>() * 32, 1) decode_kernel(const 
                     ok = false;
                     if (lane == 0) raise_error(p.error, kErrTimeout);
                 }
-                const unsigned char* at = ring + stage * kStage + (lane >> 2) * D + (lane & 3) * 16;
-                uint4 k[D / 64][2], v[D / 64][2];
+                const unsigned char* at = ring + stage * kStage;
+                auto load_k = [&](int u, int i, uint4 (&k)[D / 64]) {
 #pragma unroll
-                for (int h = 0; h < D / 64; ++h)
+                    for (int h = 0; h < D / 64; ++h)
+                        k[h] = *reinterpret_cast<const uint4*>(at + (2 * u * kTile + k_row + 8 * i) * D +
+                                                               swizzled<D>(k_row, 4 * h + (lane & 3)) * 16);
+                };
+                const uint32_t v_at = smem_u32(at) + (kTile + v_row) * D;
+                auto load_v = [&](int u, int q, uint32_t (&r)[4]) {
+                    load_transposed(r, v_at + 2 * u * kTile * D + swizzled<D>(v_row, 2 * q + (lane >> 4)) * 16);
+                };
+                float2 scale[kTiles];
 #pragma unroll
-                    for (int i = 0; i < 2; ++i) {
-                        k[h][i] = *reinterpret_cast<const uint4*>(at + 8 * i * D + h * 64);
-                        v[h][i] = *reinterpret_cast<const uint4*>(at + (kUnit + 8 * i) * D + h * 64);
-                    }
-                const float2 s = meta[stage];
-                w.step(k, v, s.x, s.y, min(kUnit, len - unit * kUnit), lane);
+                for (int u = 0; u < kTiles; ++u) scale[u] = meta[kTiles * stage + u];
+                w.step(load_k, load_v, scale, min(kUnit, len - unit * kUnit), lane);
                 __syncwarp();
                 issue(stage);
                 if (++stage == lay.stages) stage = 0, phase ^= 1;
@@ -278,7 +286,7 @@ __global__ void __launch_bounds__(warps_of<T, D>() * 32, 1) decode_kernel(const 
                 Joined<D> j;
                 j.m = w.m, j.l = w.l;
 #pragma unroll
-                for (int i = 0; i < D / 8; ++i) j.o[2 * i] = w.o[i][0], j.o[2 * i + 1] = w.o[i][1];
+                for (int i = 0; i < D / 8; ++i) j.o[4 * (i / 2) + i % 2] = w.o[i][0], j.o[4 * (i / 2) + i % 2 + 2] = w.o[i][1];
                 j.store(partials + (2 * warp + emitted) * partial, slots, lane);
                 if (lane == 0)
                     records[2 * warp + emitted] = {begin + done - last, row, item, units, from == 0, last == units};
@@ -372,10 +380,12 @@ cudaError_t launch_decode(const AttentionParams& p, int type, int format, int he
         constexpr int kDim = decltype(d)::value, kWarps = warps_of<T, kDim>();
         auto kernel = decode_kernel<T, decltype(f)::value, kDim>;
         const int group = p.heads / p.cache.kv_heads;
-        const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes);
+        CUtensorMap pages;
+        cudaError_t e = page_map(p.cache, kDim, p.cache.block_tokens == kTile ? 2 * kTile : kTile, &pages);
+        if (e == cudaSuccess) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes);
         if (e != cudaSuccess) return e;
         return launch_pdl(kernel, dim3(kCtas), dim3(kWarps * 32), size_t(layout_of(kWarps, group < 8 ? group : 8, kDim).total),
-                          stream, p);
+                          stream, p, pages);
     });
 }
 

@@ -35,19 +35,30 @@ __global__ void __launch_bounds__(kThreads) row_kernel(const AttentionParams p) 
     const int32_t* table = p.tables + int64_t(seq) * p.table_stride;
     const int n = lane >> 2, c = lane & 3;
     for (int t = 0; t < len; t += kUnit) {
-        const int block = block_id(p.cache, table, p.table_stride, t / bt, p.error);
-        const float2 s = *reinterpret_cast<const float2*>(p.cache.scales + block * p.cache.scale_stride + 2 * kh);
-        const unsigned char* kt = p.cache.pages + tile_offset(p.cache, block, kh, 0, D) + (t % bt) * D;
-        const unsigned char* vt = kt + bt * D;
-        uint4 k[D / 64][2], v[D / 64][2];
+        const unsigned char* at[kTiles];
+        float2 scale[kTiles];
 #pragma unroll
-        for (int h = 0; h < D / 64; ++h)
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                k[h][i] = *reinterpret_cast<const uint4*>(kt + (8 * i + n) * D + h * 64 + c * 16);
-                v[h][i] = *reinterpret_cast<const uint4*>(vt + (8 * i + n) * D + h * 64 + c * 16);
+        for (int u = 0; u < kTiles; ++u) {
+            const int token = t + u * kTile;
+            scale[u] = make_float2(0.f, 0.f);
+            at[u] = at[0];
+            if (token < len) {
+                const int block = block_id(p.cache, table, p.table_stride, token / bt, p.error);
+                scale[u] = *reinterpret_cast<const float2*>(p.cache.scales + block * p.cache.scale_stride + 2 * kh);
+                at[u] = p.cache.pages + tile_offset(p.cache, block, kh, 0, D) + (token % bt) * D;
             }
-        w.step(k, v, s.x, s.y, min(kUnit, len - t), lane);
+        }
+        auto load_k = [&](int u, int i, uint4 (&k)[D / 64]) {
+#pragma unroll
+            for (int h = 0; h < D / 64; ++h) k[h] = *reinterpret_cast<const uint4*>(at[u] + w.token(i, n) * D + h * 64 + c * 16);
+        };
+        auto load_v = [&](int u, int q, uint32_t (&r)[4]) {
+#pragma unroll
+            for (int g = 0; g < 4; ++g)
+                r[g] = transpose8x8(*reinterpret_cast<const uint32_t*>(at[u] + (bt + w.token(g & 1, n)) * D + 32 * q +
+                                                                       16 * (g >> 1) + 4 * c));
+        };
+        w.step(load_k, load_v, scale, min(kUnit, len - t), lane);
     }
     w.end();
     w.write(static_cast<T*>(p.out) + row * p.out_stride + h0 * D, heads, lane);

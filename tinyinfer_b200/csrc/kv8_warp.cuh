@@ -1,5 +1,6 @@
 // Attention of one query row (up to 8 query heads of one kv head) by one warp over
-// units of 16 tokens of the 8-bit cache, on warp-level tensor ops (sm_100a).
+// units of 32 tokens (two tiles of 16, each in one block) of the 8-bit cache, on
+// warp-level tensor ops (sm_100a).
 //
 // Scores: S = Q K^T as m16n8k16 products. Rows 0..7 of A are the FP16 high halves of
 // the 8 heads' queries, rows 8..15 their low halves; B's columns are 8 tokens. The codes
@@ -7,11 +8,14 @@
 // c) = (lane / 4, lane % 4) holds B's column n: the 16 bytes c of token n's row (the K
 // dimension is permuted the same way in A, so each lane's load is one 16-byte word).
 // Weights: lane (n, c) then owns head n's scores of tokens 2c, 2c + 1 of each 8, which is
-// the A layout of the second product, P V; V, read like K, is transposed by movmatrix.
+// the A layout of the second product, P V. Its B wants two tokens of one dim side by side:
+// V's bytes are read as 16-bit elements (two dims) in transposed 8 x 8 matrices, which gives
+// a lane two dims of two tokens. (A first version transposed the widened halves with
+// movmatrix: the pipe that it shares with exp2 took 660 cycles a unit, four times the rest.)
 // V's block scale is folded into the weights.
 //
-// Tensor-op sums are cut, not rounded: each added unit loses about 2^-25.7 of the sum
-// (measured: 1.8e-5 after 1000 units). FP32 outputs therefore add the products up in
+// Tensor-op sums are cut, not rounded: each added tile loses about 2^-25.7 of the sum
+// (measured: 1.8e-5 after 1000 tiles). FP32 outputs therefore add the products up in
 // chains of kChain units and the chains in FP32 registers.
 //
 // The state is a running softmax: m (largest score), l (sum of weights), and outputs in
@@ -23,8 +27,10 @@
 namespace mpb {
 namespace kv8 {
 
-constexpr int kUnit = 16;                  // tokens of a unit
-constexpr int kChain = 8;                  // units per chain of tensor-op sums (FP32 outputs)
+constexpr int kTile = 16;                  // tokens of a tile: the K of one product
+constexpr int kTiles = 2;                  // tiles of a unit: their products overlap, and votes and shuffles halve
+constexpr int kUnit = kTile * kTiles;
+constexpr int kChain = 4;                  // units per chain of tensor-op sums (FP32 outputs)
 constexpr float kWeightTop = 4096.f;       // weights are at most 2^12 in FP16
 constexpr float kUnitFloor = 7.7e-34f;     // 2^-110: below every scale the append makes
 
@@ -33,10 +39,16 @@ struct WarpRow {
     static constexpr int kHalves = D / 64;
     static constexpr bool kSplit = sizeof(T) == 4;  // BF16 outputs: weights as one FP16 half (2^-12 relative)
     uint32_t qa[D / 16][4];
-    float o[D / 8][4];  // [tile][0, 1: hi rows; 2, 3: lo rows]
+    // outputs: lane (n, c) holds head n's dims 16 i / 2 + 4 c + i % 2 + {0, 2} in o[i][0, 1]
+    // (weights' hi halves) and o[i][2, 3] (lo)
+    float o[D / 8][4];
     float sum[kSplit ? D / 8 : 1][2];  // finished chains
     float m, l, unit, inv_unit, k_factor;
     int chain;
+
+    // Token of column x of 8 in half `i` of a tile. 128-byte rows: columns 2i and 2i + 1 are
+    // four rows apart, so that the swizzled chunks which 8 lanes read lie in different banks.
+    static __device__ __forceinline__ int token(int i, int x) { return 8 * i + (D == 128 ? (x >> 1) + 4 * (x & 1) : x); }
 
     // Query heads h0 .. h0 + heads - 1 at `q` (head stride D); absent heads are zero.
     __device__ __forceinline__ void begin(const T* q, int heads, float scale, int lane) {
@@ -67,85 +79,113 @@ struct WarpRow {
         m = -INFINITY, l = 0.f, unit = kUnitFloor, inv_unit = kWeightTop / kUnitFloor, chain = 0;
     }
 
-    // One unit. k, v: [half][token n, token 8 + n] 16-byte words of this lane; tokens at
-    // or past `valid` (1 .. 16) are masked.
-    __device__ __forceinline__ void step(uint4 (&k)[kHalves][2], uint4 (&v)[kHalves][2], float ks, float vs, int valid,
-                                         int lane) {
+    // One unit. load_k(u, i, k): the 16-byte words c of every 64-byte half of token(i, n)'s row
+    // in tile u; load_v(u, q, r): dims 32 q .. 32 q + 31 of V's tile u as four transposed
+    // matrices, r[2 a + i] = chunk 2 q + a of the tokens of half i; scale[u]: the K and V
+    // scales. Tokens at or past `valid` (1 .. 32) are masked (a tile without tokens has
+    // scales 0).
+    template <class LoadK, class LoadV>
+    __device__ __forceinline__ void step(LoadK load_k, LoadV load_v, const float2 (&scale)[kTiles], int valid, int lane) {
         const int n = lane >> 2, c = lane & 3;
-        if (valid < kUnit) {  // bytes behind the last token may be NaN codes
+        float t[kTiles][2][2];
 #pragma unroll
-            for (int i = 0; i < 2; ++i)
-                if (8 * i + n >= valid) {
+        for (int u = 0; u < kTiles; ++u) {
+            const float f = k_factor * scale[u].x;
 #pragma unroll
-                    for (int h = 0; h < kHalves; ++h) k[h][i] = v[h][i] = make_uint4(0, 0, 0, 0);
+            for (int i = 0; i < 2; ++i) {
+                uint4 k[kHalves];
+                load_k(u, i, k);
+                if (valid < kUnit && u * kTile + token(i, n) >= valid) {  // bytes behind the last token may be NaN codes
+#pragma unroll
+                    for (int h = 0; h < kHalves; ++h) k[h] = make_uint4(0, 0, 0, 0);
                 }
-        }
-        float s[2][2];
+                float acc[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            float acc[4] = {0.f, 0.f, 0.f, 0.f};
+                for (int h = 0; h < kHalves; ++h) {
+                    const uint32_t w[4] = {k[h].x, k[h].y, k[h].z, k[h].w};
 #pragma unroll
-            for (int h = 0; h < kHalves; ++h) {
-                const uint32_t w[4] = {k[h][i].x, k[h][i].y, k[h][i].z, k[h][i].w};
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    uint32_t b0, b1;
-                    widen4<F>(w[j], b0, b1);
-                    mma16816(acc, qa[4 * h + j], b0, b1);
+                    for (int j = 0; j < 4; ++j) {
+                        uint32_t b0, b1;
+                        widen4<F>(w[j], b0, b1);
+                        mma16816(acc, qa[4 * h + j], b0, b1);
+                    }
                 }
+                t[u][i][0] = (acc[0] + acc[2]) * f;
+                t[u][i][1] = (acc[1] + acc[3]) * f;
             }
-            s[i][0] = acc[0] + acc[2];
-            s[i][1] = acc[1] + acc[3];
         }
-        const float f = k_factor * ks;
-        float top = -INFINITY;
+        auto live = [&](int u, int i, int j) { return u * kTile + token(i, 2 * c + j) < valid; };
+        if (valid < kUnit) {
 #pragma unroll
-        for (int i = 0; i < 2; ++i)
+            for (int u = 0; u < kTiles; ++u)
 #pragma unroll
-            for (int j = 0; j < 2; ++j) top = fmaxf(top, 8 * i + 2 * c + j < valid ? s[i][j] * f : -INFINITY);
+                for (int i = 0; i < 2; ++i)
+#pragma unroll
+                    for (int j = 0; j < 2; ++j) t[u][i][j] = live(u, i, j) ? t[u][i][j] : -INFINITY;
+        }
+        float tops[kTiles], top = -INFINITY, most = 0.f;
+#pragma unroll
+        for (int u = 0; u < kTiles; ++u) {
+            tops[u] = fmaxf(fmaxf(t[u][0][0], t[u][0][1]), fmaxf(t[u][1][0], t[u][1][1]));
+            top = fmaxf(top, tops[u]);
+            most = fmaxf(most, scale[u].y);
+        }
         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-        const float m_new = fmaxf(m, top);
-        const float reach = m_new == -INFINITY ? 0.f : vs * ex2(top - m_new);  // largest weight times scale here
-        if (__any_sync(0xffffffffu, top > m || reach > unit)) {
-            const float decay = m_new == -INFINITY ? 1.f : ex2(m - m_new);
-            const float unit_new = fmaxf(fmaxf(unit * decay, reach), kUnitFloor);
-            const float move = decay * unit / unit_new;
-            l *= decay;
+        if (__any_sync(0xffffffffu, top > m || most > unit)) {
+            const float m_new = fmaxf(m, top);
+            float reach = 0.f;  // largest weight times scale of the unit
 #pragma unroll
-            for (int i = 0; i < D / 8; ++i) {
+            for (int u = 0; u < kTiles; ++u) reach = fmaxf(reach, tops[u] == -INFINITY ? 0.f : scale[u].y * ex2(tops[u] - m_new));
+            reach = fmaxf(reach, __shfl_xor_sync(0xffffffffu, reach, 1));
+            reach = fmaxf(reach, __shfl_xor_sync(0xffffffffu, reach, 2));
+            if (__any_sync(0xffffffffu, top > m || reach > unit)) {
+                const float decay = m_new == -INFINITY ? 1.f : ex2(m - m_new);
+                const float unit_new = fmaxf(fmaxf(unit * decay, reach), kUnitFloor);
+                const float move = decay * unit / unit_new;
+                l *= decay;
 #pragma unroll
-                for (int j = 0; j < 4; ++j) o[i][j] *= move;
-                if constexpr (kSplit) sum[i][0] *= move, sum[i][1] *= move;
-            }
-            m = m_new, unit = unit_new, inv_unit = kWeightTop / unit_new;
-        }
-        const float base = m == -INFINITY ? 0.f : m, w = vs * inv_unit;
-        uint32_t a[4];
+                for (int i = 0; i < D / 8; ++i) {
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            const float p0 = 8 * i + 2 * c < valid ? ex2(fmaf(s[i][0], f, -base)) : 0.f;
-            const float p1 = 8 * i + 2 * c + 1 < valid ? ex2(fmaf(s[i][1], f, -base)) : 0.f;
-            l += p0 + p1;
-            if constexpr (kSplit) {
-                split_pair(p0 * w, p1 * w, a[2 * i], a[2 * i + 1]);
-            } else {
-                const __half2 h = __floats2half2_rn(p0 * w, p1 * w);
-                a[2 * i] = *reinterpret_cast<const uint32_t*>(&h);
-                a[2 * i + 1] = 0;
+                    for (int j = 0; j < 4; ++j) o[i][j] *= move;
+                    if constexpr (kSplit) sum[i][0] *= move, sum[i][1] *= move;
+                }
+                m = m_new, unit = unit_new, inv_unit = kWeightTop / unit_new;
             }
         }
+        const float base = m == -INFINITY ? 0.f : m;
 #pragma unroll
-        for (int h = 0; h < kHalves; ++h) {
-            const uint32_t w0[4] = {v[h][0].x, v[h][0].y, v[h][0].z, v[h][0].w};
-            const uint32_t w1[4] = {v[h][1].x, v[h][1].y, v[h][1].z, v[h][1].w};
+        for (int u = 0; u < kTiles; ++u) {
+            const float w = scale[u].y * inv_unit;
+            uint32_t a[4];
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                uint32_t x0, x1, y0, y1;
-                widen4<F>(w0[j], x0, x1);
-                widen4<F>(w1[j], y0, y1);
-                mma16816(o[8 * h + 2 * j], a, transpose8x8(x0), transpose8x8(y0));
-                mma16816(o[8 * h + 2 * j + 1], a, transpose8x8(x1), transpose8x8(y1));
+            for (int i = 0; i < 2; ++i) {
+                const float p0 = ex2(t[u][i][0] - base), p1 = ex2(t[u][i][1] - base);
+                l += p0 + p1;
+                if constexpr (kSplit) {
+                    split_pair(p0 * w, p1 * w, a[2 * i], a[2 * i + 1]);
+                } else {
+                    const __half2 h = __floats2half2_rn(p0 * w, p1 * w);
+                    a[2 * i] = *reinterpret_cast<const uint32_t*>(&h);
+                    a[2 * i + 1] = 0;
+                }
+            }
+            uint32_t keep[2];
+#pragma unroll
+            for (int i = 0; i < 2; ++i) keep[i] = (live(u, i, 0) ? 0xffffu : 0u) | (live(u, i, 1) ? 0xffff0000u : 0u);
+#pragma unroll
+            for (int q = 0; q < D / 32; ++q) {
+                uint32_t r[4];
+                load_v(u, q, r);
+                if (valid < kUnit) r[0] &= keep[0], r[1] &= keep[1], r[2] &= keep[0], r[3] &= keep[1];
+#pragma unroll
+                for (int g = 0; g < 2; ++g) {
+                    uint32_t x0, x1, y0, y1;
+                    widen_pairs<F>(r[2 * g], x0, x1);
+                    widen_pairs<F>(r[2 * g + 1], y0, y1);
+                    mma16816(o[4 * q + 2 * g], a, x0, y0);
+                    mma16816(o[4 * q + 2 * g + 1], a, x1, y1);
+                }
             }
         }
         if constexpr (kSplit) {
@@ -165,9 +205,8 @@ struct WarpRow {
         }
     }
 
-    // Sum of weights over the head's lanes; o[..][0, 1] become the head's outputs in plain
-    // units (unnormalised). Afterwards lane (n, c) holds head n's dims
-    // (i / 8) * 64 + 16 c + 2 (i % 8) + {0, 1} in o[i][0, 1].
+    // Sum of weights over the head's lanes; o[i][0, 1] become the head's outputs in plain
+    // units (unnormalised).
     __device__ __forceinline__ void end() {
         l += __shfl_xor_sync(0xffffffffu, l, 1);
         l += __shfl_xor_sync(0xffffffffu, l, 2);
@@ -187,8 +226,7 @@ struct WarpRow {
         const float r = l == 0.f ? 0.f : 1.f / l;
 #pragma unroll
         for (int i = 0; i < D / 8; i += 2)
-            store4(out + n * D + (i >> 3) * 64 + c * 16 + (i & 7) * 2, o[i][0] * r, o[i][1] * r, o[i + 1][0] * r,
-                   o[i + 1][1] * r);
+            store4(out + n * D + 8 * i + 4 * c, o[i][0] * r, o[i + 1][0] * r, o[i][1] * r, o[i + 1][1] * r);
     }
 };
 
