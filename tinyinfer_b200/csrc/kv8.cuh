@@ -71,10 +71,10 @@ cudaError_t dispatch(int type, int format, int head_dim, F f) {
 }
 
 // Bulk tensor copy of one box of page_map: token rows from `row` on, of block `block`.
-__device__ __forceinline__ void load_box(void* dst, const CUtensorMap* map, int row, int block, uint64_t* bar) {
+__device__ __forceinline__ void load_box(uint32_t dst, const CUtensorMap* map, int row, int block, uint64_t* bar) {
     asm volatile(
         "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(
-            smem_u32(dst)),
+            dst),
         "l"(map), "r"(0), "r"(row), "r"(block), "r"(smem_u32(bar))
         : "memory");
 }
@@ -170,8 +170,7 @@ __device__ __forceinline__ void row_factor(float amax, float& factor, float& inv
 
 // D (16 x 8, FP32) += A (16 x 16) B (16 x 8), FP16 operands (warp-level tensor op).
 __device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-    asm volatile(
-        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
         : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
@@ -184,12 +183,12 @@ __device__ __forceinline__ uint32_t transpose8x8(uint32_t a) {
 }
 
 // Four 8 x 8 matrices of 16-bit elements from shared memory, transposed: lane l gives
-// the address of row l % 8 of matrix l / 8.
+// the address of row l % 8 of matrix l / 8. Volatile, so that it stays behind the wait for
+// the copy that wrote the rows.
 __device__ __forceinline__ void load_transposed(uint32_t (&r)[4], uint32_t address) {
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
                  : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
-                 : "r"(address)
-                 : "memory");
+                 : "r"(address));
 }
 
 __device__ __forceinline__ void load4(const float* p, float (&v)[4]) {

@@ -42,7 +42,8 @@ __host__ __device__ constexpr Layout layout_of(int warps, int heads, int head_di
     Layout l{};
     const int stage = 2 * kUnit * head_dim;  // [tile][K, V][16 tokens][head_dim]
     const int partial = heads * (head_dim + 4) * 4;
-    const int fixed = warps * 2 * partial + warps * 2 * int(sizeof(Record)) + 1024;
+    const int misc = (warps * 32 + 1 + warps) * 8 + 4 * 4;  // scan, joins
+    const int fixed = warps * 2 * partial + warps * 2 * int(sizeof(Record)) + misc;
     int stages = (kSmemBytes - fixed) / (warps * (stage + kTiles * 8 + 8));
     stages = stages > 3 ? 3 : stages;
     l.stages = stages;
@@ -51,7 +52,7 @@ __host__ __device__ constexpr Layout layout_of(int warps, int heads, int head_di
     l.meta = l.records + warps * 2 * int(sizeof(Record));
     l.bars = l.meta + warps * stages * kTiles * 8;
     l.misc = l.bars + warps * stages * 8;
-    l.total = l.misc + 1024;
+    l.total = l.misc + misc;
     return l;
 }
 static_assert(layout_of(12, 8, 128).stages >= 1 && layout_of(16, 8, 64).stages >= 2 && layout_of(8, 8, 128).stages >= 2);
@@ -125,9 +126,9 @@ __global__ void __launch_bounds__(warps_of<T, D>() * 32, 1)
     Record* records = reinterpret_cast<Record*>(smem + lay.records);
     float2* meta = reinterpret_cast<float2*>(smem + lay.meta) + warp * lay.stages * kTiles;
     uint64_t* bars = reinterpret_cast<uint64_t*>(smem + lay.bars) + warp * lay.stages;
-    int64_t* scan = reinterpret_cast<int64_t*>(smem + lay.misc);                  // [kWarps + 1]
-    int* first = reinterpret_cast<int*>(scan + kWarps + 1);                       // [kWarps][3] row, item, unit
-    int* joins = first + 3 * kWarps;                                              // [2] CTAs to join, 0: none
+    int64_t* sums = reinterpret_cast<int64_t*>(smem + lay.misc);  // [kWarps] units of each warp's rows
+    int64_t* before = sums + kWarps;                              // [kThreads + 1] units before each thread's rows
+    int* joins = reinterpret_cast<int*>(before + kThreads + 1);   // [2] CTAs to join (0: none), [2] their records
     if (lane == 0)
         for (int i = 0; i < lay.stages; ++i) mbar_init(bars + i, 1);
     if (lane < 2) records[2 * warp + lane].units = 0;
@@ -135,80 +136,92 @@ __global__ void __launch_bounds__(warps_of<T, D>() * 32, 1)
     fence_barrier_init();
     pdl_enter();
 
-    // ---- units of all rows, and where this CTA's warps begin
+    // ---- units of all rows (thread t adds up rows t share .. ), and where each warp begins
     const int bt = p.cache.block_tokens;
     const int64_t longest = int64_t(p.table_stride) * bt;
     const int share = (p.count + kThreads - 1) / kThreads;
-    const int r0 = min(tid * share, p.count), r1 = min(r0 + share, p.count);
     auto tokens = [&](int row) {
         const int n = p.lengths[row];
         if (n >= 0 && n <= longest) return n;
         raise_error(p.error, kErrBounds);
         return 0;
     };
-    int64_t mine = 0;
-    for (int r = r0; r < r1; ++r) mine += (tokens(r) + kUnit - 1) / kUnit;
-    int64_t before = mine;  // inclusive scan over the warp
+    auto units_of = [&](int row) { return row < p.count ? int((unsigned(tokens(row)) + kUnit - 1) / kUnit) : 0; };
+    {
+        int64_t mine = 0;
+        for (int i = 0; i < share; ++i) mine += units_of(tid * share + i);
+        int64_t upto = mine;  // inclusive scan over the warp
 #pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-        const int64_t x = __shfl_up_sync(0xffffffffu, before, o);
-        if (lane >= o) before += x;
+        for (int o = 1; o < 32; o <<= 1) {
+            const int64_t x = __shfl_up_sync(0xffffffffu, upto, o);
+            if (lane >= o) upto += x;
+        }
+        if (lane == 31) sums[warp] = upto;
+        __syncthreads();
+        int64_t x = lane < warp ? sums[lane] : 0;
+#pragma unroll
+        for (int o = 16; o; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
+        before[tid] = x + upto - mine;
+        if (tid == kThreads - 1) before[kThreads] = x + upto;
+        __syncthreads();
     }
-    if (lane == 31) scan[warp] = before;
-    before -= mine;
-    __syncthreads();
-    int64_t total = 0;
-    for (int w = 0; w < kWarps; ++w) {
-        if (w == warp) before += total;
-        total += scan[w];
-    }
-    total *= per;
+    const int64_t total = before[kThreads] * per;
     const int64_t want = (total + kWarps * kMinUnits - 1) / (kWarps * kMinUnits);
     const int ctas = int(want < int64_t(gridDim.x) ? want : int64_t(gridDim.x));
-    const int64_t workers = int64_t(ctas) * kWarps;
-    // where the run of each of the CTA's warps begins, and the next CTA's first (lane = warp)
-    const int64_t starts = total * (int64_t(blockIdx.x) * kWarps + min(lane, kWarps)) / (workers ? workers : 1);
-    auto cta_of = [&](int64_t unit) { return int(((unit + 1) * workers - 1) / total / kWarps); };
-    // rows without tokens
-    for (int r = blockIdx.x; r < p.count; r += gridDim.x)
-        if (tokens(r) == 0) {
-            T* out = static_cast<T*>(p.out) + r * p.out_stride;
-            for (int i = tid; i < p.heads * D / 4; i += kThreads) store4(out + 4 * i, 0.f, 0.f, 0.f, 0.f);
-        }
-    if (int(blockIdx.x) >= ctas) return;
-    for (int w = 0; w < kWarps; ++w) {
-        const int64_t g = __shfl_sync(0xffffffffu, starts, w);
-        if (g < before * per || g >= (before + mine) * per) continue;
-        int64_t x = before;
-        for (int r = r0; r < r1; ++r) {
-            const int u = (tokens(r) + kUnit - 1) / kUnit;
-            if (g < (x + u) * per) {
-                const int in = int(g - x * per);
-                first[3 * w] = r, first[3 * w + 1] = in / u, first[3 * w + 2] = in % u;
+    // worker w's run: `base` units, one more for the first `extra` workers
+    const int workers = max(ctas, 1) * kWarps;
+    const int64_t base = total >> 32 ? total / workers : int64_t(uint32_t(total) / uint32_t(workers));
+    const int extra = int(total - base * workers);
+    auto cta_of = [&](int64_t unit) {
+        const int64_t split = extra * (base + 1);
+        return int(unit < split ? unit / (base + 1) : extra + (unit - split) / base) / kWarps;
+    };
+    const int worker = blockIdx.x * kWarps + warp;
+    const int64_t begin = worker * base + min(worker, extra);
+    const int run = int(blockIdx.x) < ctas ? int(base) + (worker < extra) : 0;
+    int row = 0, item = 0, unit = 0;
+    if (run > 0) {
+        // the last thread whose rows begin at or before `begin`, then the row among its rows
+        int t = (31 - __clz(__ballot_sync(0xffffffffu, before[lane * kWarps] * per <= begin))) * kWarps;
+        t += 31 - __clz(__ballot_sync(0xffffffffu, lane < kWarps && before[t + min(lane, kWarps - 1)] * per <= begin));
+        row = t * share;
+        int64_t at = before[t];
+        for (int end = row + share;; row += 32) {  // 32 rows at a time
+            const int mine = row + lane < end ? units_of(row + lane) : 0;
+            int upto = mine;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const int x = __shfl_up_sync(0xffffffffu, upto, o);
+                if (lane >= o) upto += x;
+            }
+            const unsigned past = __ballot_sync(0xffffffffu, (at + upto) * per > begin);
+            if (past) {
+                const int i = __ffs(past) - 1;
+                const int u = __shfl_sync(0xffffffffu, mine, i);
+                const int in = int(begin - (at + __shfl_sync(0xffffffffu, upto, i) - u) * per);
+                row += i, item = in / u, unit = in % u;
                 break;
             }
-            x += u;
+            at += __shfl_sync(0xffffffffu, upto, 31);
         }
     }
-    __syncthreads();
 
-    // ---- this warp's run
-    const int64_t begin = __shfl_sync(0xffffffffu, starts, warp);
-    const int run = int(__shfl_sync(0xffffffffu, starts, warp + 1) - begin);
-    if (run > 0) {
-        const int in_page = bt / kTile;
-        // producer: the next unit to copy, and a window of 32 tiles (block, row, scales) over the lanes
-        int c_row = first[3 * warp], c_item = first[3 * warp + 1], c_unit = first[3 * warp + 2];
-        int c_len = tokens(c_row), c_left = run, w_base = -32;
-        int w_block = 0, w_at = 0;
-        float2 w_scale{};
+    // ---- this warp's run. Producer: the next unit to copy, and a window of 32 tiles (block,
+    // row, scales) over the lanes
+    const int in_page = bt / kTile;
+    const uint32_t ring_at = smem_u32(ring) + (lane & 1) * (kStage / 2);
+    int c_row = row, c_item = item, c_unit = unit, c_left = run, c_len = run ? tokens(row) : 0;
+    int w_next = 16, w_block = 0, w_at = 0, w_live = 0;  // w_next: unit of the window that comes next
+    float2 w_scale{};
+    {
         auto issue = [&](int stage) {
             if (c_left == 0) return;
-            if (kTiles * c_unit >= w_base + 32) {
-                w_base = kTiles * c_unit;
-                const int tile = w_base + lane;
+            if (w_next == 16) {
+                w_next = 0;
+                const int tile = kTiles * c_unit + lane;
                 w_scale = make_float2(0.f, 0.f);
-                if (tile * kTile < c_len && lane < kTiles * c_left) {
+                w_live = tile * kTile < c_len && lane < kTiles * c_left;
+                if (w_live) {
                     const int kh = c_item / subs;
                     w_block = block_id(p.cache, p.tables + int64_t(c_row) * p.table_stride, p.table_stride, tile / in_page,
                                        p.error);
@@ -216,21 +229,19 @@ __global__ void __launch_bounds__(warps_of<T, D>() * 32, 1)
                     w_at = kh * 2 * bt + tile % in_page * kTile;
                 }
             }
-            const int mine = lane + w_base - kTiles * c_unit;  // this lane's tile of the unit, if it has one
-            const bool both = (kTiles * c_unit + 1) * kTile < c_len;
-            if (mine == 0) mbar_arrive_expect_tx(bars + stage, both ? kStage : kStage / 2);
-            __syncwarp();
-            if (mine == 0 || mine == 1) {
-                meta[kTiles * stage + mine] = w_scale;
-                if (mine == 0 || both) {
-                    unsigned char* to = ring + stage * kStage + mine * (kStage / 2);
-                    load_box(to, &pages, w_at, w_block, bars + stage);
-                    if (in_page > 1) load_box(to + kTile * D, &pages, w_at + bt, w_block, bars + stage);
+            if (lane >> 1 == w_next) {  // two lanes copy a tile each
+                const int tiles = __popc(__ballot_sync(3u << (lane & ~1), w_live));
+                if (!(lane & 1)) mbar_arrive_expect_tx(bars + stage, tiles * (kStage / 2));
+                __syncwarp(3u << (lane & ~1));
+                meta[kTiles * stage + (lane & 1)] = w_scale;
+                if (w_live) {
+                    load_box(ring_at + stage * kStage, &pages, w_at, w_block, bars + stage);
+                    if (in_page > 1) load_box(ring_at + stage * kStage + kTile * D, &pages, w_at + bt, w_block, bars + stage);
                 }
             }
-            --c_left;
-            if (++c_unit * kUnit >= c_len && c_left) {
-                c_unit = 0, w_base = -32;
+            ++w_next, ++c_unit, --c_left;
+            if (c_unit * kUnit >= c_len && c_left) {
+                c_unit = 0, w_next = 16;
                 if (++c_item == per) {
                     c_item = 0;
                     do c_len = tokens(++c_row);
@@ -241,7 +252,14 @@ __global__ void __launch_bounds__(warps_of<T, D>() * 32, 1)
         for (int s = 0; s < lay.stages; ++s) issue(s);
         __syncwarp();
 
-        int row = first[3 * warp], item = first[3 * warp + 1], unit = first[3 * warp + 2];
+        // rows without tokens, while the copies fly
+        for (int r = blockIdx.x * kWarps + warp; r < p.count; r += gridDim.x * kWarps)
+            if (tokens(r) == 0) {
+                T* out = static_cast<T*>(p.out) + r * p.out_stride;
+                for (int i = lane; i < p.heads * D / 4; i += 32) store4(out + 4 * i, 0.f, 0.f, 0.f, 0.f);
+            }
+        if (int(blockIdx.x) >= ctas) return;
+
         const int k_row = WarpRow<T, F, D>::token(0, lane >> 2);                    // and 8 rows on
         const int v_row = WarpRow<T, F, D>::token((lane >> 3) & 1, lane & 7);       // this lane's matrix row
         int stage = 0, emitted = 0;
@@ -260,11 +278,9 @@ __global__ void __launch_bounds__(warps_of<T, D>() * 32, 1)
                     if (lane == 0) raise_error(p.error, kErrTimeout);
                 }
                 const unsigned char* at = ring + stage * kStage;
-                auto load_k = [&](int u, int i, uint4 (&k)[D / 64]) {
-#pragma unroll
-                    for (int h = 0; h < D / 64; ++h)
-                        k[h] = *reinterpret_cast<const uint4*>(at + (2 * u * kTile + k_row + 8 * i) * D +
-                                                               swizzled<D>(k_row, 4 * h + (lane & 3)) * 16);
+                auto load_k = [&](int u, int i, int h) {
+                    return *reinterpret_cast<const uint4*>(at + (2 * u * kTile + k_row + 8 * i) * D +
+                                                           swizzled<D>(k_row, 4 * h + (lane & 3)) * 16);
                 };
                 const uint32_t v_at = smem_u32(at) + (kTile + v_row) * D;
                 auto load_v = [&](int u, int q, uint32_t (&r)[4]) {
@@ -340,7 +356,7 @@ __global__ void __launch_bounds__(warps_of<T, D>() * 32, 1)
                 counters[c0] = 0;
                 joins[r.begins] = n;
                 records[index].begins = c0 + 1;  // read back below as the joining record
-                first[r.begins] = index;
+                joins[2 + r.begins] = index;
             }
             __threadfence();
         }
@@ -352,7 +368,7 @@ __global__ void __launch_bounds__(warps_of<T, D>() * 32, 1)
     for (int k = 0; k < 2; ++k) {
         const int n = joins[k];
         if (n == 0) continue;
-        const Record r = records[first[k]];
+        const Record r = records[joins[2 + k]];
         const int c0 = r.begins - 1;
         Joined<D> j;
         j.clear();

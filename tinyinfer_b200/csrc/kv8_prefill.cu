@@ -48,9 +48,8 @@ __global__ void __launch_bounds__(kThreads) row_kernel(const AttentionParams p) 
                 at[u] = p.cache.pages + tile_offset(p.cache, block, kh, 0, D) + (token % bt) * D;
             }
         }
-        auto load_k = [&](int u, int i, uint4 (&k)[D / 64]) {
-#pragma unroll
-            for (int h = 0; h < D / 64; ++h) k[h] = *reinterpret_cast<const uint4*>(at[u] + w.token(i, n) * D + h * 64 + c * 16);
+        auto load_k = [&](int u, int i, int h) {
+            return *reinterpret_cast<const uint4*>(at[u] + w.token(i, n) * D + h * 64 + c * 16);
         };
         auto load_v = [&](int u, int q, uint32_t (&r)[4]) {
 #pragma unroll

@@ -18,9 +18,12 @@
 // (measured: 1.8e-5 after 1000 tiles). FP32 outputs therefore add the products up in
 // chains of kChain units and the chains in FP32 registers.
 //
-// The state is a running softmax: m (largest score), l (sum of weights), and outputs in
-// units of `unit`, the largest weight times scale so far (moved whenever m moves or a
-// larger product comes), so that the weights fill FP16's range.
+// The state is a running softmax: m (the reference score), l (sum of weights), and outputs
+// in units of `unit`, a power of two at most the largest weight times scale so far, so that
+// the weights fill FP16's range. FP16 has room for weights 8 times 2^12 (`unit` is below the
+// largest by up to 2), so m and unit move only when a score passes m by 2 (in powers of
+// two) or a scale reaches twice the unit: moving them every time that the maximum grew cost a
+// fifth of the instructions.
 #pragma once
 #include "kv8.cuh"
 
@@ -31,8 +34,9 @@ constexpr int kTile = 16;                  // tokens of a tile: the K of one pro
 constexpr int kTiles = 2;                  // tiles of a unit: their products overlap, and votes and shuffles halve
 constexpr int kUnit = kTile * kTiles;
 constexpr int kChain = 4;                  // units per chain of tensor-op sums (FP32 outputs)
-constexpr float kWeightTop = 4096.f;       // weights are at most 2^12 in FP16
-constexpr float kUnitFloor = 7.7e-34f;     // 2^-110: below every scale the append makes
+constexpr float kWeightTop = 4096.f;       // a weight of `unit` is 2^12 in FP16
+constexpr float kSlack = 2.f;              // a score may pass m by this (weights up to 2^2)
+constexpr float kUnitFloor = 7.70371977754894e-34f;  // 2^-110: below every scale the append makes
 
 template <class T, int F, int D>
 struct WarpRow {
@@ -79,39 +83,46 @@ struct WarpRow {
         m = -INFINITY, l = 0.f, unit = kUnitFloor, inv_unit = kWeightTop / kUnitFloor, chain = 0;
     }
 
-    // One unit. load_k(u, i, k): the 16-byte words c of every 64-byte half of token(i, n)'s row
-    // in tile u; load_v(u, q, r): dims 32 q .. 32 q + 31 of V's tile u as four transposed
+    // One unit. load_k(u, i, h): the 16-byte word c of 64-byte half h of token(i, n)'s row in
+    // tile u (bytes behind the last token may be NaN codes: they become zero); load_v(u, q, r): dims 32 q .. 32 q + 31 of V's tile u as four transposed
     // matrices, r[2 a + i] = chunk 2 q + a of the tokens of half i; scale[u]: the K and V
     // scales. Tokens at or past `valid` (1 .. 32) are masked (a tile without tokens has
     // scales 0).
     template <class LoadK, class LoadV>
     __device__ __forceinline__ void step(LoadK load_k, LoadV load_v, const float2 (&scale)[kTiles], int valid, int lane) {
         const int n = lane >> 2, c = lane & 3;
+        float acc[kTiles][2][4];
+#pragma unroll
+        for (int h = 0; h < kHalves; ++h) {
+            uint4 k[kTiles][2];
+#pragma unroll
+            for (int u = 0; u < kTiles; ++u)
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    k[u][i] = load_k(u, i, h);
+                    if (valid < kUnit && u * kTile + token(i, n) >= valid) k[u][i] = make_uint4(0, 0, 0, 0);
+                    if (h == 0) acc[u][i][0] = acc[u][i][1] = acc[u][i][2] = acc[u][i][3] = 0.f;
+                }
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+#pragma unroll
+                for (int u = 0; u < kTiles; ++u)
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        const uint4 w = k[u][i];
+                        uint32_t b0, b1;
+                        widen4<F>(j == 0 ? w.x : j == 1 ? w.y : j == 2 ? w.z : w.w, b0, b1);
+                        mma16816(acc[u][i], qa[4 * h + j], b0, b1);
+                    }
+        }
         float t[kTiles][2][2];
 #pragma unroll
         for (int u = 0; u < kTiles; ++u) {
             const float f = k_factor * scale[u].x;
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
-                uint4 k[kHalves];
-                load_k(u, i, k);
-                if (valid < kUnit && u * kTile + token(i, n) >= valid) {  // bytes behind the last token may be NaN codes
-#pragma unroll
-                    for (int h = 0; h < kHalves; ++h) k[h] = make_uint4(0, 0, 0, 0);
-                }
-                float acc[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                for (int h = 0; h < kHalves; ++h) {
-                    const uint32_t w[4] = {k[h].x, k[h].y, k[h].z, k[h].w};
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        uint32_t b0, b1;
-                        widen4<F>(w[j], b0, b1);
-                        mma16816(acc, qa[4 * h + j], b0, b1);
-                    }
-                }
-                t[u][i][0] = (acc[0] + acc[2]) * f;
-                t[u][i][1] = (acc[1] + acc[3]) * f;
+                t[u][i][0] = (acc[u][i][0] + acc[u][i][2]) * f;
+                t[u][i][1] = (acc[u][i][1] + acc[u][i][3]) * f;
             }
         }
         auto live = [&](int u, int i, int j) { return u * kTile + token(i, 2 * c + j) < valid; };
@@ -123,36 +134,15 @@ struct WarpRow {
 #pragma unroll
                     for (int j = 0; j < 2; ++j) t[u][i][j] = live(u, i, j) ? t[u][i][j] : -INFINITY;
         }
-        float tops[kTiles], top = -INFINITY, most = 0.f;
+        float top = -INFINITY, most = 0.f;
 #pragma unroll
         for (int u = 0; u < kTiles; ++u) {
-            tops[u] = fmaxf(fmaxf(t[u][0][0], t[u][0][1]), fmaxf(t[u][1][0], t[u][1][1]));
-            top = fmaxf(top, tops[u]);
+            top = fmaxf(top, fmaxf(fmaxf(t[u][0][0], t[u][0][1]), fmaxf(t[u][1][0], t[u][1][1])));
             most = fmaxf(most, scale[u].y);
         }
         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-        if (__any_sync(0xffffffffu, top > m || most > unit)) {
-            const float m_new = fmaxf(m, top);
-            float reach = 0.f;  // largest weight times scale of the unit
-#pragma unroll
-            for (int u = 0; u < kTiles; ++u) reach = fmaxf(reach, tops[u] == -INFINITY ? 0.f : scale[u].y * ex2(tops[u] - m_new));
-            reach = fmaxf(reach, __shfl_xor_sync(0xffffffffu, reach, 1));
-            reach = fmaxf(reach, __shfl_xor_sync(0xffffffffu, reach, 2));
-            if (__any_sync(0xffffffffu, top > m || reach > unit)) {
-                const float decay = m_new == -INFINITY ? 1.f : ex2(m - m_new);
-                const float unit_new = fmaxf(fmaxf(unit * decay, reach), kUnitFloor);
-                const float move = decay * unit / unit_new;
-                l *= decay;
-#pragma unroll
-                for (int i = 0; i < D / 8; ++i) {
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) o[i][j] *= move;
-                    if constexpr (kSplit) sum[i][0] *= move, sum[i][1] *= move;
-                }
-                m = m_new, unit = unit_new, inv_unit = kWeightTop / unit_new;
-            }
-        }
+        if (__any_sync(0xffffffffu, top > m + kSlack || most >= 2.f * unit)) move(t, scale, top);
         const float base = m == -INFINITY ? 0.f : m;
 #pragma unroll
         for (int u = 0; u < kTiles; ++u) {
@@ -170,9 +160,10 @@ struct WarpRow {
                     a[2 * i + 1] = 0;
                 }
             }
-            uint32_t keep[2];
+            uint32_t keep[2] = {0xffffffffu, 0xffffffffu};
+            if (valid < kUnit)
 #pragma unroll
-            for (int i = 0; i < 2; ++i) keep[i] = (live(u, i, 0) ? 0xffffu : 0u) | (live(u, i, 1) ? 0xffff0000u : 0u);
+                for (int i = 0; i < 2; ++i) keep[i] = (live(u, i, 0) ? 0xffffu : 0u) | (live(u, i, 1) ? 0xffff0000u : 0u);
 #pragma unroll
             for (int q = 0; q < D / 32; ++q) {
                 uint32_t r[4];
@@ -194,6 +185,33 @@ struct WarpRow {
                 chain = 0;
             }
         }
+    }
+
+    // Takes the largest score as the reference and the largest weight times scale as the unit,
+    // if a head needs it.
+    __device__ __forceinline__ void move(const float (&t)[kTiles][2][2], const float2 (&scale)[kTiles], float top) {
+        const float m_new = fmaxf(m, top);
+        float reach = 0.f;  // largest weight times scale of the unit
+#pragma unroll
+        for (int u = 0; u < kTiles; ++u) {
+            const float tops = fmaxf(fmaxf(t[u][0][0], t[u][0][1]), fmaxf(t[u][1][0], t[u][1][1]));
+            if (tops != -INFINITY) reach = fmaxf(reach, scale[u].y * ex2(tops - m_new));
+        }
+        reach = fmaxf(reach, __shfl_xor_sync(0xffffffffu, reach, 1));
+        reach = fmaxf(reach, __shfl_xor_sync(0xffffffffu, reach, 2));
+        if (!__any_sync(0xffffffffu, top > m + kSlack || reach >= 2.f * unit)) return;
+        const float decay = m_new == -INFINITY ? 1.f : ex2(m - m_new);
+        const float largest = fminf(fmaxf(fmaxf(unit * decay, reach), kUnitFloor), 8.507059e37f);
+        const int exponent = (__float_as_int(largest) >> 23) - 127;  // rounded down to a power of two
+        const float by = decay * (unit * pow2(-exponent));
+        l *= decay;
+#pragma unroll
+        for (int i = 0; i < D / 8; ++i) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) o[i][j] *= by;
+            if constexpr (kSplit) sum[i][0] *= by, sum[i][1] *= by;
+        }
+        m = m_new, unit = pow2(exponent), inv_unit = kWeightTop * pow2(-exponent);
     }
 
     __device__ __forceinline__ void close() {
