@@ -52,7 +52,7 @@ def refused(op, code, cache_kw=None, error=None, **kw):
 @pytest.mark.parametrize("code,kw", [
     (mp.MP_ERR_INVALID, {"pages": None}), (mp.MP_ERR_INVALID, {"scales": None}), (mp.MP_ERR_INVALID, {"pages": A + 8}),
     (mp.MP_ERR_INVALID, {"scales": A + 4}), (mp.MP_ERR_INVALID, {"page_stride": 6143}),
-    (mp.MP_ERR_INVALID, {"page_stride": 6144 + 8}), (mp.MP_ERR_INVALID, {"page_stride": 6128}), (mp.MP_ERR_INVALID, {"page_stride": 1 << 40}),
+    (mp.MP_ERR_INVALID, {"page_stride": 6144 + 8}), (mp.MP_ERR_INVALID, {"page_stride": 6128}),
     (mp.MP_ERR_INVALID, {"scale_stride": 4}), (mp.MP_ERR_INVALID, {"scale_stride": 7}),
     (mp.MP_ERR_INVALID, {"format": 2}), (mp.MP_ERR_INVALID, {"kv_heads": 0}), (mp.MP_ERR_INVALID, {"kv_heads": 2}),
     (mp.MP_ERR_INVALID, {"max_blocks": 0}), (mp.MP_ERR_UNSUPPORTED, {"head_dim": 96}),

@@ -3,7 +3,6 @@
 // metadata. The layout is mp_kv8_cache's (miniprefix_b200.h): a block holds, per kv
 // head, a K tile and a V tile of [block_tokens][head_dim] bytes, each with one scale.
 #pragma once
-#include <cuda.h>
 #include <cuda_bf16.h>
 
 #include "common.cuh"
@@ -50,10 +49,6 @@ struct AttentionParams {
 cudaError_t launch_append(const AppendParams& p, int type, int format, int head_dim, cudaStream_t stream);
 cudaError_t launch_decode(const AttentionParams& p, int type, int format, int head_dim, cudaStream_t stream);
 cudaError_t launch_prefill(const AttentionParams& p, int type, int format, int head_dim, cudaStream_t stream);
-// Tensor map of the cache's pages for TMA boxes of `box_rows` token rows of one tile: the
-// dimensions are (dim, kv head x K/V x slot, block), rows land in shared memory with the
-// 64- or 128-byte swizzle of their length.
-cudaError_t page_map(const Cache& cache, int head_dim, int box_rows, CUtensorMap* map);
 size_t decode_workspace(int group, int head_dim);
 size_t prefill_workspace(int group, int head_dim);
 
@@ -70,16 +65,7 @@ cudaError_t dispatch(int type, int format, int head_dim, F f) {
     return type == MP_TYPE_F32 ? by_format(float{}) : by_format(__nv_bfloat16{});
 }
 
-// Bulk tensor copy of one box of page_map: token rows from `row` on, of block `block`.
-__device__ __forceinline__ void load_box(uint32_t dst, const CUtensorMap* map, int row, int block, uint64_t* bar) {
-    asm volatile(
-        "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(
-            dst),
-        "l"(map), "r"(0), "r"(row), "r"(block), "r"(smem_u32(bar))
-        : "memory");
-}
-
-// 16-byte chunk at which a box's swizzle puts chunk `chunk` of token row `row`.
+// Position of 16-byte chunk `chunk` of token row `row` in a swizzled tile in shared memory.
 template <int D>
 __device__ __forceinline__ int swizzled(int row, int chunk) {
     return chunk ^ (D == 128 ? row & 7 : (row >> 1) & 3);

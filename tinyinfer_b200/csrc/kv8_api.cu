@@ -1,8 +1,6 @@
 // Entry points of the 8-bit paged K/V cache operators: argument checks, then one
 // launch on the caller's stream. Nothing here allocates, copies or synchronises
 // (mp_kv8_status alone synchronises).
-#include <cudaTypedefs.h>
-
 #include "kv8.cuh"
 
 namespace {
@@ -24,9 +22,8 @@ int check_cache(const mp_kv8_cache* c) {
     if (c->head_dim != 64 && c->head_dim != 128) return refuse(MP_ERR_UNSUPPORTED, "kv8: head_dim is not 64 or 128");
     if (c->block_tokens < 16 || c->block_tokens > 256 || c->block_tokens % 16)
         return refuse(MP_ERR_UNSUPPORTED, "kv8: block_tokens is not a multiple of 16 up to 256");
-    if (c->page_stride < int64_t(c->kv_heads) * 2 * c->block_tokens * c->head_dim || c->page_stride % 16 ||
-        c->page_stride >= int64_t(1) << 40)
-        return refuse(MP_ERR_INVALID, "kv8: page_stride below a block's bytes, no multiple of 16, or 2^40 and more");
+    if (c->page_stride < int64_t(c->kv_heads) * 2 * c->block_tokens * c->head_dim || c->page_stride % 16)
+        return refuse(MP_ERR_INVALID, "kv8: page_stride below a block's bytes or no multiple of 16");
     if (c->scale_stride < 2 * c->kv_heads || c->scale_stride % 2)
         return refuse(MP_ERR_INVALID, "kv8: scale_stride below 2 * kv_heads or odd");
     if (!aligned(c->pages, 16) || !aligned(c->scales, 8)) return refuse(MP_ERR_INVALID, "kv8: misaligned cache");
@@ -95,25 +92,6 @@ bool geometry(const mp_kv8_cache* c, int heads) {
     } while (0)
 
 }  // namespace
-
-cudaError_t mpb::kv8::page_map(const Cache& c, int head_dim, int box_rows, CUtensorMap* map) {
-    static const PFN_cuTensorMapEncodeTiled_v12000 encode = [] {
-        cudaDriverEntryPointQueryResult q{};
-        void* p = nullptr;
-        const cudaError_t e = cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &p, 12000, cudaEnableDefault, &q);
-        return e == cudaSuccess && q == cudaDriverEntryPointSuccess ? reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(p)
-                                                                    : nullptr;
-    }();
-    if (!encode) return cudaErrorNotSupported;
-    const cuuint64_t dims[3] = {cuuint64_t(head_dim), cuuint64_t(c.kv_heads) * 2 * c.block_tokens, cuuint64_t(c.max_blocks)};
-    const cuuint64_t strides[2] = {cuuint64_t(head_dim), cuuint64_t(c.page_stride)};
-    const cuuint32_t box[3] = {cuuint32_t(head_dim), cuuint32_t(box_rows), 1}, steps[3] = {1, 1, 1};
-    const CUresult r = encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, c.pages, dims, strides, box, steps,
-                              CU_TENSOR_MAP_INTERLEAVE_NONE,
-                              head_dim == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B,
-                              CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-    return r == CUDA_SUCCESS ? cudaSuccess : cudaErrorInvalidValue;
-}
 
 extern "C" int mp_kv8_append(const mp_kv8_cache* cache, const mp_kv8_append_args* a, uint32_t* device_error,
                              void* stream) {

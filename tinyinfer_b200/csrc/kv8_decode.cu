@@ -36,7 +36,7 @@ struct Record {  // a partial of one warp, or none (units 0)
 
 // Shared memory of a CTA; `heads` = partial rows (query heads of an item, up to 8).
 struct Layout {
-    int partials, records, meta, bars, misc, total, stages;
+    int partials, records, meta, misc, total, stages;
 };
 __host__ __device__ constexpr Layout layout_of(int warps, int heads, int head_dim) {
     Layout l{};
@@ -44,19 +44,22 @@ __host__ __device__ constexpr Layout layout_of(int warps, int heads, int head_di
     const int partial = heads * (head_dim + 4) * 4;
     const int misc = (warps * 32 + 1 + warps) * 8 + 4 * 4;  // scan, joins
     const int fixed = warps * 2 * partial + warps * 2 * int(sizeof(Record)) + misc;
-    int stages = (kSmemBytes - fixed) / (warps * (stage + kTiles * 8 + 8));
+    int stages = (kSmemBytes - fixed) / (warps * (stage + kTiles * 8));
     stages = stages > 3 ? 3 : stages;
     l.stages = stages;
     l.partials = warps * stages * stage;
     l.records = l.partials + warps * 2 * partial;
     l.meta = l.records + warps * 2 * int(sizeof(Record));
-    l.bars = l.meta + warps * stages * kTiles * 8;
-    l.misc = l.bars + warps * stages * 8;
+    l.misc = l.meta + warps * stages * kTiles * 8;
     l.total = l.misc + misc;
     return l;
 }
 static_assert(layout_of(12, 8, 128).stages >= 1 && layout_of(16, 8, 64).stages >= 2 && layout_of(8, 8, 128).stages >= 2);
 static_assert(layout_of(12, 8, 128).total <= kSmemBytes && layout_of(16, 1, 64).total <= kSmemBytes);
+
+__device__ __forceinline__ void copy16(uint32_t to, const void* from) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory");
+}
 
 // A partial row of one query head: head_dim outputs, then max and sum.
 template <int D>
@@ -113,7 +116,7 @@ struct Joined {
 
 template <class T, int F, int D>
 __global__ void __launch_bounds__(warps_of<T, D>() * 32, 1)
-    decode_kernel(const AttentionParams p, const __grid_constant__ CUtensorMap pages) {
+    decode_kernel(const AttentionParams p) {
     constexpr int kWarps = warps_of<T, D>(), kThreads = kWarps * 32, kStage = 2 * kUnit * D;
     extern __shared__ __align__(1024) unsigned char smem[];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -125,15 +128,11 @@ __global__ void __launch_bounds__(warps_of<T, D>() * 32, 1)
     float* partials = reinterpret_cast<float*>(smem + lay.partials);
     Record* records = reinterpret_cast<Record*>(smem + lay.records);
     float2* meta = reinterpret_cast<float2*>(smem + lay.meta) + warp * lay.stages * kTiles;
-    uint64_t* bars = reinterpret_cast<uint64_t*>(smem + lay.bars) + warp * lay.stages;
     int64_t* sums = reinterpret_cast<int64_t*>(smem + lay.misc);  // [kWarps] units of each warp's rows
     int64_t* before = sums + kWarps;                              // [kThreads + 1] units before each thread's rows
     int* joins = reinterpret_cast<int*>(before + kThreads + 1);   // [2] CTAs to join (0: none), [2] their records
-    if (lane == 0)
-        for (int i = 0; i < lay.stages; ++i) mbar_init(bars + i, 1);
     if (lane < 2) records[2 * warp + lane].units = 0;
     if (tid < 2) joins[tid] = 0;
-    fence_barrier_init();
     pdl_enter();
 
     // ---- units of all rows (thread t adds up rows t share .. ), and where each warp begins
@@ -209,45 +208,56 @@ __global__ void __launch_bounds__(warps_of<T, D>() * 32, 1)
     // ---- this warp's run. Producer: the next unit to copy, and a window of 32 tiles (block,
     // row, scales) over the lanes
     const int in_page = bt / kTile;
-    const uint32_t ring_at = smem_u32(ring) + (lane & 1) * (kStage / 2);
+    // 16-byte words of a tile row by row, 32 lanes at a time: kRows rows, kTimes times
+    constexpr int kRows = 512 / D, kTimes = kTile / kRows;
+    const int to_row = lane / (D / 16);
+    uint32_t to[2];  // a row and one kRows further on (which the swizzle may tell apart), words of this lane
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+        to[i] = smem_u32(ring) + (to_row + i * kRows) * D + swizzled<D>(to_row + i * kRows, lane % (D / 16)) * 16;
     int c_row = row, c_item = item, c_unit = unit, c_left = run, c_len = run ? tokens(row) : 0;
-    int w_next = 16, w_block = 0, w_at = 0, w_live = 0;  // w_next: unit of the window that comes next
+    int w_next = 16;                       // unit of the window that comes next
+    const unsigned char* w_at = nullptr;   // this lane's tile (K; V is one block of rows on)
     float2 w_scale{};
     {
         auto issue = [&](int stage) {
-            if (c_left == 0) return;
-            if (w_next == 16) {
-                w_next = 0;
-                const int tile = kTiles * c_unit + lane;
-                w_scale = make_float2(0.f, 0.f);
-                w_live = tile * kTile < c_len && lane < kTiles * c_left;
-                if (w_live) {
-                    const int kh = c_item / subs;
-                    w_block = block_id(p.cache, p.tables + int64_t(c_row) * p.table_stride, p.table_stride, tile / in_page,
-                                       p.error);
-                    w_scale = *reinterpret_cast<const float2*>(p.cache.scales + w_block * p.cache.scale_stride + 2 * kh);
-                    w_at = kh * 2 * bt + tile % in_page * kTile;
+            if (c_left) {
+                if (w_next == 16) {
+                    w_next = 0;
+                    const int tile = kTiles * c_unit + lane;
+                    w_scale = make_float2(0.f, 0.f);
+                    if (tile * kTile < c_len && lane < kTiles * c_left) {
+                        const int kh = c_item / subs;
+                        const int block = block_id(p.cache, p.tables + int64_t(c_row) * p.table_stride, p.table_stride,
+                                                   tile / in_page, p.error);
+                        w_scale = *reinterpret_cast<const float2*>(p.cache.scales + block * p.cache.scale_stride + 2 * kh);
+                        w_at = p.cache.pages + tile_offset(p.cache, block, kh, 0, D) + tile % in_page * (kTile * D);
+                    }
+                }
+                if (lane >> 1 == w_next) meta[kTiles * stage + (lane & 1)] = w_scale;
+#pragma unroll
+                for (int u = 0; u < kTiles; ++u) {
+                    const unsigned char* from = reinterpret_cast<const unsigned char*>(
+                        __shfl_sync(0xffffffffu, reinterpret_cast<uint64_t>(w_at), kTiles * w_next + u)) + lane * 16;
+                    if ((kTiles * c_unit + u) * kTile >= c_len) break;
+#pragma unroll
+                    for (int i = 0; i < kTimes; ++i) {
+                        const uint32_t at = to[i & 1] + stage * kStage + u * (kStage / 2) + (i >> 1) * (2 * kRows * D);
+                        copy16(at, from + i * 512);
+                        copy16(at + kTile * D, from + bt * D + i * 512);
+                    }
+                }
+                ++w_next, ++c_unit, --c_left;
+                if (c_unit * kUnit >= c_len && c_left) {
+                    c_unit = 0, w_next = 16;
+                    if (++c_item == per) {
+                        c_item = 0;
+                        do c_len = tokens(++c_row);
+                        while (c_len == 0);
+                    }
                 }
             }
-            if (lane >> 1 == w_next) {  // two lanes copy a tile each
-                const int tiles = __popc(__ballot_sync(3u << (lane & ~1), w_live));
-                if (!(lane & 1)) mbar_arrive_expect_tx(bars + stage, tiles * (kStage / 2));
-                __syncwarp(3u << (lane & ~1));
-                meta[kTiles * stage + (lane & 1)] = w_scale;
-                if (w_live) {
-                    load_box(ring_at + stage * kStage, &pages, w_at, w_block, bars + stage);
-                    if (in_page > 1) load_box(ring_at + stage * kStage + kTile * D, &pages, w_at + bt, w_block, bars + stage);
-                }
-            }
-            ++w_next, ++c_unit, --c_left;
-            if (c_unit * kUnit >= c_len && c_left) {
-                c_unit = 0, w_next = 16;
-                if (++c_item == per) {
-                    c_item = 0;
-                    do c_len = tokens(++c_row);
-                    while (c_len == 0);
-                }
-            }
+            asm volatile("cp.async.commit_group;" ::: "memory");  // one per unit, empty ones included
         };
         for (int s = 0; s < lay.stages; ++s) issue(s);
         __syncwarp();
@@ -263,8 +273,6 @@ __global__ void __launch_bounds__(warps_of<T, D>() * 32, 1)
         const int k_row = WarpRow<T, F, D>::token(0, lane >> 2);                    // and 8 rows on
         const int v_row = WarpRow<T, F, D>::token((lane >> 3) & 1, lane & 7);       // this lane's matrix row
         int stage = 0, emitted = 0;
-        uint32_t phase = 0;
-        bool ok = true;
         for (int done = 0; done < run;) {
             const int len = tokens(row), units = (len + kUnit - 1) / kUnit;
             const int last = min(units, unit + run - done), from = unit;
@@ -273,10 +281,14 @@ __global__ void __launch_bounds__(warps_of<T, D>() * 32, 1)
             WarpRow<T, F, D> w;
             w.begin(static_cast<const T*>(p.q) + row * p.q_stride + h0 * D, heads, p.scale, lane);
             for (; unit < last; ++unit) {
-                if (ok && !mbar_wait_bounded(bars + stage, phase)) {
-                    ok = false;
-                    if (lane == 0) raise_error(p.error, kErrTimeout);
+                if (lay.stages == 3) {
+                    asm volatile("cp.async.wait_group 2;" ::: "memory");
+                } else if (lay.stages == 2) {
+                    asm volatile("cp.async.wait_group 1;" ::: "memory");
+                } else {
+                    asm volatile("cp.async.wait_group 0;" ::: "memory");
                 }
+                __syncwarp();
                 const unsigned char* at = ring + stage * kStage;
                 auto load_k = [&](int u, int i, int h) {
                     return *reinterpret_cast<const uint4*>(at + (2 * u * kTile + k_row + 8 * i) * D +
@@ -289,10 +301,14 @@ __global__ void __launch_bounds__(warps_of<T, D>() * 32, 1)
                 float2 scale[kTiles];
 #pragma unroll
                 for (int u = 0; u < kTiles; ++u) scale[u] = meta[kTiles * stage + u];
-                w.step(load_k, load_v, scale, min(kUnit, len - unit * kUnit), lane);
+                if (len - unit * kUnit >= kUnit) {
+                    w.template step<false>(load_k, load_v, scale, kUnit, lane);
+                } else {
+                    w.template step<true>(load_k, load_v, scale, len - unit * kUnit, lane);
+                }
                 __syncwarp();
                 issue(stage);
-                if (++stage == lay.stages) stage = 0, phase ^= 1;
+                if (++stage == lay.stages) stage = 0;
             }
             w.end();
             done += last - from;
@@ -396,12 +412,10 @@ cudaError_t launch_decode(const AttentionParams& p, int type, int format, int he
         constexpr int kDim = decltype(d)::value, kWarps = warps_of<T, kDim>();
         auto kernel = decode_kernel<T, decltype(f)::value, kDim>;
         const int group = p.heads / p.cache.kv_heads;
-        CUtensorMap pages;
-        cudaError_t e = page_map(p.cache, kDim, p.cache.block_tokens == kTile ? 2 * kTile : kTile, &pages);
-        if (e == cudaSuccess) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes);
+        const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes);
         if (e != cudaSuccess) return e;
         return launch_pdl(kernel, dim3(kCtas), dim3(kWarps * 32), size_t(layout_of(kWarps, group < 8 ? group : 8, kDim).total),
-                          stream, p, pages);
+                          stream, p);
     });
 }
 

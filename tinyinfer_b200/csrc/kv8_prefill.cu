@@ -57,7 +57,11 @@ __global__ void __launch_bounds__(kThreads) row_kernel(const AttentionParams p) 
                 r[g] = transpose8x8(*reinterpret_cast<const uint32_t*>(at[u] + (bt + w.token(g & 1, n)) * D + 32 * q +
                                                                        16 * (g >> 1) + 4 * c));
         };
-        w.step(load_k, load_v, scale, min(kUnit, len - t), lane);
+        if (len - t >= kUnit) {
+            w.template step<false>(load_k, load_v, scale, kUnit, lane);
+        } else {
+            w.template step<true>(load_k, load_v, scale, len - t, lane);
+        }
     }
     w.end();
     w.write(static_cast<T*>(p.out) + row * p.out_stride + h0 * D, heads, lane);

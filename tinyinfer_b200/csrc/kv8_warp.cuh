@@ -86,9 +86,9 @@ struct WarpRow {
     // One unit. load_k(u, i, h): the 16-byte word c of 64-byte half h of token(i, n)'s row in
     // tile u (bytes behind the last token may be NaN codes: they become zero); load_v(u, q, r): dims 32 q .. 32 q + 31 of V's tile u as four transposed
     // matrices, r[2 a + i] = chunk 2 q + a of the tokens of half i; scale[u]: the K and V
-    // scales. Tokens at or past `valid` (1 .. 32) are masked (a tile without tokens has
-    // scales 0).
-    template <class LoadK, class LoadV>
+    // scales. kLast: tokens at or past `valid` (1 .. 32) are masked (a tile without tokens
+    // has scales 0); else all 32 are there.
+    template <bool kLast, class LoadK, class LoadV>
     __device__ __forceinline__ void step(LoadK load_k, LoadV load_v, const float2 (&scale)[kTiles], int valid, int lane) {
         const int n = lane >> 2, c = lane & 3;
         float acc[kTiles][2][4];
@@ -100,7 +100,7 @@ struct WarpRow {
 #pragma unroll
                 for (int i = 0; i < 2; ++i) {
                     k[u][i] = load_k(u, i, h);
-                    if (valid < kUnit && u * kTile + token(i, n) >= valid) k[u][i] = make_uint4(0, 0, 0, 0);
+                    if (kLast && u * kTile + token(i, n) >= valid) k[u][i] = make_uint4(0, 0, 0, 0);
                     if (h == 0) acc[u][i][0] = acc[u][i][1] = acc[u][i][2] = acc[u][i][3] = 0.f;
                 }
 #pragma unroll
@@ -126,7 +126,7 @@ struct WarpRow {
             }
         }
         auto live = [&](int u, int i, int j) { return u * kTile + token(i, 2 * c + j) < valid; };
-        if (valid < kUnit) {
+        if constexpr (kLast) {
 #pragma unroll
             for (int u = 0; u < kTiles; ++u)
 #pragma unroll
@@ -161,14 +161,14 @@ struct WarpRow {
                 }
             }
             uint32_t keep[2] = {0xffffffffu, 0xffffffffu};
-            if (valid < kUnit)
+            if constexpr (kLast)
 #pragma unroll
                 for (int i = 0; i < 2; ++i) keep[i] = (live(u, i, 0) ? 0xffffu : 0u) | (live(u, i, 1) ? 0xffff0000u : 0u);
 #pragma unroll
             for (int q = 0; q < D / 32; ++q) {
                 uint32_t r[4];
                 load_v(u, q, r);
-                if (valid < kUnit) r[0] &= keep[0], r[1] &= keep[1], r[2] &= keep[0], r[3] &= keep[1];
+                if constexpr (kLast) r[0] &= keep[0], r[1] &= keep[1], r[2] &= keep[0], r[3] &= keep[1];
 #pragma unroll
                 for (int g = 0; g < 2; ++g) {
                     uint32_t x0, x1, y0, y1;
