@@ -1,81 +1,660 @@
-// mp_kv8_attention_prefill: causal attention of packed chunks of rows over the 8-bit paged cache.
-#include "kv8_warp.cuh"
+// mp_kv8_attention_prefill: causal attention of packed chunks of rows over the 8-bit
+// paged cache, on tcgen05 (sm_100a).
+//
+// A work item is (block of rows of one sequence, kv head): rows x query heads of the group
+// fill two 128-vector tiles (vector v of a tile: row v / group, head v % group), and its
+// context is a run of 128-token K/V tiles. All items' tiles, in order, are dealt out in
+// equal runs to one CTA per SM, so a long context with few rows is shared like many short
+// ones; the device plans this itself from row_offsets and starts.
+//
+// Roles of a CTA (16 warps):
+//  * warps 8-11 widen K and V codes to FP16 tiles in shared memory (exact; K token-major,
+//    V token-major too: the tensor core reads it transposed), with their blocks' scales;
+//  * one thread of warp 12 issues the products: S = Q K^T into tensor memory, O = P V
+//    with P from tensor memory;
+//  * warps 0-3 and 4-7 own one tile each, a thread per vector: running softmax of S's
+//    row, weights written over S in place, O's rows added up.
+// While one tile's threads work on their S, the tensor core runs the other's O and S.
+//
+// FP32 precision: the query is two FP16 halves (each row scaled by a power of two towards
+// FP16's top), so S is two products per useful one; the weights, with V's scales folded
+// in, are two halves as well. BF16 inputs and outputs take one of each. The tensor core
+// cuts its sums (measured: 9e-8 of the sum per product of 16), so O starts anew with
+// every 128 tokens and is added up in FP32 registers, and the small halves' products go
+// first.
+//
+// Bound by the tensor core, exp2 and the softmax's other instructions alike: per 256
+// vectors x 128 tokens of FP32 at head_dim 64 each takes about 2050 cycles.
+#include "kv8.cuh"
+#include "umma.cuh"
 
 namespace mpb {
 namespace kv8 {
 namespace {
 
-constexpr int kThreads = 128;
+constexpr int kCtas = 148;
+constexpr int kThreads = 512;
+constexpr int kM = 128;       // vectors of a tile
+constexpr int kN = 128;       // tokens of a K/V tile
+// Scale rows in flight. Row j + 4 is written after P V of tile j + 1 completed (its V slot
+// was needed for tile j + 3), so every thread has read row j by then.
+constexpr int kScaleSlots = 4;
+constexpr int kGroupTokens = 16;  // tokens that share a block's scales at least
+constexpr int kGroups = kN / kGroupTokens;
+constexpr float kWeightTop = 4096.f, kSlack = 2.f, kUnitFloor = 7.70371977754894e-34f;  // as in kv8_warp.cuh
 
-// One warp per (row, kv head, 8 query heads), token unit by token unit.
-template <class T, int F, int D>
-__global__ void __launch_bounds__(kThreads) row_kernel(const AttentionParams p) {
-    pdl_enter();
-    const int lane = threadIdx.x & 31;
-    const int group = p.heads / p.cache.kv_heads, subs = (group + 7) / 8;
-    const int64_t item = int64_t(blockIdx.x) * (kThreads / 32) + (threadIdx.x >> 5);
-    const int per = p.cache.kv_heads * subs;
-    const int row = int(item / per), kh = int(item % per) / subs, sub = int(item % per) % subs;
-    if (row >= p.rows) return;
-    const int bt = p.cache.block_tokens;
-    int before = 0;
-    for (int i = lane; i < p.count; i += 32) before += p.row_offsets[i + 1] <= row;
-    const int seq = __reduce_add_sync(0xffffffffu, before);
-    if (seq >= p.count) return;
-    const int begin = p.row_offsets[seq], start = p.starts[seq];
-    const int64_t end = int64_t(start) + row - begin + 1;
-    if (row < begin || start < 0 || end > int64_t(p.table_stride) * bt) {
-        if (lane == 0) raise_error(p.error, kErrBounds);
-        return;
+template <class T, int D>
+struct Shape {
+    static constexpr int kHalves = sizeof(T) == 4 ? 2 : 1;              // FP16 halves of q and of the weights
+    static constexpr int kTileBytes = kM * D * 2;                       // one FP16 tile
+    static constexpr int kStages = kHalves == 2 && D == 128 ? 1 : 2;    // K (and V) tiles in shared memory
+    static constexpr int kQ = 0;                                        // [2 tiles][halves]
+    static constexpr int kK = kQ + 2 * kHalves * kTileBytes;
+    static constexpr int kV = kK + kStages * kTileBytes;
+    static constexpr int kScales = kV + kStages * kTileBytes;           // [slots][groups] (K, V)
+    static constexpr int kBars = kScales + kScaleSlots * kGroups * 8;
+    static constexpr int kPlan = kBars + 32 * 8;                        // planning, and a few words
+    static constexpr int kSmem = kPlan + (kThreads + 1) * 4 + (kThreads + 1) * 8 + 2 * 16 * 8 + 64;
+    static constexpr int kAlloc = kSmem + 1024;                         // alignment slack
+    static constexpr uint32_t kTmemCols = 512;                          // S: 2 x 128, O: 2 x D
+};
+static_assert(Shape<float, 128>::kAlloc <= 232448 && Shape<__nv_bfloat16, 128>::kAlloc <= 232448);
+
+// Descriptor of an MN-major operand tile: rows of 128 bytes (64 elements of the MN
+// dimension), 8-row groups of 1024 bytes along K, 64-element blocks kTileRows rows apart.
+__device__ __forceinline__ uint64_t mn_desc(uint32_t tile, uint32_t block_bytes) {
+    uint64_t d = (tile >> 4) & 0x3FFFull;
+    d |= uint64_t(block_bytes >> 4) << 16;
+    d |= uint64_t(1024 >> 4) << 32;
+    d |= uint64_t(1) << 46;
+    d |= uint64_t(2) << 61;
+    return d;
+}
+
+// D (TMEM) (+)= A (TMEM) . B, one K step of 16 FP16 elements.
+__device__ __forceinline__ void mma_f16_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
+        "r"(a), "l"(b), "r"(idesc), "r"(accumulate));
+}
+
+__device__ __forceinline__ void tmem_load16(uint32_t taddr, float (&r)[16]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
+        "%15}, [%16];"
+        : "=f"(r[0]), "=f"(r[1]), "=f"(r[2]), "=f"(r[3]), "=f"(r[4]), "=f"(r[5]), "=f"(r[6]), "=f"(r[7]), "=f"(r[8]),
+          "=f"(r[9]), "=f"(r[10]), "=f"(r[11]), "=f"(r[12]), "=f"(r[13]), "=f"(r[14]), "=f"(r[15])
+        : "r"(taddr));
+}
+__device__ __forceinline__ void tmem_store8(uint32_t taddr, const uint32_t (&r)[8]) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"r"(taddr), "r"(r[0]),
+                 "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
+                 : "memory");
+}
+__device__ __forceinline__ void tmem_wait_load() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void tmem_wait_store() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+// One item's tiles k0 .. k1 - 1 (of `tiles`), and what it covers.
+struct Segment {
+    int seq, row0, rows, position, head, k0, k1, tiles;
+    int64_t first;  // device-wide index of the item's tile 0
+};
+
+// The blocks of rows of all sequences in order, and a run of their tiles.
+struct Cursor {
+    const AttentionParams* p;
+    int block_rows;  // rows of a full item
+    int seq, block, head, k;
+    int64_t at;      // device-wide index of the next tile
+    int left;
+
+    // rows of sequence i, 0 for one whose metadata is out of range
+    static __device__ __forceinline__ int rows_of(const AttentionParams& p, int i, int& begin, int& start) {
+        begin = p.row_offsets[i], start = p.starts[i];
+        const int end = p.row_offsets[i + 1];
+        if (begin < 0 || end < begin || end > p.rows || (end > begin && start < 0) ||
+            int64_t(start) + (end - begin) > int64_t(p.table_stride) * p.cache.block_tokens) {
+            if (end != begin) raise_error(p.error, kErrBounds);
+            return 0;
+        }
+        return end - begin;
     }
-    const int len = int(end);
-    const int h0 = kh * group + sub * 8, heads = min(8, group - sub * 8);
-    WarpRow<T, F, D> w;
-    w.begin(static_cast<const T*>(p.q) + row * p.q_stride + h0 * D, heads, p.scale, lane);
-    const int32_t* table = p.tables + int64_t(seq) * p.table_stride;
-    const int n = lane >> 2, c = lane & 3;
-    for (int t = 0; t < len; t += kUnit) {
-        const unsigned char* at[kTiles];
-        float2 scale[kTiles];
+    static __device__ __forceinline__ int tiles_of(int start, int rows, int block, int block_rows) {
+        return (start + min((block + 1) * block_rows, rows) + kN - 1) / kN;
+    }
+    // The next segment; false when the run is done.
+    __device__ __forceinline__ bool next(Segment& s) {
+        if (left <= 0) return false;
+        int begin, start, rows = rows_of(*p, seq, begin, start);
+        while (block * block_rows >= rows) {
+            block = 0, head = 0, k = 0;
+            rows = rows_of(*p, ++seq, begin, start);
+        }
+        s.seq = seq, s.head = head;
+        s.row0 = begin + block * block_rows;
+        s.rows = min(block_rows, rows - block * block_rows);
+        s.position = start + block * block_rows;
+        s.tiles = tiles_of(start, rows, block, block_rows);
+        s.k0 = k, s.k1 = min(s.tiles, k + left);
+        s.first = at - k;
+        left -= s.k1 - s.k0, at += s.k1 - s.k0;
+        k = 0;
+        if (++head == p->cache.kv_heads) head = 0, ++block;
+        return true;
+    }
+};
+
+template <class T, int F, int D>
+__global__ void __launch_bounds__(kThreads, 1) prefill_kernel(const AttentionParams p) {
+    using S = Shape<T, D>;
+    constexpr int kHalves = S::kHalves, kStages = S::kStages;
+    extern __shared__ unsigned char smem_raw[];
+    unsigned char* sm = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    float2* scales = reinterpret_cast<float2*>(sm + S::kScales);
+    uint64_t* bars = reinterpret_cast<uint64_t*>(sm + S::kBars);
+    uint64_t *k_full = bars, *k_empty = bars + 2, *v_full = bars + 4, *v_empty = bars + 6;
+    uint64_t *q_full = bars + 8, *s_full = bars + 10, *p_full = bars + 12;  // per tile
+    uint64_t *scales_full = bars + 14, *joined = bars + 18;                 // per scale slot; per tile
+    uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(bars + 20);
+    int* failed = reinterpret_cast<int*>(bars + 21);
+    int* last = reinterpret_cast<int*>(bars + 22);  // [2] whether this CTA joins the parts, per tile
+    int64_t* units_before = reinterpret_cast<int64_t*>(sm + S::kPlan);       // [kThreads + 1]
+    int64_t* sums = units_before + kThreads + 1;                             // [16], [16]
+    int* blocks_before = reinterpret_cast<int*>(sums + 32);                  // [kThreads + 1]
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+
+    if (warp == 12) tmem_alloc(tmem_holder, S::kTmemCols);
+    if (tid == 0) {
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(k_full + i, 4), mbar_init(v_full + i, 4);
+            mbar_init(k_empty + i, 1), mbar_init(v_empty + i, 1);
+            mbar_init(q_full + i, kM), mbar_init(s_full + i, 1), mbar_init(p_full + i, kM), mbar_init(joined + i, kM);
+        }
+        for (int i = 0; i < kScaleSlots; ++i) mbar_init(scales_full + i, 1);
+        *failed = 0;
+        fence_barrier_init();
+    }
+    pdl_enter();
+
+    // ---- plan: blocks of rows of each thread's sequences, then tiles of each thread's blocks
+    const int group = p.heads / p.cache.kv_heads, tile_rows = kM / group, block_rows = 2 * tile_rows;
+    const int share = (p.count + kThreads - 1) / kThreads;
+    auto scan = [&](int64_t mine, int64_t* partial) {  // exclusive sum over the threads before
+        int64_t upto = mine;
 #pragma unroll
-        for (int u = 0; u < kTiles; ++u) {
-            const int token = t + u * kTile;
-            scale[u] = make_float2(0.f, 0.f);
-            at[u] = at[0];
-            if (token < len) {
-                const int block = block_id(p.cache, table, p.table_stride, token / bt, p.error);
-                scale[u] = *reinterpret_cast<const float2*>(p.cache.scales + block * p.cache.scale_stride + 2 * kh);
-                at[u] = p.cache.pages + tile_offset(p.cache, block, kh, 0, D) + (token % bt) * D;
+        for (int o = 1; o < 32; o <<= 1) {
+            const int64_t x = __shfl_up_sync(0xffffffffu, upto, o);
+            if (lane >= o) upto += x;
+        }
+        if (lane == 31) partial[warp] = upto;
+        __syncthreads();
+        int64_t x = lane < warp ? partial[lane] : 0;
+#pragma unroll
+        for (int o = 16; o; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
+        return x + upto - mine;
+    };
+    int begin, start;
+    {
+        int mine = 0;
+        for (int i = 0; i < share; ++i)
+            if (tid * share + i < p.count)
+                mine += (Cursor::rows_of(p, tid * share + i, begin, start) + block_rows - 1) / block_rows;
+        const int before = int(scan(mine, sums));
+        blocks_before[tid] = before;
+        if (tid == kThreads - 1) blocks_before[kThreads] = before + mine;
+        __syncthreads();
+    }
+    const int blocks = blocks_before[kThreads], each = (blocks + kThreads - 1) / kThreads;
+    // sequence and block of the flattened block index `f` (< blocks)
+    auto locate = [&](int f, int& seq, int& block) {
+        int t = 0;
+#pragma unroll
+        for (int o = kThreads / 2; o; o >>= 1)
+            if (blocks_before[t + o] <= f) t += o;
+        block = f - blocks_before[t];
+        for (seq = t * share;; ++seq) {
+            const int n = (Cursor::rows_of(p, seq, begin, start) + block_rows - 1) / block_rows;
+            if (block < n) return;
+            block -= n;
+        }
+    };
+    {
+        int64_t mine = 0;
+        if (tid * each < blocks) {
+            int seq, block;
+            locate(tid * each, seq, block);
+            int rows = Cursor::rows_of(p, seq, begin, start);
+            for (int i = 0; i < min(each, blocks - tid * each); ++i, ++block) {
+                while (block * block_rows >= rows) block = 0, rows = Cursor::rows_of(p, ++seq, begin, start);
+                mine += Cursor::tiles_of(start, rows, block, block_rows);
             }
         }
-        auto load_k = [&](int u, int i, int h) {
-            return *reinterpret_cast<const uint4*>(at[u] + w.token(i, n) * D + h * 64 + c * 16);
-        };
-        auto load_v = [&](int u, int q, uint32_t (&r)[4]) {
+        const int64_t before = scan(mine, sums + 16);
+        units_before[tid] = before;
+        if (tid == kThreads - 1) units_before[kThreads] = before + mine;
+        __syncthreads();
+    }
+    const int heads = p.cache.kv_heads;
+    const int64_t total = units_before[kThreads] * heads;
+    const int ctas = int(total < int64_t(gridDim.x) ? total : int64_t(gridDim.x));
+    const int64_t base = ctas ? (total >> 32 ? total / ctas : int64_t(uint32_t(total) / uint32_t(ctas))) : 0;
+    const int extra = int(total - base * ctas);
+    auto cta_of = [&](int64_t unit) {
+        const int64_t split = extra * (base + 1);
+        return int(unit < split ? unit / (base + 1) : extra + (unit - split) / base);
+    };
+    Cursor cursor{&p, block_rows, 0, 0, 0, 0, 0, 0};
+    cursor.left = int(blockIdx.x) < ctas ? int(base) + (int(blockIdx.x) < extra) : 0;
+    if (cursor.left) {
+        cursor.at = blockIdx.x * base + min(int(blockIdx.x), extra);
+        int t = 0;
 #pragma unroll
-            for (int g = 0; g < 4; ++g)
-                r[g] = transpose8x8(*reinterpret_cast<const uint32_t*>(at[u] + (bt + w.token(g & 1, n)) * D + 32 * q +
-                                                                       16 * (g >> 1) + 4 * c));
-        };
-        if (len - t >= kUnit) {
-            w.template step<false>(load_k, load_v, scale, kUnit, lane);
-        } else {
-            w.template step<true>(load_k, load_v, scale, len - t, lane);
+        for (int o = kThreads / 2; o; o >>= 1)
+            if (units_before[t + o] * heads <= cursor.at) t += o;
+        locate(t * each, cursor.seq, cursor.block);
+        int64_t in = cursor.at - units_before[t] * heads;
+        for (int rows = Cursor::rows_of(p, cursor.seq, begin, start);; ++cursor.block) {
+            while (cursor.block * block_rows >= rows) cursor.block = 0, rows = Cursor::rows_of(p, ++cursor.seq, begin, start);
+            const int n = Cursor::tiles_of(start, rows, cursor.block, block_rows);
+            if (in < int64_t(n) * heads) {
+                cursor.head = int(in) / n, cursor.k = int(in) % n;
+                break;
+            }
+            in -= int64_t(n) * heads;
         }
     }
-    w.end();
-    w.write(static_cast<T*>(p.out) + row * p.out_stride + h0 * D, heads, lane);
+    tmem_fence_before();
+    __syncthreads();
+    tmem_fence_after();
+    const uint32_t tmem = *tmem_holder;
+    // tiles of a segment that tile w's rows see: none if it has no rows
+    auto tiles_for = [&](const Segment& s, int w) {
+        const int rows = min(s.rows, (w + 1) * tile_rows);
+        return rows <= w * tile_rows ? 0 : max(0, min(s.k1, (s.position + rows + kN - 1) / kN) - s.k0);
+    };
+    // Bounded wait of one thread, or of a whole warp (whose lanes then agree). After a wait
+    // that expired every role leaves its loops at its next wait.
+    auto wait_one = [&](uint64_t* bar, uint32_t parity) {
+        if (*reinterpret_cast<volatile int*>(failed)) return false;
+        if (mbar_wait_bounded(bar, parity)) return true;
+        *reinterpret_cast<volatile int*>(failed) = 1;
+        raise_error(p.error, kErrTimeout);
+        return false;
+    };
+    auto wait = [&](uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, wait_one(bar, parity)) != 0; };
+
+    // registers: 2 x 128 x 200 + 128 x 72 + 128 x 40 = 512 x 128
+    if (warp < 8) {
+        // ================================================================ softmax, one thread per vector
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 200;");
+        const int w = warp >> 2, v = tid & (kM - 1);
+        const uint32_t lanes = uint32_t((warp & 3) * 32) << 16;
+        const uint32_t s_at = tmem + w * kN + lanes, o_at = tmem + 2 * kN + w * D + lanes;
+        const float sign = p.scale < 0.f ? -1.f : 1.f;  // the sign goes to q: scores' factors stay positive
+        uint32_t phase = 0, join_phase = 0;
+        int slot = 0;
+        Segment seg;
+        bool ok = true;
+        while (ok && cursor.next(seg)) {
+            const int tiles = tiles_for(seg, w), most = seg.k1 - seg.k0;
+            const int row = w * tile_rows + v / group;
+            const bool live = v < tile_rows * group && row < seg.rows;
+            const int position = seg.position + row, head = seg.head * group + v % group;
+            float o[D], m = -INFINITY, l = 0.f, unit = kUnitFloor, inv_unit = kWeightTop / kUnitFloor, k_factor = 0.f;
+#pragma unroll
+            for (int d = 0; d < D; ++d) o[d] = 0.f;
+            if (tiles) {
+                // ---- the query row as FP16 halves, K-major with the 128-byte swizzle
+                const T* q = static_cast<const T*>(p.q) + int64_t(seg.row0 + row) * p.q_stride + head * D;
+                float amax = 0.f;
+                if (live) {
+#pragma unroll
+                    for (int i = 0; i < D; i += 4) {
+                        float x[4];
+                        load4(q + i, x);
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) amax = fmaxf(amax, fabsf(x[j]));
+                    }
+                }
+                float factor, inverse;
+                row_factor(amax, factor, inverse);
+                k_factor = inverse * (p.scale * sign) * kLog2e;
+                factor *= sign;
+#pragma unroll
+                for (int i = 0; i < D; i += 8) {
+                    float x[8] = {};
+                    if (live) {
+                        load4(q + i, *reinterpret_cast<float(*)[4]>(x));
+                        load4(q + i + 4, *reinterpret_cast<float(*)[4]>(x + 4));
+                    }
+                    uint32_t hi[4], lo[4];
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) split_pair(x[2 * j] * factor, x[2 * j + 1] * factor, hi[j], lo[j]);
+                    unsigned char* to = sm + S::kQ + w * kHalves * S::kTileBytes + (i / 64) * (kM * 128) +
+                                        sw128_offset(v, (i % 64) / 8);
+                    *reinterpret_cast<uint4*>(to) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+                    if constexpr (kHalves == 2)
+                        *reinterpret_cast<uint4*>(to + S::kTileBytes) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+                }
+                fence_proxy_async_shared();
+                mbar_arrive(q_full + w);
+            }
+            // O of the previous tile: this thread's row
+            auto add_outputs = [&] {
+#pragma unroll
+                for (int i = 0; i < D; i += 16) {
+                    float x[16];
+                    tmem_load16(o_at + i, x);
+                    tmem_wait_load();
+#pragma unroll
+                    for (int j = 0; j < 16; ++j) o[i + j] += x[j];
+                }
+            };
+            for (int j = 0; j < tiles; ++j) {
+                if (!(ok = wait(s_full + w, phase))) break;
+                phase ^= 1;
+                tmem_fence_after();
+                if (j) add_outputs();
+                const int sl = (slot + j) % kScaleSlots;
+                if (!(ok = wait(scales_full + sl, ((slot + j) / kScaleSlots) & 1))) break;
+                const float2* scale = scales + sl * kGroups;
+                const int t0 = (seg.k0 + j) * kN;
+                const int visible = live ? min(max(position + 1 - t0, 0), kN) : 0;
+                const bool cut = __any_sync(0xffffffffu, visible < kN);
+                // largest score, largest weight times scale
+                auto largest_of = [&](int g) {  // of 16 scores, scaled
+                    float x[16];
+                    tmem_load16(s_at + g * 16, x);
+                    tmem_wait_load();
+                    if (cut) {
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) x[i] = g * 16 + i < visible ? x[i] : -INFINITY;
+                    }
+                    float big = x[0];
+#pragma unroll
+                    for (int i = 1; i < 16; ++i) big = fmaxf(big, x[i]);
+                    return g * 16 < visible ? big * (k_factor * scale[g].x) : -INFINITY;
+                };
+                float top = -INFINITY, most_scale = 0.f;
+#pragma unroll
+                for (int g = 0; g < kGroups; ++g) {
+                    top = fmaxf(top, largest_of(g));
+                    most_scale = fmaxf(most_scale, g * 16 < visible ? scale[g].y : 0.f);
+                }
+                if (__any_sync(0xffffffffu, top > m + kSlack || most_scale >= 2.f * unit)) {
+                    const float m_new = fmaxf(m, top);
+                    float reach = 0.f;  // largest weight times scale
+                    for (int g = 0; g < kGroups; ++g) {
+                        const float t = largest_of(g);
+                        if (t != -INFINITY) reach = fmaxf(reach, scale[g].y * ex2(t - m_new));
+                    }
+                    if (top > m + kSlack || reach >= 2.f * unit) {
+                        const float decay = m_new == -INFINITY ? 1.f : ex2(m - m_new);
+                        const float largest = fminf(fmaxf(fmaxf(unit * decay, reach), kUnitFloor), 8.507059e37f);
+                        const int e = (__float_as_int(largest) >> 23) - 127;
+                        const float by = decay * (unit * pow2(-e));
+                        l *= decay;
+#pragma unroll
+                        for (int d = 0; d < D; ++d) o[d] *= by;
+                        m = m_new, unit = pow2(e), inv_unit = kWeightTop * pow2(-e);
+                    }
+                }
+                const float base_m = m == -INFINITY ? 0.f : m;
+#pragma unroll
+                for (int g = 0; g < kGroups; ++g) {
+                    float x[16];
+                    tmem_load16(s_at + g * 16, x);
+                    tmem_wait_load();
+                    const float2 sc = scale[g];
+                    const float f = k_factor * sc.x;
+                    const float wt = g * 16 < visible ? sc.y * inv_unit : 0.f;
+                    float sum0 = 0.f, sum1 = 0.f;
+                    uint32_t hi[8], lo[8];
+#pragma unroll
+                    for (int i = 0; i < 16; i += 2) {
+                        float p0 = ex2(fmaf(x[i], f, -base_m)), p1 = ex2(fmaf(x[i + 1], f, -base_m));
+                        if (cut) {
+                            p0 = g * 16 + i < visible ? p0 : 0.f;
+                            p1 = g * 16 + i + 1 < visible ? p1 : 0.f;
+                        }
+                        sum0 += p0, sum1 += p1;
+                        if constexpr (kHalves == 2) {
+                            split_pair(p0 * wt, p1 * wt, hi[i / 2], lo[i / 2]);
+                        } else {
+                            const __half2 h = __floats2half2_rn(p0 * wt, p1 * wt);
+                            hi[i / 2] = *reinterpret_cast<const uint32_t*>(&h);
+                        }
+                    }
+                    l += sum0 + sum1;
+                    // over the scores just read: 16 columns hold 8 of high halves, 8 of low
+                    tmem_store8(s_at + g * 16, hi);
+                    if constexpr (kHalves == 2) tmem_store8(s_at + g * 16 + 8, lo);
+                }
+                tmem_wait_store();
+                tmem_fence_before();
+                mbar_arrive(p_full + w);
+            }
+            if (ok && tiles) {
+                if ((ok = wait(s_full + w, phase))) {
+                    phase ^= 1;
+                    tmem_fence_after();
+                    add_outputs();
+                    tmem_fence_before();
+                }
+            }
+            slot += most;
+            if (!ok) break;
+            const float u = unit * (1.f / kWeightTop);
+            T* out = static_cast<T*>(p.out) + int64_t(seg.row0 + row) * p.out_stride + head * D;
+            if (seg.k0 == 0 && seg.k1 == seg.tiles) {
+                if (live) {
+                    const float r = l == 0.f ? 0.f : u / l;
+#pragma unroll
+                    for (int d = 0; d < D; d += 4) store4(out + d, o[d] * r, o[d + 1] * r, o[d + 2] * r, o[d + 3] * r);
+                }
+                continue;
+            }
+            // ---- a part of the item: to the workspace; the last CTA to arrive joins them. Slot 0 of
+            // a CTA: the item began earlier, slot 1: it begins here. Vectors side by side.
+            constexpr int64_t kPart = int64_t(kM) * (D + 2);
+            unsigned* counters = static_cast<unsigned*>(p.workspace);
+            float* parts = reinterpret_cast<float*>(static_cast<unsigned char*>(p.workspace) + kCtas * 2 * 4 + 96);
+            auto part = [&](int cta, int which) { return parts + ((int64_t(cta) * 2 + which) * 2 + w) * kPart; };
+            float* mine = part(blockIdx.x, seg.k0 == 0);
+#pragma unroll
+            for (int d = 0; d < D; d += 4)
+                *reinterpret_cast<float4*>(mine + d * kM + v * 4) = make_float4(o[d] * u, o[d + 1] * u, o[d + 2] * u, o[d + 3] * u);
+            *reinterpret_cast<float2*>(mine + D * kM + v * 2) = make_float2(m, l);
+            __threadfence();
+            auto meet = [&] {  // the tile's 128 threads
+                mbar_arrive(joined + w);
+                ok = wait(joined + w, join_phase);
+                join_phase ^= 1;
+                return ok;
+            };
+            if (!meet()) break;
+            const int c0 = cta_of(seg.first), n = cta_of(seg.first + seg.tiles - 1) - c0 + 1;
+            if (v == 0) {
+                const bool mine_last = atomicAdd(counters + 2 * c0 + w, 1u) == unsigned(n - 1);
+                if (mine_last) counters[2 * c0 + w] = 0;
+                last[w] = mine_last;
+                __threadfence();
+            }
+            if (!meet()) break;
+            if (*reinterpret_cast<volatile int*>(last + w)) {
+                m = -INFINITY, l = 0.f;
+#pragma unroll
+                for (int d = 0; d < D; ++d) o[d] = 0.f;
+                for (int i = 0; i < n; ++i) {
+                    const float* from = part(c0 + i, i == 0);
+                    const float2 ml = __ldcg(reinterpret_cast<const float2*>(from + D * kM + v * 2));
+                    const float big = fmaxf(m, ml.x);
+                    const float a = m == big ? 1.f : ex2(m - big), b = ml.x == big ? 1.f : ex2(ml.x - big);
+                    l = l * a + ml.y * b;
+                    m = big;
+#pragma unroll
+                    for (int d = 0; d < D; d += 4) {
+                        const float4 x = __ldcg(reinterpret_cast<const float4*>(from + d * kM + v * 4));
+                        o[d] = fmaf(o[d], a, x.x * b), o[d + 1] = fmaf(o[d + 1], a, x.y * b);
+                        o[d + 2] = fmaf(o[d + 2], a, x.z * b), o[d + 3] = fmaf(o[d + 3], a, x.w * b);
+                    }
+                }
+                if (live) {
+                    const float r = l == 0.f ? 0.f : 1.f / l;
+#pragma unroll
+                    for (int d = 0; d < D; d += 4) store4(out + d, o[d] * r, o[d + 1] * r, o[d + 2] * r, o[d + 3] * r);
+                }
+            }
+            if (!meet()) break;  // `last` may be written again
+        }
+    } else if (warp < 12) {
+        // ================================================================ codes -> FP16 tiles
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+        const int t = tid & 127, bt = p.cache.block_tokens;
+        constexpr int kWords = kN * D / 16 / 128;  // 16-byte words of a thread per tile
+        constexpr int kChunks = D / 16;            // words of a token
+        int slot = 0;
+        Segment seg;
+        bool ok = true;
+        while (ok && cursor.next(seg)) {
+            const int32_t* table = p.tables + int64_t(seg.seq) * p.table_stride;
+            const int len = seg.position + seg.rows;
+            for (int k = seg.k0; ok && k < seg.k1; ++k, ++slot) {
+                const int stage = slot % kStages;
+                const uint32_t parity = ((slot / kStages) & 1) ^ 1;
+                const unsigned char* from[kWords];
+#pragma unroll
+                for (int i = 0; i < kWords; ++i) {
+                    const int token = k * kN + (t + i * 128) / kChunks;
+                    from[i] = nullptr;
+                    if (token < len) {
+                        const int block = block_id(p.cache, table, p.table_stride, token / bt, p.error);
+                        from[i] = p.cache.pages + tile_offset(p.cache, block, seg.head, 0, D) + (token % bt) * D + t % kChunks * 16;
+                    }
+                }
+#pragma unroll
+                for (int part = 0; part < 2; ++part) {
+                    uint4 c[kWords];
+#pragma unroll
+                    for (int i = 0; i < kWords; ++i)
+                        c[i] = from[i] ? __ldg(reinterpret_cast<const uint4*>(from[i] + part * bt * D)) : make_uint4(0, 0, 0, 0);
+                    if (part == 0 && t < kGroups) {
+                        const int token = k * kN + t * kGroupTokens;
+                        float2 s = make_float2(0.f, 0.f);
+                        if (token < len) {
+                            const int block = block_id(p.cache, table, p.table_stride, token / bt, p.error);
+                            s = *reinterpret_cast<const float2*>(p.cache.scales + block * p.cache.scale_stride + 2 * seg.head);
+                        }
+                        scales[slot % kScaleSlots * kGroups + t] = s;
+                    }
+                    if (part == 0 && warp == 8) {
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(scales_full + slot % kScaleSlots);
+                    }
+                    if (!(ok = wait((part ? v_empty : k_empty) + stage, parity))) break;
+                    unsigned char* tile = sm + (part ? S::kV : S::kK) + stage * S::kTileBytes;
+#pragma unroll
+                    for (int i = 0; i < kWords; ++i) {
+                        const int token = (t + i * 128) / kChunks, chunk = t % kChunks;
+                        uint32_t h[8];
+                        widen4<F>(c[i].x, h[0], h[1]);
+                        widen4<F>(c[i].y, h[2], h[3]);
+                        widen4<F>(c[i].z, h[4], h[5]);
+                        widen4<F>(c[i].w, h[6], h[7]);
+                        unsigned char* to = tile + (chunk / 4) * (kN * 128);
+                        *reinterpret_cast<uint4*>(to + sw128_offset(token, 2 * (chunk % 4))) = make_uint4(h[0], h[1], h[2], h[3]);
+                        *reinterpret_cast<uint4*>(to + sw128_offset(token, 2 * (chunk % 4) + 1)) = make_uint4(h[4], h[5], h[6], h[7]);
+                    }
+                    fence_proxy_async_shared();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive((part ? v_full : k_full) + stage);
+                }
+            }
+        }
+    } else {
+        // ================================================================ products
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
+        if (warp == 12 && lane == 0) {
+            constexpr uint32_t kIdescS = umma_idesc_f16<kM, kN>();
+            constexpr uint32_t kIdescO = umma_idesc_f16<kM, D>() | (1u << 16);  // B is MN-major
+            int slot = 0;
+            uint32_t q_phase = 0, p_phase = 0;  // one bit per tile
+            Segment seg;
+            bool ok = true;
+            while (ok && cursor.next(seg)) {
+                const int most = seg.k1 - seg.k0;
+                const int n0 = tiles_for(seg, 0), n1 = tiles_for(seg, 1);
+                for (int j = 0; ok && j <= most; ++j) {
+                    const int sj = (slot + j) % kStages, sp = (slot + j + kStages - 1) % kStages;  // this tile's, the last's
+                    if (j < most) ok = wait_one(k_full + sj, ((slot + j) / kStages) & 1);
+                    if (ok && j) ok = wait_one(v_full + sp, ((slot + j - 1) / kStages) & 1);
+                    for (int w = 0; ok && w < 2; ++w) {
+                        const int n = w ? n1 : n0;
+                        if (j > n || n == 0) continue;
+                        const uint32_t s_at = tmem + w * kN, o_at = tmem + 2 * kN + w * D;
+                        if (j == 0) {
+                            if (!(ok = wait_one(q_full + w, (q_phase >> w) & 1))) break;
+                            q_phase ^= 1u << w;
+                        } else {
+                            if (!(ok = wait_one(p_full + w, (p_phase >> w) & 1))) break;
+                            p_phase ^= 1u << w;
+                        }
+                        tmem_fence_after();
+                        if (j) {
+                            const uint32_t v_at = smem_u32(sm + S::kV + sp * S::kTileBytes);
+#pragma unroll
+                            for (int half = kHalves - 1; half >= 0; --half)
+#pragma unroll
+                                for (int i = 0; i < kN / 16; ++i)
+                                    mma_f16_ts(o_at, s_at + i * 16 + half * 8, mn_desc(v_at + i * 2048, kN * 128), kIdescO,
+                                               half != kHalves - 1 || i != 0);
+                        }
+                        if (j < n) {
+                            const unsigned char* kt = sm + S::kK + sj * S::kTileBytes;
+                            const unsigned char* qt = sm + S::kQ + w * kHalves * S::kTileBytes;
+#pragma unroll
+                            for (int half = kHalves - 1; half >= 0; --half)
+#pragma unroll
+                                for (int i = 0; i < D / 16; ++i)
+                                    mma_f16(s_at,
+                                            smem_desc(qt + half * S::kTileBytes + (i / 4) * (kM * 128)) + uint64_t(i % 4 * 2),
+                                            smem_desc(kt + (i / 4) * (kN * 128)) + uint64_t(i % 4 * 2), kIdescS,
+                                            half != kHalves - 1 || i != 0);
+                        }
+                        mma_commit(s_full + w);
+                    }
+                    if (!ok) break;
+                    if (j < most) mma_commit(k_empty + sj);
+                    if (j) mma_commit(v_empty + sp);
+                }
+                slot += most;
+            }
+        }
+        __syncwarp();
+    }
+    tmem_fence_before();
+    __syncthreads();
+    if (warp == 12) {
+        tmem_fence_after();
+        tmem_dealloc(tmem, S::kTmemCols);
+    }
 }
 
 }  // namespace
 
-size_t prefill_workspace(int, int) { return 256; }
+size_t prefill_workspace(int, int head_dim) {
+    return kCtas * 2 * 4 + 96 + size_t(kCtas) * 4 * kM * (head_dim + 2) * 4;
+}
 
 cudaError_t launch_prefill(const AttentionParams& p, int type, int format, int head_dim, cudaStream_t stream) {
-    const int64_t items = int64_t(p.rows) * p.cache.kv_heads * ((p.heads / p.cache.kv_heads + 7) / 8);
     return dispatch(type, format, head_dim, [&](auto t, auto f, auto d) {
-        return launch_pdl(row_kernel<decltype(t), decltype(f)::value, decltype(d)::value>,
-                          dim3(unsigned((items + 3) / 4)), dim3(kThreads), 0, stream, p);
+        using S = Shape<decltype(t), decltype(d)::value>;
+        auto kernel = prefill_kernel<decltype(t), decltype(f)::value, decltype(d)::value>;
+        const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kAlloc);
+        if (e != cudaSuccess) return e;
+        return launch_pdl(kernel, dim3(kCtas), dim3(kThreads), S::kAlloc, stream, p);
     });
 }
 
