@@ -4,8 +4,9 @@
 // A work item is (block of rows of one sequence, kv head): rows x query heads of the group
 // fill two 128-vector tiles (vector v of a tile: row v / group, head v % group), and its
 // context is a run of 128-token K/V tiles. All items' tiles, in order, are dealt out in
-// equal runs to one CTA per SM, so a long context with few rows is shared like many short
-// ones; the device plans this itself from row_offsets and starts.
+// equal runs to one CTA per SM (an item counts kSetup tiles more, for its queries and
+// outputs), so a long context with few rows is shared like many short ones; the device plans
+// this itself from row_offsets and starts.
 //
 // Roles of a CTA (16 warps):
 //  * warps 8-11 widen K and V codes to FP16 tiles in shared memory (exact; K token-major,
@@ -15,6 +16,9 @@
 //  * warps 0-3 and 4-7 own one tile each, a thread per vector: running softmax of S's
 //    row, weights written over S in place, O's rows added up.
 // While one tile's threads work on their S, the tensor core runs the other's O and S.
+//
+// Outputs: FP32 ones are added up in registers, tile by tile; BF16 ones stay in tensor
+// memory over an item's tiles.
 //
 // FP32 precision: the query is two FP16 halves (each row scaled by a power of two towards
 // FP16's top), so S is two products per useful one; the weights, with V's scales folded
@@ -39,6 +43,7 @@ constexpr int kN = 128;       // tokens of a K/V tile
 // Scale rows in flight. Row j + 4 is written after P V of tile j + 1 completed (its V slot
 // was needed for tile j + 3), so every thread has read row j by then.
 constexpr int kScaleSlots = 4;
+constexpr int kSetup = 2;     // an item's start and end cost about this many tiles
 constexpr int kGroupTokens = 16;  // tokens that share a block's scales at least
 constexpr int kGroups = kN / kGroupTokens;
 constexpr float kWeightTop = 4096.f, kSlack = 2.f, kUnitFloor = 7.70371977754894e-34f;  // as in kv8_warp.cuh
@@ -47,6 +52,7 @@ template <class T, int D>
 struct Shape {
     static constexpr int kHalves = sizeof(T) == 4 ? 2 : 1;              // FP16 halves of q and of the weights
     static constexpr int kTileBytes = kM * D * 2;                       // one FP16 tile
+    static constexpr bool kAdd = kHalves == 2;                          // O starts anew with every tile
     static constexpr int kStages = kHalves == 2 && D == 128 ? 1 : 2;    // K (and V) tiles in shared memory
     static constexpr int kQ = 0;                                        // [2 tiles][halves]
     static constexpr int kK = kQ + 2 * kHalves * kTileBytes;
@@ -56,6 +62,10 @@ struct Shape {
     static constexpr int kPlan = kBars + 32 * 8;                        // planning, and a few words
     static constexpr int kSmem = kPlan + (kThreads + 1) * 4 + (kThreads + 1) * 8 + 2 * 16 * 8 + 64;
     static constexpr int kAlloc = kSmem + 1024;                         // alignment slack
+    // registers a thread of each role: together the 512 x 128 of the launch
+    static constexpr int kSoftmaxRegs = D == 64 ? 160 : kHalves == 1 ? 168 : 184;
+    static constexpr int kWidenRegs = D == 64 ? 104 : kHalves == 1 ? 104 : 80;
+    static constexpr int kProductRegs = 512 - 2 * kSoftmaxRegs - kWidenRegs;
     static constexpr uint32_t kTmemCols = 512;                          // S: 2 x 128, O: 2 x D
 };
 static_assert(Shape<float, 128>::kAlloc <= 232448 && Shape<__nv_bfloat16, 128>::kAlloc <= 232448);
@@ -96,18 +106,33 @@ __device__ __forceinline__ void tmem_store8(uint32_t taddr, const uint32_t (&r)[
 __device__ __forceinline__ void tmem_wait_load() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void tmem_wait_store() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
+// Two or four values of a row, or zeros.
+__device__ __forceinline__ void load_few(const float* p, bool on, float (&x)[2]) {
+    const float2 v = on ? *reinterpret_cast<const float2*>(p) : make_float2(0.f, 0.f);
+    x[0] = v.x, x[1] = v.y;
+}
+__device__ __forceinline__ void load_few(const __nv_bfloat16* p, bool on, float (&x)[2]) {
+    const uint32_t v = on ? *reinterpret_cast<const uint32_t*>(p) : 0u;
+    x[0] = __uint_as_float(v << 16), x[1] = __uint_as_float(v & 0xffff0000u);
+}
+template <class T>
+__device__ __forceinline__ void load_few(const T* p, bool on, float (&x)[4]) {
+    x[0] = x[1] = x[2] = x[3] = 0.f;
+    if (on) load4(p, x);
+}
+
 // One item's tiles k0 .. k1 - 1 (of `tiles`), and what it covers.
 struct Segment {
     int seq, row0, rows, position, head, k0, k1, tiles;
-    int64_t first;  // device-wide index of the item's tile 0
+    int64_t first;  // device-wide index of the item's first unit (its tiles follow kSetup units)
 };
 
 // The blocks of rows of all sequences in order, and a run of their tiles.
 struct Cursor {
     const AttentionParams* p;
     int block_rows;  // rows of a full item
-    int seq, block, head, k;
-    int64_t at;      // device-wide index of the next tile
+    int seq, block, head, k;  // k: unit of the item, kSetup + tile
+    int64_t at;               // device-wide index of the next unit
     int left;
 
     // rows of sequence i, 0 for one whose metadata is out of range
@@ -121,11 +146,17 @@ struct Cursor {
         }
         return end - begin;
     }
-    static __device__ __forceinline__ int tiles_of(int start, int rows, int block, int block_rows) {
-        return (start + min((block + 1) * block_rows, rows) + kN - 1) / kN;
+    static __device__ __forceinline__ int units_of(int start, int rows, int block, int block_rows) {
+        return kSetup + (start + min((block + 1) * block_rows, rows) + kN - 1) / kN;
     }
     // The next segment; false when the run is done.
     __device__ __forceinline__ bool next(Segment& s) {
+        do
+            if (!advance(s)) return false;
+        while (s.k0 >= s.k1);  // the run ends within an item's set-up units
+        return true;
+    }
+    __device__ __forceinline__ bool advance(Segment& s) {
         if (left <= 0) return false;
         int begin, start, rows = rows_of(*p, seq, begin, start);
         while (block * block_rows >= rows) {
@@ -136,10 +167,11 @@ struct Cursor {
         s.row0 = begin + block * block_rows;
         s.rows = min(block_rows, rows - block * block_rows);
         s.position = start + block * block_rows;
-        s.tiles = tiles_of(start, rows, block, block_rows);
-        s.k0 = k, s.k1 = min(s.tiles, k + left);
+        const int units = units_of(start, rows, block, block_rows), end = min(units, k + left);
+        s.tiles = units - kSetup;
+        s.k0 = max(k - kSetup, 0), s.k1 = end - kSetup;
         s.first = at - k;
-        left -= s.k1 - s.k0, at += s.k1 - s.k0;
+        left -= end - k, at += end - k;
         k = 0;
         if (++head == p->cache.kv_heads) head = 0, ++block;
         return true;
@@ -178,7 +210,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_kernel(const AttentionPar
     }
     pdl_enter();
 
-    // ---- plan: blocks of rows of each thread's sequences, then tiles of each thread's blocks
+    // ---- plan: blocks of rows of each thread's sequences, then units of each thread's blocks
     const int group = p.heads / p.cache.kv_heads, tile_rows = kM / group, block_rows = 2 * tile_rows;
     const int share = (p.count + kThreads - 1) / kThreads;
     auto scan = [&](int64_t mine, int64_t* partial) {  // exclusive sum over the threads before
@@ -228,7 +260,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_kernel(const AttentionPar
             int rows = Cursor::rows_of(p, seq, begin, start);
             for (int i = 0; i < min(each, blocks - tid * each); ++i, ++block) {
                 while (block * block_rows >= rows) block = 0, rows = Cursor::rows_of(p, ++seq, begin, start);
-                mine += Cursor::tiles_of(start, rows, block, block_rows);
+                mine += Cursor::units_of(start, rows, block, block_rows);
             }
         }
         const int64_t before = scan(mine, sums + 16);
@@ -257,7 +289,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_kernel(const AttentionPar
         int64_t in = cursor.at - units_before[t] * heads;
         for (int rows = Cursor::rows_of(p, cursor.seq, begin, start);; ++cursor.block) {
             while (cursor.block * block_rows >= rows) cursor.block = 0, rows = Cursor::rows_of(p, ++cursor.seq, begin, start);
-            const int n = Cursor::tiles_of(start, rows, cursor.block, block_rows);
+            const int n = Cursor::units_of(start, rows, cursor.block, block_rows);
             if (in < int64_t(n) * heads) {
                 cursor.head = int(in) / n, cursor.k = int(in) % n;
                 break;
@@ -285,10 +317,9 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_kernel(const AttentionPar
     };
     auto wait = [&](uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, wait_one(bar, parity)) != 0; };
 
-    // registers: 2 x 128 x 200 + 128 x 72 + 128 x 40 = 512 x 128
     if (warp < 8) {
         // ================================================================ softmax, one thread per vector
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 200;");
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(S::kSoftmaxRegs));
         const int w = warp >> 2, v = tid & (kM - 1);
         const uint32_t lanes = uint32_t((warp & 3) * 32) << 16;
         const uint32_t s_at = tmem + w * kN + lanes, o_at = tmem + 2 * kN + w * D + lanes;
@@ -301,62 +332,68 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_kernel(const AttentionPar
             const int tiles = tiles_for(seg, w), most = seg.k1 - seg.k0;
             const int row = w * tile_rows + v / group;
             const bool live = v < tile_rows * group && row < seg.rows;
-            const int position = seg.position + row, head = seg.head * group + v % group;
+            const int position = seg.position + row;
             float o[D], m = -INFINITY, l = 0.f, unit = kUnitFloor, inv_unit = kWeightTop / kUnitFloor, k_factor = 0.f;
 #pragma unroll
             for (int d = 0; d < D; ++d) o[d] = 0.f;
             if (tiles) {
-                // ---- the query row as FP16 halves, K-major with the 128-byte swizzle
-                const T* q = static_cast<const T*>(p.q) + int64_t(seg.row0 + row) * p.q_stride + head * D;
-                float amax = 0.f;
-                if (live) {
+                // ---- query rows as FP16 halves, K-major with the 128-byte swizzle: the warp reads its 32
+                // vectors one by one, D / 32 values a lane, four in flight
+                constexpr int kPer = D / 32;
+                const int v0 = v & ~31;
+#pragma unroll 1
+                for (int r = 0; r < 32; r += 4) {
+                    float x[4][kPer];
 #pragma unroll
-                    for (int i = 0; i < D; i += 4) {
-                        float x[4];
-                        load4(q + i, x);
-#pragma unroll
-                        for (int j = 0; j < 4; ++j) amax = fmaxf(amax, fabsf(x[j]));
+                    for (int i = 0; i < 4; ++i) {
+                        const int vec = v0 + r + i, of = w * tile_rows + vec / group;
+                        const bool on = vec < tile_rows * group && of < seg.rows;
+                        const T* q = static_cast<const T*>(p.q) + int64_t(seg.row0 + of) * p.q_stride +
+                                     (seg.head * group + vec % group) * D + lane * kPer;
+                        load_few(q, on, x[i]);
                     }
-                }
-                float factor, inverse;
-                row_factor(amax, factor, inverse);
-                k_factor = inverse * (p.scale * sign) * kLog2e;
-                factor *= sign;
 #pragma unroll
-                for (int i = 0; i < D; i += 8) {
-                    float x[8] = {};
-                    if (live) {
-                        load4(q + i, *reinterpret_cast<float(*)[4]>(x));
-                        load4(q + i + 4, *reinterpret_cast<float(*)[4]>(x + 4));
+                    for (int i = 0; i < 4; ++i) {
+                        float amax = fabsf(x[i][0]);
+#pragma unroll
+                        for (int c = 1; c < kPer; ++c) amax = fmaxf(amax, fabsf(x[i][c]));
+                        amax = warp_max(amax);
+                        float factor, inverse;
+                        row_factor(amax, factor, inverse);
+                        if (lane == r + i) k_factor = inverse * (p.scale * sign) * kLog2e;
+                        factor *= sign;
+                        const int d = lane * kPer;
+                        unsigned char* to = sm + S::kQ + w * kHalves * S::kTileBytes + (d / 64) * (kM * 128) +
+                                            sw128_offset(v0 + r + i, (d % 64) / 8) + (d % 8) * 2;
+#pragma unroll
+                        for (int c = 0; c < kPer; c += 2) {
+                            uint32_t hi, lo;
+                            split_pair(x[i][c] * factor, x[i][c + 1] * factor, hi, lo);
+                            *reinterpret_cast<uint32_t*>(to + 2 * c) = hi;
+                            if constexpr (kHalves == 2) *reinterpret_cast<uint32_t*>(to + S::kTileBytes + 2 * c) = lo;
+                        }
                     }
-                    uint32_t hi[4], lo[4];
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) split_pair(x[2 * j] * factor, x[2 * j + 1] * factor, hi[j], lo[j]);
-                    unsigned char* to = sm + S::kQ + w * kHalves * S::kTileBytes + (i / 64) * (kM * 128) +
-                                        sw128_offset(v, (i % 64) / 8);
-                    *reinterpret_cast<uint4*>(to) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-                    if constexpr (kHalves == 2)
-                        *reinterpret_cast<uint4*>(to + S::kTileBytes) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
                 }
                 fence_proxy_async_shared();
                 mbar_arrive(q_full + w);
             }
-            // O of the previous tile: this thread's row
+            // O's row of this thread: two groups of 16 columns in flight
             auto add_outputs = [&] {
 #pragma unroll
-                for (int i = 0; i < D; i += 16) {
-                    float x[16];
+                for (int i = 0; i < D; i += 32) {
+                    float x[16], y[16];
                     tmem_load16(o_at + i, x);
+                    tmem_load16(o_at + i + 16, y);
                     tmem_wait_load();
 #pragma unroll
-                    for (int j = 0; j < 16; ++j) o[i + j] += x[j];
+                    for (int j = 0; j < 16; ++j) o[i + j] += x[j], o[i + 16 + j] += y[j];
                 }
             };
             for (int j = 0; j < tiles; ++j) {
                 if (!(ok = wait(s_full + w, phase))) break;
                 phase ^= 1;
                 tmem_fence_after();
-                if (j) add_outputs();
+                if (S::kAdd && j) add_outputs();
                 const int sl = (slot + j) % kScaleSlots;
                 if (!(ok = wait(scales_full + sl, ((slot + j) / kScaleSlots) & 1))) break;
                 const float2* scale = scales + sl * kGroups;
@@ -364,49 +401,65 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_kernel(const AttentionPar
                 const int visible = live ? min(max(position + 1 - t0, 0), kN) : 0;
                 const bool cut = __any_sync(0xffffffffu, visible < kN);
                 // largest score, largest weight times scale
-                auto largest_of = [&](int g) {  // of 16 scores, scaled
-                    float x[16];
-                    tmem_load16(s_at + g * 16, x);
-                    tmem_wait_load();
-                    if (cut) {
-#pragma unroll
-                        for (int i = 0; i < 16; ++i) x[i] = g * 16 + i < visible ? x[i] : -INFINITY;
+                // f(x, g) for every group of 16 scores, the next group's load in flight
+                auto each_group = [&](auto f) {
+                    float x[16], y[16];
+                    tmem_load16(s_at, x);
+#pragma unroll 1
+                    for (int g = 0; g < kGroups; g += 2) {
+                        tmem_wait_load();
+                        tmem_load16(s_at + g * 16 + 16, y);
+                        f(x, g);
+                        tmem_wait_load();
+                        if (g + 2 < kGroups) tmem_load16(s_at + g * 16 + 32, x);
+                        f(y, g + 1);
                     }
-                    float big = x[0];
+                };
+                auto largest_of = [&](float (&x)[16], int g) {  // scaled
+                    float big = cut && g * 16 >= visible ? -INFINITY : x[0];
 #pragma unroll
-                    for (int i = 1; i < 16; ++i) big = fmaxf(big, x[i]);
+                    for (int i = 1; i < 16; ++i) big = fmaxf(big, cut && g * 16 + i >= visible ? -INFINITY : x[i]);
                     return g * 16 < visible ? big * (k_factor * scale[g].x) : -INFINITY;
                 };
                 float top = -INFINITY, most_scale = 0.f;
-#pragma unroll
-                for (int g = 0; g < kGroups; ++g) {
-                    top = fmaxf(top, largest_of(g));
+                each_group([&](float (&x)[16], int g) {
+                    top = fmaxf(top, largest_of(x, g));
                     most_scale = fmaxf(most_scale, g * 16 < visible ? scale[g].y : 0.f);
-                }
+                });
                 if (__any_sync(0xffffffffu, top > m + kSlack || most_scale >= 2.f * unit)) {
                     const float m_new = fmaxf(m, top);
                     float reach = 0.f;  // largest weight times scale
-                    for (int g = 0; g < kGroups; ++g) {
-                        const float t = largest_of(g);
+                    each_group([&](float (&x)[16], int g) {
+                        const float t = largest_of(x, g);
                         if (t != -INFINITY) reach = fmaxf(reach, scale[g].y * ex2(t - m_new));
-                    }
+                    });
+                    float by = 1.f;
                     if (top > m + kSlack || reach >= 2.f * unit) {
                         const float decay = m_new == -INFINITY ? 1.f : ex2(m - m_new);
                         const float largest = fminf(fmaxf(fmaxf(unit * decay, reach), kUnitFloor), 8.507059e37f);
                         const int e = (__float_as_int(largest) >> 23) - 127;
-                        const float by = decay * (unit * pow2(-e));
+                        by = decay * (unit * pow2(-e));
                         l *= decay;
+                        m = m_new, unit = pow2(e), inv_unit = kWeightTop * pow2(-e);
+                    }
+                    if constexpr (S::kAdd) {
 #pragma unroll
                         for (int d = 0; d < D; ++d) o[d] *= by;
-                        m = m_new, unit = pow2(e), inv_unit = kWeightTop * pow2(-e);
+                    } else if (j) {
+#pragma unroll 1
+                        for (int i = 0; i < D; i += 16) {
+                            float x[16];
+                            tmem_load16(o_at + i, x);
+                            tmem_wait_load();
+#pragma unroll
+                            for (int c = 0; c < 16; ++c) x[c] *= by;
+                            tmem_store8(o_at + i, *reinterpret_cast<uint32_t(*)[8]>(x));
+                            tmem_store8(o_at + i + 8, *reinterpret_cast<uint32_t(*)[8]>(x + 8));
+                        }
                     }
                 }
                 const float base_m = m == -INFINITY ? 0.f : m;
-#pragma unroll
-                for (int g = 0; g < kGroups; ++g) {
-                    float x[16];
-                    tmem_load16(s_at + g * 16, x);
-                    tmem_wait_load();
+                each_group([&](float (&x)[16], int g) {
                     const float2 sc = scale[g];
                     const float f = k_factor * sc.x;
                     const float wt = g * 16 < visible ? sc.y * inv_unit : 0.f;
@@ -431,29 +484,47 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_kernel(const AttentionPar
                     // over the scores just read: 16 columns hold 8 of high halves, 8 of low
                     tmem_store8(s_at + g * 16, hi);
                     if constexpr (kHalves == 2) tmem_store8(s_at + g * 16 + 8, lo);
-                }
+                });
                 tmem_wait_store();
                 tmem_fence_before();
                 mbar_arrive(p_full + w);
             }
-            if (ok && tiles) {
-                if ((ok = wait(s_full + w, phase))) {
-                    phase ^= 1;
-                    tmem_fence_after();
-                    add_outputs();
-                    tmem_fence_before();
-                }
+            if (ok && tiles && (ok = wait(s_full + w, phase))) {
+                phase ^= 1;
+                tmem_fence_after();
+                add_outputs();
+                tmem_fence_before();
             }
             slot += most;
             if (!ok) break;
             const float u = unit * (1.f / kWeightTop);
-            T* out = static_cast<T*>(p.out) + int64_t(seg.row0 + row) * p.out_stride + head * D;
-            if (seg.k0 == 0 && seg.k1 == seg.tiles) {
-                if (live) {
-                    const float r = l == 0.f ? 0.f : u / l;
+            // rows out through this tile's query buffer (its products are done): the warp's 32 rows,
+            // 16-byte words XOR-ed by the row against bank conflicts, then row by row
+            auto write_rows = [&](float r) {
+                constexpr int kWords = D * int(sizeof(T)) / 16, kEach = 16 / int(sizeof(T));
+                unsigned char* stage = sm + S::kQ + w * kHalves * S::kTileBytes + (v & ~31) * (kWords * 16);
 #pragma unroll
-                    for (int d = 0; d < D; d += 4) store4(out + d, o[d] * r, o[d + 1] * r, o[d + 2] * r, o[d + 3] * r);
+                for (int i = 0; i < kWords; ++i) {
+                    T* to = reinterpret_cast<T*>(stage + lane * (kWords * 16) + (i ^ (lane & 7)) * 16);
+#pragma unroll
+                    for (int c = 0; c < kEach; c += 4)
+                        store4(to + c, o[i * kEach + c] * r, o[i * kEach + c + 1] * r, o[i * kEach + c + 2] * r, o[i * kEach + c + 3] * r);
                 }
+                __syncwarp();
+#pragma unroll 4
+                for (int i = lane; i < 32 * kWords; i += 32) {
+                    const int from = i / kWords, word = i % kWords, vec = (v & ~31) + from, of = w * tile_rows + vec / group;
+                    if (vec < tile_rows * group && of < seg.rows) {
+                        T* out = static_cast<T*>(p.out) + int64_t(seg.row0 + of) * p.out_stride +
+                                 (seg.head * group + vec % group) * D;
+                        reinterpret_cast<uint4*>(out)[word] =
+                            *reinterpret_cast<const uint4*>(stage + from * (kWords * 16) + (word ^ (from & 7)) * 16);
+                    }
+                }
+                __syncwarp();
+            };
+            if (seg.k0 == 0 && seg.k1 == seg.tiles) {
+                if (tiles) write_rows(l == 0.f ? 0.f : u / l);
                 continue;
             }
             // ---- a part of the item: to the workspace; the last CTA to arrive joins them. Slot 0 of
@@ -475,7 +546,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_kernel(const AttentionPar
                 return ok;
             };
             if (!meet()) break;
-            const int c0 = cta_of(seg.first), n = cta_of(seg.first + seg.tiles - 1) - c0 + 1;
+            const int c0 = cta_of(seg.first + kSetup), n = cta_of(seg.first + kSetup + seg.tiles - 1) - c0 + 1;
             if (v == 0) {
                 const bool mine_last = atomicAdd(counters + 2 * c0 + w, 1u) == unsigned(n - 1);
                 if (mine_last) counters[2 * c0 + w] = 0;
@@ -501,68 +572,75 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_kernel(const AttentionPar
                         o[d + 2] = fmaf(o[d + 2], a, x.z * b), o[d + 3] = fmaf(o[d + 3], a, x.w * b);
                     }
                 }
-                if (live) {
-                    const float r = l == 0.f ? 0.f : 1.f / l;
-#pragma unroll
-                    for (int d = 0; d < D; d += 4) store4(out + d, o[d] * r, o[d + 1] * r, o[d + 2] * r, o[d + 3] * r);
-                }
+                write_rows(l == 0.f ? 0.f : 1.f / l);
             }
             if (!meet()) break;  // `last` may be written again
         }
     } else if (warp < 12) {
         // ================================================================ codes -> FP16 tiles
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(S::kWidenRegs));
         const int t = tid & 127, bt = p.cache.block_tokens;
         constexpr int kWords = kN * D / 16 / 128;  // 16-byte words of a thread per tile
         constexpr int kChunks = D / 16;            // words of a token
+        const int word = t % kChunks * 16;
         int slot = 0;
         Segment seg;
         bool ok = true;
         while (ok && cursor.next(seg)) {
             const int32_t* table = p.tables + int64_t(seg.seq) * p.table_stride;
             const int len = seg.position + seg.rows;
-            for (int k = seg.k0; ok && k < seg.k1; ++k, ++slot) {
-                const int stage = slot % kStages;
-                const uint32_t parity = ((slot / kStages) & 1) ^ 1;
-                const unsigned char* from[kWords];
+            // blocks of this thread's words of tile k (-1: behind the last token), and the block whose scales it
+            // brings; the codes of the tile in work. Both are loaded a tile ahead.
+            int block[kWords], scale_block;
+            uint4 code[2][kWords];
+            float2 scale;
+            auto blocks_of = [&](int k) {
 #pragma unroll
                 for (int i = 0; i < kWords; ++i) {
                     const int token = k * kN + (t + i * 128) / kChunks;
-                    from[i] = nullptr;
-                    if (token < len) {
-                        const int block = block_id(p.cache, table, p.table_stride, token / bt, p.error);
-                        from[i] = p.cache.pages + tile_offset(p.cache, block, seg.head, 0, D) + (token % bt) * D + t % kChunks * 16;
-                    }
+                    block[i] = k < seg.k1 && token < len ? block_id(p.cache, table, p.table_stride, token / bt, p.error) : -1;
                 }
+                const int token = k * kN + t * kGroupTokens;
+                scale_block = t < kGroups && k < seg.k1 && token < len ? block_id(p.cache, table, p.table_stride, token / bt, p.error) : -1;
+            };
+            auto load = [&](int k, int part) {
+#pragma unroll
+                for (int i = 0; i < kWords; ++i) {
+                    const int token = k * kN + (t + i * 128) / kChunks;
+                    code[part][i] = block[i] < 0 ? make_uint4(0, 0, 0, 0)
+                                                 : __ldg(reinterpret_cast<const uint4*>(
+                                                       p.cache.pages + tile_offset(p.cache, block[i], seg.head, part, D) +
+                                                       token % bt * D + word));
+                }
+                if (part == 0) {
+                    scale = make_float2(0.f, 0.f);
+                    if (scale_block >= 0)
+                        scale = *reinterpret_cast<const float2*>(p.cache.scales + scale_block * p.cache.scale_stride + 2 * seg.head);
+                }
+            };
+            blocks_of(seg.k0);
+            load(seg.k0, 0);
+            load(seg.k0, 1);
+            blocks_of(seg.k0 + 1);
+            for (int k = seg.k0; ok && k < seg.k1; ++k, ++slot) {
+                const int stage = slot % kStages;
+                const uint32_t parity = ((slot / kStages) & 1) ^ 1;
+                if (t < kGroups) scales[slot % kScaleSlots * kGroups + t] = scale;
+                __syncwarp();
+                if (t == 0) mbar_arrive(scales_full + slot % kScaleSlots);
 #pragma unroll
                 for (int part = 0; part < 2; ++part) {
-                    uint4 c[kWords];
-#pragma unroll
-                    for (int i = 0; i < kWords; ++i)
-                        c[i] = from[i] ? __ldg(reinterpret_cast<const uint4*>(from[i] + part * bt * D)) : make_uint4(0, 0, 0, 0);
-                    if (part == 0 && t < kGroups) {
-                        const int token = k * kN + t * kGroupTokens;
-                        float2 s = make_float2(0.f, 0.f);
-                        if (token < len) {
-                            const int block = block_id(p.cache, table, p.table_stride, token / bt, p.error);
-                            s = *reinterpret_cast<const float2*>(p.cache.scales + block * p.cache.scale_stride + 2 * seg.head);
-                        }
-                        scales[slot % kScaleSlots * kGroups + t] = s;
-                    }
-                    if (part == 0 && warp == 8) {
-                        __syncwarp();
-                        if (lane == 0) mbar_arrive(scales_full + slot % kScaleSlots);
-                    }
                     if (!(ok = wait((part ? v_empty : k_empty) + stage, parity))) break;
                     unsigned char* tile = sm + (part ? S::kV : S::kK) + stage * S::kTileBytes;
 #pragma unroll
                     for (int i = 0; i < kWords; ++i) {
                         const int token = (t + i * 128) / kChunks, chunk = t % kChunks;
+                        const uint4 c = code[part][i];
                         uint32_t h[8];
-                        widen4<F>(c[i].x, h[0], h[1]);
-                        widen4<F>(c[i].y, h[2], h[3]);
-                        widen4<F>(c[i].z, h[4], h[5]);
-                        widen4<F>(c[i].w, h[6], h[7]);
+                        widen4<F>(c.x, h[0], h[1]);
+                        widen4<F>(c.y, h[2], h[3]);
+                        widen4<F>(c.z, h[4], h[5]);
+                        widen4<F>(c.w, h[6], h[7]);
                         unsigned char* to = tile + (chunk / 4) * (kN * 128);
                         *reinterpret_cast<uint4*>(to + sw128_offset(token, 2 * (chunk % 4))) = make_uint4(h[0], h[1], h[2], h[3]);
                         *reinterpret_cast<uint4*>(to + sw128_offset(token, 2 * (chunk % 4) + 1)) = make_uint4(h[4], h[5], h[6], h[7]);
@@ -570,15 +648,20 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_kernel(const AttentionPar
                     fence_proxy_async_shared();
                     __syncwarp();
                     if (lane == 0) mbar_arrive((part ? v_full : k_full) + stage);
+                    load(k + 1, part);
                 }
+                blocks_of(k + 2);
             }
         }
     } else {
         // ================================================================ products
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(S::kProductRegs));
         if (warp == 12 && lane == 0) {
             constexpr uint32_t kIdescS = umma_idesc_f16<kM, kN>();
             constexpr uint32_t kIdescO = umma_idesc_f16<kM, D>() | (1u << 16);  // B is MN-major
+            // descriptors' low bits are addresses / 16: adding moves them
+            const uint64_t q_desc = smem_desc(sm + S::kQ), k_desc = smem_desc(sm + S::kK);
+            const uint64_t v_desc = mn_desc(smem_u32(sm + S::kV), kN * 128);
             int slot = 0;
             uint32_t q_phase = 0, p_phase = 0;  // one bit per tile
             Segment seg;
@@ -603,24 +686,23 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_kernel(const AttentionPar
                         }
                         tmem_fence_after();
                         if (j) {
-                            const uint32_t v_at = smem_u32(sm + S::kV + sp * S::kTileBytes);
+                            const uint64_t vd = v_desc + uint64_t(sp * (S::kTileBytes >> 4));
 #pragma unroll
                             for (int half = kHalves - 1; half >= 0; --half)
 #pragma unroll
                                 for (int i = 0; i < kN / 16; ++i)
-                                    mma_f16_ts(o_at, s_at + i * 16 + half * 8, mn_desc(v_at + i * 2048, kN * 128), kIdescO,
-                                               half != kHalves - 1 || i != 0);
+                                    mma_f16_ts(o_at, s_at + i * 16 + half * 8, vd + uint64_t(i * (2048 >> 4)), kIdescO,
+                                               half != kHalves - 1 || i != 0 || (!S::kAdd && j > 1));
                         }
                         if (j < n) {
-                            const unsigned char* kt = sm + S::kK + sj * S::kTileBytes;
-                            const unsigned char* qt = sm + S::kQ + w * kHalves * S::kTileBytes;
+                            const uint64_t kd = k_desc + uint64_t(sj * (S::kTileBytes >> 4));
+                            const uint64_t qd = q_desc + uint64_t(w * kHalves * (S::kTileBytes >> 4));
 #pragma unroll
                             for (int half = kHalves - 1; half >= 0; --half)
 #pragma unroll
                                 for (int i = 0; i < D / 16; ++i)
-                                    mma_f16(s_at,
-                                            smem_desc(qt + half * S::kTileBytes + (i / 4) * (kM * 128)) + uint64_t(i % 4 * 2),
-                                            smem_desc(kt + (i / 4) * (kN * 128)) + uint64_t(i % 4 * 2), kIdescS,
+                                    mma_f16(s_at, qd + uint64_t(half * (S::kTileBytes >> 4) + (i / 4) * (kM * 128 >> 4) + i % 4 * 2),
+                                            kd + uint64_t((i / 4) * (kN * 128 >> 4) + i % 4 * 2), kIdescS,
                                             half != kHalves - 1 || i != 0);
                         }
                         mma_commit(s_full + w);
