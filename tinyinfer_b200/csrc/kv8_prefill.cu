@@ -57,8 +57,8 @@ struct Shape {
     static constexpr int kQ = 0;                                        // [2 tiles][halves]
     static constexpr int kK = kQ + 2 * kHalves * kTileBytes;
     static constexpr int kV = kK + kStages * kTileBytes;
-    static constexpr int kScales = kV + kStages * kTileBytes;           // [slots][groups] (K, V)
-    static constexpr int kBars = kScales + kScaleSlots * kGroups * 8;
+    static constexpr int kScales = kV + kStages * kTileBytes;           // [slots][groups] K, V, log2 V, 1 / V
+    static constexpr int kBars = kScales + kScaleSlots * kGroups * 16;
     static constexpr int kPlan = kBars + 32 * 8;                        // planning, and a few words
     static constexpr int kSmem = kPlan + (kThreads + 1) * 4 + (kThreads + 1) * 8 + 2 * 16 * 8 + 64;
     static constexpr int kAlloc = kSmem + 1024;                         // alignment slack
@@ -90,12 +90,29 @@ __device__ __forceinline__ void mma_f16_ts(uint32_t d, uint32_t a, uint64_t b, u
         "r"(a), "l"(b), "r"(idesc), "r"(accumulate));
 }
 
-__device__ __forceinline__ void tmem_load16(uint32_t taddr, float (&r)[16]) {
+// Columns of this warp's TMEM lanes, waited for: a register of a load in flight must not be
+// moved, and the compiler does not know that it is.
+__device__ __forceinline__ void tmem_load(uint32_t taddr, float (&r)[16]) {
     asm volatile(
-        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
-        "%15}, [%16];"
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {"
+        "%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15"
+        "}, [%16];\n\t"
+        "tcgen05.wait::ld.sync.aligned;"
         : "=f"(r[0]), "=f"(r[1]), "=f"(r[2]), "=f"(r[3]), "=f"(r[4]), "=f"(r[5]), "=f"(r[6]), "=f"(r[7]), "=f"(r[8]),
           "=f"(r[9]), "=f"(r[10]), "=f"(r[11]), "=f"(r[12]), "=f"(r[13]), "=f"(r[14]), "=f"(r[15])
+        : "r"(taddr));
+}
+__device__ __forceinline__ void tmem_load(uint32_t taddr, float (&r)[32]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {"
+        "%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24,"
+        "%25, %26, %27, %28, %29, %30, %31"
+        "}, [%32];\n\t"
+        "tcgen05.wait::ld.sync.aligned;"
+        : "=f"(r[0]), "=f"(r[1]), "=f"(r[2]), "=f"(r[3]), "=f"(r[4]), "=f"(r[5]), "=f"(r[6]), "=f"(r[7]), "=f"(r[8]),
+          "=f"(r[9]), "=f"(r[10]), "=f"(r[11]), "=f"(r[12]), "=f"(r[13]), "=f"(r[14]), "=f"(r[15]), "=f"(r[16]),
+          "=f"(r[17]), "=f"(r[18]), "=f"(r[19]), "=f"(r[20]), "=f"(r[21]), "=f"(r[22]), "=f"(r[23]), "=f"(r[24]),
+          "=f"(r[25]), "=f"(r[26]), "=f"(r[27]), "=f"(r[28]), "=f"(r[29]), "=f"(r[30]), "=f"(r[31])
         : "r"(taddr));
 }
 __device__ __forceinline__ void tmem_store8(uint32_t taddr, const uint32_t (&r)[8]) {
@@ -103,8 +120,30 @@ __device__ __forceinline__ void tmem_store8(uint32_t taddr, const uint32_t (&r)[
                  "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
                  : "memory");
 }
-__device__ __forceinline__ void tmem_wait_load() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void tmem_wait_store() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+// Packed FP32 pairs: x * f + c, and a += b.
+__device__ __forceinline__ float2 fma_pair(float x0, float x1, float f, float c) {
+    float2 r;
+    asm("{\n\t.reg .b64 x, f, c;\n\t"
+        "mov.b64 x, {%2, %3};\n\t"
+        "mov.b64 f, {%4, %4};\n\t"
+        "mov.b64 c, {%5, %5};\n\t"
+        "fma.rn.f32x2 x, x, f, c;\n\t"
+        "mov.b64 {%0, %1}, x;\n\t}"
+        : "=f"(r.x), "=f"(r.y)
+        : "f"(x0), "f"(x1), "f"(f), "f"(c));
+    return r;
+}
+__device__ __forceinline__ void add_pair(float& a0, float& a1, float b0, float b1) {
+    asm("{\n\t.reg .b64 a, b;\n\t"
+        "mov.b64 a, {%0, %1};\n\t"
+        "mov.b64 b, {%2, %3};\n\t"
+        "add.rn.f32x2 a, a, b;\n\t"
+        "mov.b64 {%0, %1}, a;\n\t}"
+        : "+f"(a0), "+f"(a1)
+        : "f"(b0), "f"(b1));
+}
 
 // Two or four values of a row, or zeros.
 __device__ __forceinline__ void load_few(const float* p, bool on, float (&x)[2]) {
@@ -184,7 +223,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_kernel(const AttentionPar
     constexpr int kHalves = S::kHalves, kStages = S::kStages;
     extern __shared__ unsigned char smem_raw[];
     unsigned char* sm = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-    float2* scales = reinterpret_cast<float2*>(sm + S::kScales);
+    float4* scales = reinterpret_cast<float4*>(sm + S::kScales);
     uint64_t* bars = reinterpret_cast<uint64_t*>(sm + S::kBars);
     uint64_t *k_full = bars, *k_empty = bars + 2, *v_full = bars + 4, *v_empty = bars + 6;
     uint64_t *q_full = bars + 8, *s_full = bars + 10, *p_full = bars + 12;  // per tile
@@ -333,7 +372,8 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_kernel(const AttentionPar
             const int row = w * tile_rows + v / group;
             const bool live = v < tile_rows * group && row < seg.rows;
             const int position = seg.position + row;
-            float o[D], m = -INFINITY, l = 0.f, unit = kUnitFloor, inv_unit = kWeightTop / kUnitFloor, k_factor = 0.f;
+            float o[D], m = -INFINITY, l = 0.f, unit = kUnitFloor, k_factor = 0.f;
+            int unit_log = -110;
 #pragma unroll
             for (int d = 0; d < D; ++d) o[d] = 0.f;
             if (tiles) {
@@ -377,16 +417,14 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_kernel(const AttentionPar
                 fence_proxy_async_shared();
                 mbar_arrive(q_full + w);
             }
-            // O's row of this thread: two groups of 16 columns in flight
+            // O's row of this thread
             auto add_outputs = [&] {
 #pragma unroll
-                for (int i = 0; i < D; i += 32) {
-                    float x[16], y[16];
-                    tmem_load16(o_at + i, x);
-                    tmem_load16(o_at + i + 16, y);
-                    tmem_wait_load();
+                for (int i = 0; i < D; i += 16) {
+                    float x[16];
+                    tmem_load(o_at + i, x);
 #pragma unroll
-                    for (int j = 0; j < 16; ++j) o[i + j] += x[j], o[i + 16 + j] += y[j];
+                    for (int j = 0; j < 16; j += 2) add_pair(o[i + j], o[i + j + 1], x[j], x[j + 1]);
                 }
             };
             for (int j = 0; j < tiles; ++j) {
@@ -396,95 +434,111 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_kernel(const AttentionPar
                 if (S::kAdd && j) add_outputs();
                 const int sl = (slot + j) % kScaleSlots;
                 if (!(ok = wait(scales_full + sl, ((slot + j) / kScaleSlots) & 1))) break;
-                const float2* scale = scales + sl * kGroups;
+                const float4* scale = scales + sl * kGroups;
                 const int t0 = (seg.k0 + j) * kN;
                 const int visible = live ? min(max(position + 1 - t0, 0), kN) : 0;
                 const bool cut = __any_sync(0xffffffffu, visible < kN);
                 // largest score, largest weight times scale
-                // f(x, g) for every group of 16 scores, the next group's load in flight
+                // f(x, g) for every group of 16 scores, kAtOnce of them per load
+                constexpr int kAtOnce = S::kAdd && D == 128 ? 1 : 2;
                 auto each_group = [&](auto f) {
-                    float x[16], y[16];
-                    tmem_load16(s_at, x);
 #pragma unroll 1
-                    for (int g = 0; g < kGroups; g += 2) {
-                        tmem_wait_load();
-                        tmem_load16(s_at + g * 16 + 16, y);
-                        f(x, g);
-                        tmem_wait_load();
-                        if (g + 2 < kGroups) tmem_load16(s_at + g * 16 + 32, x);
-                        f(y, g + 1);
+                    for (int g = 0; g < kGroups; g += kAtOnce) {
+                        float x[16 * kAtOnce];
+                        tmem_load(s_at + g * 16, x);
+#pragma unroll
+                        for (int i = 0; i < kAtOnce; ++i) f(*reinterpret_cast<float(*)[16]>(x + 16 * i), g + i);
                     }
                 };
-                auto largest_of = [&](float (&x)[16], int g) {  // scaled
-                    float big = cut && g * 16 >= visible ? -INFINITY : x[0];
+                // the tile's weights; kCut: some row of the warp does not see all of its tokens
+                auto weigh = [&](auto is_cut) {
+                    constexpr bool kCut = decltype(is_cut)::value;
+                    auto largest_of = [&](float (&x)[16], int g) {  // scaled
+                        if constexpr (kCut) {
 #pragma unroll
-                    for (int i = 1; i < 16; ++i) big = fmaxf(big, cut && g * 16 + i >= visible ? -INFINITY : x[i]);
-                    return g * 16 < visible ? big * (k_factor * scale[g].x) : -INFINITY;
-                };
-                float top = -INFINITY, most_scale = 0.f;
-                each_group([&](float (&x)[16], int g) {
-                    top = fmaxf(top, largest_of(x, g));
-                    most_scale = fmaxf(most_scale, g * 16 < visible ? scale[g].y : 0.f);
-                });
-                if (__any_sync(0xffffffffu, top > m + kSlack || most_scale >= 2.f * unit)) {
-                    const float m_new = fmaxf(m, top);
-                    float reach = 0.f;  // largest weight times scale
+                            for (int i = 0; i < 16; ++i) x[i] = g * 16 + i < visible ? x[i] : -INFINITY;
+                        }
+                        float big = x[0];
+#pragma unroll
+                        for (int i = 1; i < 16; ++i) big = fmaxf(big, x[i]);
+                        return kCut && g * 16 >= visible ? -INFINITY : big * (k_factor * scale[g].x);
+                    };
+                    float top = -INFINITY, most_scale = 0.f;
                     each_group([&](float (&x)[16], int g) {
-                        const float t = largest_of(x, g);
-                        if (t != -INFINITY) reach = fmaxf(reach, scale[g].y * ex2(t - m_new));
+                        top = fmaxf(top, largest_of(x, g));
+                        most_scale = fmaxf(most_scale, kCut && g * 16 >= visible ? 0.f : scale[g].y);
                     });
-                    float by = 1.f;
-                    if (top > m + kSlack || reach >= 2.f * unit) {
-                        const float decay = m_new == -INFINITY ? 1.f : ex2(m - m_new);
-                        const float largest = fminf(fmaxf(fmaxf(unit * decay, reach), kUnitFloor), 8.507059e37f);
-                        const int e = (__float_as_int(largest) >> 23) - 127;
-                        by = decay * (unit * pow2(-e));
-                        l *= decay;
-                        m = m_new, unit = pow2(e), inv_unit = kWeightTop * pow2(-e);
-                    }
-                    if constexpr (S::kAdd) {
+                    if (__any_sync(0xffffffffu, top > m + kSlack || most_scale >= 2.f * unit)) {
+                        const float m_new = fmaxf(m, top);
+                        float reach = 0.f;  // largest weight times scale
+                        each_group([&](float (&x)[16], int g) {
+                            const float t = largest_of(x, g);
+                            if (t != -INFINITY) reach = fmaxf(reach, scale[g].y * ex2(t - m_new));
+                        });
+                        float by = 1.f;
+                        if (top > m + kSlack || reach >= 2.f * unit) {
+                            const float decay = m_new == -INFINITY ? 1.f : ex2(m - m_new);
+                            const float largest = fminf(fmaxf(fmaxf(unit * decay, reach), kUnitFloor), 8.507059e37f);
+                            unit_log = (__float_as_int(largest) >> 23) - 127;
+                            by = decay * (unit * pow2(-unit_log));
+                            l *= decay;
+                            m = m_new, unit = pow2(unit_log);
+                        }
+                        if constexpr (S::kAdd) {
 #pragma unroll
-                        for (int d = 0; d < D; ++d) o[d] *= by;
-                    } else if (j) {
+                            for (int d = 0; d < D; ++d) o[d] *= by;
+                        } else if (j) {
 #pragma unroll 1
-                        for (int i = 0; i < D; i += 16) {
-                            float x[16];
-                            tmem_load16(o_at + i, x);
-                            tmem_wait_load();
+                            for (int i = 0; i < D; i += 16) {
+                                float x[16];
+                                tmem_load(o_at + i, x);
 #pragma unroll
-                            for (int c = 0; c < 16; ++c) x[c] *= by;
-                            tmem_store8(o_at + i, *reinterpret_cast<uint32_t(*)[8]>(x));
-                            tmem_store8(o_at + i + 8, *reinterpret_cast<uint32_t(*)[8]>(x + 8));
+                                for (int c = 0; c < 16; ++c) x[c] *= by;
+                                tmem_store8(o_at + i, *reinterpret_cast<uint32_t(*)[8]>(x));
+                                tmem_store8(o_at + i + 8, *reinterpret_cast<uint32_t(*)[8]>(x + 8));
+                            }
                         }
                     }
+                    // weight * V scale = 2^(score - m + log2 scale - log2 unit + 12). A scale below unit * 2^-40
+                    // counts as that: its weights are zero in FP16 either way, but l needs them
+                    const float base_m = m == -INFINITY ? 0.f : m, shift = 12.f - float(unit_log);
+                    const float least = fmaxf(unit * 9.094947e-13f, 1.17549435e-38f);
+                    each_group([&](float (&x)[16], int g) {
+                        const float4 sc = scale[g];
+                        const bool small = sc.y < least;
+                        const float f = k_factor * sc.x;
+                        const float c = (small ? -28.f : sc.z + shift) - base_m;
+                        const float back = small ? 268435456.f : sc.w * (unit * (1.f / kWeightTop));
+                        float sum0 = 0.f, sum1 = 0.f;
+                        uint32_t hi[8];
+                        [[maybe_unused]] uint32_t lo[8];
+#pragma unroll
+                        for (int i = 0; i < 16; i += 2) {
+                            const float2 t = fma_pair(x[i], x[i + 1], f, c);
+                            float p0 = ex2(t.x), p1 = ex2(t.y);
+                            if constexpr (kCut) {
+                                p0 = g * 16 + i < visible ? p0 : 0.f;
+                                p1 = g * 16 + i + 1 < visible ? p1 : 0.f;
+                            }
+                            add_pair(sum0, sum1, p0, p1);
+                            if constexpr (kHalves == 2) {
+                                split_pair(p0, p1, hi[i / 2], lo[i / 2]);
+                            } else {
+                                const __half2 h = __floats2half2_rn(p0, p1);
+                                hi[i / 2] = *reinterpret_cast<const uint32_t*>(&h);
+                            }
+                        }
+                        l = fmaf(sum0 + sum1, kCut && g * 16 >= visible ? 0.f : back, l);
+                        // over the scores just read: 16 columns hold 8 of high halves, 8 of low
+                        tmem_store8(s_at + g * 16, hi);
+                        if constexpr (kHalves == 2) tmem_store8(s_at + g * 16 + 8, lo);
+                    });
+                };
+                if (cut) {
+                    weigh(std::true_type{});
+                } else {
+                    weigh(std::false_type{});
                 }
-                const float base_m = m == -INFINITY ? 0.f : m;
-                each_group([&](float (&x)[16], int g) {
-                    const float2 sc = scale[g];
-                    const float f = k_factor * sc.x;
-                    const float wt = g * 16 < visible ? sc.y * inv_unit : 0.f;
-                    float sum0 = 0.f, sum1 = 0.f;
-                    uint32_t hi[8], lo[8];
-#pragma unroll
-                    for (int i = 0; i < 16; i += 2) {
-                        float p0 = ex2(fmaf(x[i], f, -base_m)), p1 = ex2(fmaf(x[i + 1], f, -base_m));
-                        if (cut) {
-                            p0 = g * 16 + i < visible ? p0 : 0.f;
-                            p1 = g * 16 + i + 1 < visible ? p1 : 0.f;
-                        }
-                        sum0 += p0, sum1 += p1;
-                        if constexpr (kHalves == 2) {
-                            split_pair(p0 * wt, p1 * wt, hi[i / 2], lo[i / 2]);
-                        } else {
-                            const __half2 h = __floats2half2_rn(p0 * wt, p1 * wt);
-                            hi[i / 2] = *reinterpret_cast<const uint32_t*>(&h);
-                        }
-                    }
-                    l += sum0 + sum1;
-                    // over the scores just read: 16 columns hold 8 of high halves, 8 of low
-                    tmem_store8(s_at + g * 16, hi);
-                    if constexpr (kHalves == 2) tmem_store8(s_at + g * 16 + 8, lo);
-                });
                 tmem_wait_store();
                 tmem_fence_before();
                 mbar_arrive(p_full + w);
@@ -582,50 +636,55 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_kernel(const AttentionPar
         const int t = tid & 127, bt = p.cache.block_tokens;
         constexpr int kWords = kN * D / 16 / 128;  // 16-byte words of a thread per tile
         constexpr int kChunks = D / 16;            // words of a token
-        const int word = t % kChunks * 16;
+        const int first_token = t / kChunks, chunk = t % kChunks, in_page = bt / kGroupTokens;
+        const int own = first_token % kGroupTokens * D + chunk * 16;
+        // the word's 16 FP16 values in a tile: two 16-byte chunks of the token's row
+        const int to0 = (chunk / 4) * (kN * 128) + int(sw128_offset(first_token, 2 * (chunk % 4)));
+        const int to1 = (chunk / 4) * (kN * 128) + int(sw128_offset(first_token, 2 * (chunk % 4) + 1));
         int slot = 0;
         Segment seg;
         bool ok = true;
         while (ok && cursor.next(seg)) {
             const int32_t* table = p.tables + int64_t(seg.seq) * p.table_stride;
             const int len = seg.position + seg.rows;
-            // blocks of this thread's words of tile k (-1: behind the last token), and the block whose scales it
-            // brings; the codes of the tile in work. Both are loaded a tile ahead.
-            int block[kWords], scale_block;
+            // Lane g < 8 finds the block of tile k's 16 tokens from 16 g on: the offset of their K
+            // rows (V's are one block of rows on) and their scales. Codes and scales are loaded a tile
+            // ahead, offsets two.
+            int64_t offset = 0;
+            float2 scale, next_scale;
             uint4 code[2][kWords];
-            float2 scale;
-            auto blocks_of = [&](int k) {
-#pragma unroll
-                for (int i = 0; i < kWords; ++i) {
-                    const int token = k * kN + (t + i * 128) / kChunks;
-                    block[i] = k < seg.k1 && token < len ? block_id(p.cache, table, p.table_stride, token / bt, p.error) : -1;
+            auto find = [&](int k) {
+                const int tile = k * kGroups + lane;
+                next_scale = make_float2(0.f, 0.f);
+                if (lane < kGroups && k < seg.k1 && tile * kGroupTokens < len) {
+                    const int block = block_id(p.cache, table, p.table_stride, tile / in_page, p.error);
+                    offset = tile_offset(p.cache, block, seg.head, 0, D) + tile % in_page * (kGroupTokens * D);
+                    if (warp == 8)
+                        next_scale = *reinterpret_cast<const float2*>(p.cache.scales + block * p.cache.scale_stride + 2 * seg.head);
                 }
-                const int token = k * kN + t * kGroupTokens;
-                scale_block = t < kGroups && k < seg.k1 && token < len ? block_id(p.cache, table, p.table_stride, token / bt, p.error) : -1;
             };
             auto load = [&](int k, int part) {
+                const int left = k < seg.k1 ? len - k * kN : 0;  // tokens of the tile
 #pragma unroll
                 for (int i = 0; i < kWords; ++i) {
-                    const int token = k * kN + (t + i * 128) / kChunks;
-                    code[part][i] = block[i] < 0 ? make_uint4(0, 0, 0, 0)
-                                                 : __ldg(reinterpret_cast<const uint4*>(
-                                                       p.cache.pages + tile_offset(p.cache, block[i], seg.head, part, D) +
-                                                       token % bt * D + word));
-                }
-                if (part == 0) {
-                    scale = make_float2(0.f, 0.f);
-                    if (scale_block >= 0)
-                        scale = *reinterpret_cast<const float2*>(p.cache.scales + scale_block * p.cache.scale_stride + 2 * seg.head);
+                    const int group_of = first_token / kGroupTokens + i * (kN / kWords) / kGroupTokens;
+                    const int64_t at = __shfl_sync(0xffffffffu, offset, group_of);
+                    code[part][i] = make_uint4(0, 0, 0, 0);
+                    if (first_token + i * (kN / kWords) < left)
+                        code[part][i] = __ldg(reinterpret_cast<const uint4*>(p.cache.pages + at + part * bt * D + own));
                 }
             };
-            blocks_of(seg.k0);
+            find(seg.k0);
             load(seg.k0, 0);
             load(seg.k0, 1);
-            blocks_of(seg.k0 + 1);
+            scale = next_scale;
+            find(seg.k0 + 1);
             for (int k = seg.k0; ok && k < seg.k1; ++k, ++slot) {
                 const int stage = slot % kStages;
                 const uint32_t parity = ((slot / kStages) & 1) ^ 1;
-                if (t < kGroups) scales[slot % kScaleSlots * kGroups + t] = scale;
+                if (t < kGroups)
+                    scales[slot % kScaleSlots * kGroups + t] =
+                        make_float4(scale.x, scale.y, __log2f(scale.y), scale.y == 0.f ? 0.f : 1.f / scale.y);
                 __syncwarp();
                 if (t == 0) mbar_arrive(scales_full + slot % kScaleSlots);
 #pragma unroll
@@ -634,23 +693,23 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_kernel(const AttentionPar
                     unsigned char* tile = sm + (part ? S::kV : S::kK) + stage * S::kTileBytes;
 #pragma unroll
                     for (int i = 0; i < kWords; ++i) {
-                        const int token = (t + i * 128) / kChunks, chunk = t % kChunks;
                         const uint4 c = code[part][i];
                         uint32_t h[8];
                         widen4<F>(c.x, h[0], h[1]);
                         widen4<F>(c.y, h[2], h[3]);
                         widen4<F>(c.z, h[4], h[5]);
                         widen4<F>(c.w, h[6], h[7]);
-                        unsigned char* to = tile + (chunk / 4) * (kN * 128);
-                        *reinterpret_cast<uint4*>(to + sw128_offset(token, 2 * (chunk % 4))) = make_uint4(h[0], h[1], h[2], h[3]);
-                        *reinterpret_cast<uint4*>(to + sw128_offset(token, 2 * (chunk % 4) + 1)) = make_uint4(h[4], h[5], h[6], h[7]);
+                        unsigned char* to = tile + i * (kN / kWords) * 128;  // whole groups of 8 rows on: same swizzle
+                        *reinterpret_cast<uint4*>(to + to0) = make_uint4(h[0], h[1], h[2], h[3]);
+                        *reinterpret_cast<uint4*>(to + to1) = make_uint4(h[4], h[5], h[6], h[7]);
                     }
                     fence_proxy_async_shared();
                     __syncwarp();
                     if (lane == 0) mbar_arrive((part ? v_full : k_full) + stage);
                     load(k + 1, part);
                 }
-                blocks_of(k + 2);
+                scale = next_scale;
+                find(k + 2);
             }
         }
     } else {
