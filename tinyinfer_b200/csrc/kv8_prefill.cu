@@ -63,8 +63,8 @@ struct Shape {
     static constexpr int kSmem = kPlan + (kThreads + 1) * 4 + (kThreads + 1) * 8 + 2 * 16 * 8 + 64;
     static constexpr int kAlloc = kSmem + 1024;                         // alignment slack
     // registers a thread of each role: together the 512 x 128 of the launch
-    static constexpr int kSoftmaxRegs = D == 64 ? 160 : kHalves == 1 ? 168 : 184;
-    static constexpr int kWidenRegs = D == 64 ? 104 : kHalves == 1 ? 104 : 80;
+    static constexpr int kSoftmaxRegs = D == 64 ? 168 : kHalves == 1 ? 168 : 184;
+    static constexpr int kWidenRegs = D == 64 ? 96 : kHalves == 1 ? 104 : 80;
     static constexpr int kProductRegs = 512 - 2 * kSoftmaxRegs - kWidenRegs;
     static constexpr uint32_t kTmemCols = 512;                          // S: 2 x 128, O: 2 x D
 };
@@ -98,8 +98,8 @@ __device__ __forceinline__ void tmem_load(uint32_t taddr, float (&r)[16]) {
         "%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15"
         "}, [%16];\n\t"
         "tcgen05.wait::ld.sync.aligned;"
-        : "=f"(r[0]), "=f"(r[1]), "=f"(r[2]), "=f"(r[3]), "=f"(r[4]), "=f"(r[5]), "=f"(r[6]), "=f"(r[7]), "=f"(r[8]),
-          "=f"(r[9]), "=f"(r[10]), "=f"(r[11]), "=f"(r[12]), "=f"(r[13]), "=f"(r[14]), "=f"(r[15])
+        : "=f"(r[0]), "=f"(r[1]), "=f"(r[2]), "=f"(r[3]), "=f"(r[4]), "=f"(r[5]), "=f"(r[6]), "=f"(r[7]),
+          "=f"(r[8]), "=f"(r[9]), "=f"(r[10]), "=f"(r[11]), "=f"(r[12]), "=f"(r[13]), "=f"(r[14]), "=f"(r[15])
         : "r"(taddr));
 }
 __device__ __forceinline__ void tmem_load(uint32_t taddr, float (&r)[32]) {
@@ -109,12 +109,23 @@ __device__ __forceinline__ void tmem_load(uint32_t taddr, float (&r)[32]) {
         "%25, %26, %27, %28, %29, %30, %31"
         "}, [%32];\n\t"
         "tcgen05.wait::ld.sync.aligned;"
-        : "=f"(r[0]), "=f"(r[1]), "=f"(r[2]), "=f"(r[3]), "=f"(r[4]), "=f"(r[5]), "=f"(r[6]), "=f"(r[7]), "=f"(r[8]),
-          "=f"(r[9]), "=f"(r[10]), "=f"(r[11]), "=f"(r[12]), "=f"(r[13]), "=f"(r[14]), "=f"(r[15]), "=f"(r[16]),
-          "=f"(r[17]), "=f"(r[18]), "=f"(r[19]), "=f"(r[20]), "=f"(r[21]), "=f"(r[22]), "=f"(r[23]), "=f"(r[24]),
-          "=f"(r[25]), "=f"(r[26]), "=f"(r[27]), "=f"(r[28]), "=f"(r[29]), "=f"(r[30]), "=f"(r[31])
+        : "=f"(r[0]), "=f"(r[1]), "=f"(r[2]), "=f"(r[3]), "=f"(r[4]), "=f"(r[5]), "=f"(r[6]), "=f"(r[7]),
+          "=f"(r[8]), "=f"(r[9]), "=f"(r[10]), "=f"(r[11]), "=f"(r[12]), "=f"(r[13]), "=f"(r[14]), "=f"(r[15]),
+          "=f"(r[16]), "=f"(r[17]), "=f"(r[18]), "=f"(r[19]), "=f"(r[20]), "=f"(r[21]), "=f"(r[22]), "=f"(r[23]),
+          "=f"(r[24]), "=f"(r[25]), "=f"(r[26]), "=f"(r[27]), "=f"(r[28]), "=f"(r[29]), "=f"(r[30]), "=f"(r[31])
         : "r"(taddr));
 }
+// One lane of the (converged) warp.
+__device__ __forceinline__ bool elect() {
+    uint32_t one;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "elect.sync _|p, 0xffffffff;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(one));
+    return one != 0;
+}
+
 __device__ __forceinline__ void tmem_store8(uint32_t taddr, const uint32_t (&r)[8]) {
     asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"r"(taddr), "r"(r[0]),
                  "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
@@ -122,27 +133,42 @@ __device__ __forceinline__ void tmem_store8(uint32_t taddr, const uint32_t (&r)[
 }
 __device__ __forceinline__ void tmem_wait_store() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
-// Packed FP32 pairs: x * f + c, and a += b.
-__device__ __forceinline__ float2 fma_pair(float x0, float x1, float f, float c) {
-    float2 r;
-    asm("{\n\t.reg .b64 x, f, c;\n\t"
-        "mov.b64 x, {%2, %3};\n\t"
-        "mov.b64 f, {%4, %4};\n\t"
-        "mov.b64 c, {%5, %5};\n\t"
-        "fma.rn.f32x2 x, x, f, c;\n\t"
-        "mov.b64 {%0, %1}, x;\n\t}"
-        : "=f"(r.x), "=f"(r.y)
-        : "f"(x0), "f"(x1), "f"(f), "f"(c));
-    return r;
+// Packed pairs of FP32 (two 32-bit registers side by side).
+using Pair = unsigned long long;
+__device__ __forceinline__ Pair pair(float a, float b) {
+    Pair p;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(p) : "f"(a), "f"(b));
+    return p;
 }
-__device__ __forceinline__ void add_pair(float& a0, float& a1, float b0, float b1) {
-    asm("{\n\t.reg .b64 a, b;\n\t"
-        "mov.b64 a, {%0, %1};\n\t"
-        "mov.b64 b, {%2, %3};\n\t"
-        "add.rn.f32x2 a, a, b;\n\t"
-        "mov.b64 {%0, %1}, a;\n\t}"
-        : "+f"(a0), "+f"(a1)
-        : "f"(b0), "f"(b1));
+__device__ __forceinline__ float2 unpair(Pair p) {
+    float2 v;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(v.x), "=f"(v.y) : "l"(p));
+    return v;
+}
+__device__ __forceinline__ Pair fma_pair(Pair a, Pair b, Pair c) {
+    Pair p;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(p) : "l"(a), "l"(b), "l"(c));
+    return p;
+}
+__device__ __forceinline__ Pair add_pair(Pair a, Pair b) {
+    Pair p;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(p) : "l"(a), "l"(b));
+    return p;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float m;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(m) : "f"(a), "f"(b), "f"(c));
+    return m;
+}
+// split_pair of a packed pair
+__device__ __forceinline__ void split_packed(Pair p, Pair minus_one, uint32_t& hi, uint32_t& lo) {
+    const float2 v = unpair(p);
+    const __half2 h = __floats2half2_rn(v.x, v.y);
+    const float2 f = __half22float2(h);
+    const float2 rest = unpair(fma_pair(pair(f.x, f.y), minus_one, p));
+    const __half2 l = __floats2half2_rn(rest.x, rest.y);
+    hi = *reinterpret_cast<const uint32_t*>(&h);
+    lo = *reinterpret_cast<const uint32_t*>(&l);
 }
 
 // Two or four values of a row, or zeros.
@@ -419,12 +445,16 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_kernel(const AttentionPar
             }
             // O's row of this thread
             auto add_outputs = [&] {
+                constexpr int kColumns = S::kAdd && D == 128 ? 16 : 32;
 #pragma unroll
-                for (int i = 0; i < D; i += 16) {
-                    float x[16];
+                for (int i = 0; i < D; i += kColumns) {
+                    float x[kColumns];
                     tmem_load(o_at + i, x);
 #pragma unroll
-                    for (int j = 0; j < 16; j += 2) add_pair(o[i + j], o[i + j + 1], x[j], x[j + 1]);
+                    for (int j = 0; j < kColumns; j += 2) {
+                        const float2 v = unpair(add_pair(pair(o[i + j], o[i + j + 1]), pair(x[j], x[j + 1])));
+                        o[i + j] = v.x, o[i + j + 1] = v.y;
+                    }
                 }
             };
             for (int j = 0; j < tiles; ++j) {
@@ -439,9 +469,9 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_kernel(const AttentionPar
                 const int visible = live ? min(max(position + 1 - t0, 0), kN) : 0;
                 const bool cut = __any_sync(0xffffffffu, visible < kN);
                 // largest score, largest weight times scale
-                // f(x, g) for every group of 16 scores, kAtOnce of them per load
-                constexpr int kAtOnce = S::kAdd && D == 128 ? 1 : 2;
-                auto each_group = [&](auto f) {
+                // f(x, g) for every group of 16 scores, `at_once` of them per load
+                auto each_group = [&](auto at_once, auto f) {
+                    constexpr int kAtOnce = decltype(at_once)::value;
 #pragma unroll 1
                     for (int g = 0; g < kGroups; g += kAtOnce) {
                         float x[16 * kAtOnce];
@@ -450,28 +480,30 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_kernel(const AttentionPar
                         for (int i = 0; i < kAtOnce; ++i) f(*reinterpret_cast<float(*)[16]>(x + 16 * i), g + i);
                     }
                 };
+                using One = std::integral_constant<int, 1>;
                 // the tile's weights; kCut: some row of the warp does not see all of its tokens
                 auto weigh = [&](auto is_cut) {
                     constexpr bool kCut = decltype(is_cut)::value;
+                    using Some = std::integral_constant<int, kCut || (S::kAdd && D == 128) ? 1 : 2>;
                     auto largest_of = [&](float (&x)[16], int g) {  // scaled
                         if constexpr (kCut) {
 #pragma unroll
                             for (int i = 0; i < 16; ++i) x[i] = g * 16 + i < visible ? x[i] : -INFINITY;
                         }
-                        float big = x[0];
+                        float big = fmaxf(x[0], x[1]);
 #pragma unroll
-                        for (int i = 1; i < 16; ++i) big = fmaxf(big, x[i]);
+                        for (int i = 2; i < 16; i += 2) big = max3(big, x[i], x[i + 1]);
                         return kCut && g * 16 >= visible ? -INFINITY : big * (k_factor * scale[g].x);
                     };
                     float top = -INFINITY, most_scale = 0.f;
-                    each_group([&](float (&x)[16], int g) {
+                    each_group(Some{}, [&](float (&x)[16], int g) {
                         top = fmaxf(top, largest_of(x, g));
                         most_scale = fmaxf(most_scale, kCut && g * 16 >= visible ? 0.f : scale[g].y);
                     });
                     if (__any_sync(0xffffffffu, top > m + kSlack || most_scale >= 2.f * unit)) {
                         const float m_new = fmaxf(m, top);
                         float reach = 0.f;  // largest weight times scale
-                        each_group([&](float (&x)[16], int g) {
+                        each_group(One{}, [&](float (&x)[16], int g) {
                             const float t = largest_of(x, g);
                             if (t != -INFINITY) reach = fmaxf(reach, scale[g].y * ex2(t - m_new));
                         });
@@ -502,33 +534,37 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_kernel(const AttentionPar
                     // weight * V scale = 2^(score - m + log2 scale - log2 unit + 12). A scale below unit * 2^-40
                     // counts as that: its weights are zero in FP16 either way, but l needs them
                     const float base_m = m == -INFINITY ? 0.f : m, shift = 12.f - float(unit_log);
+                    [[maybe_unused]] const Pair minus_one = pair(-1.f, -1.f);
                     const float least = fmaxf(unit * 9.094947e-13f, 1.17549435e-38f);
-                    each_group([&](float (&x)[16], int g) {
+                    each_group(Some{}, [&](float (&x)[16], int g) {
                         const float4 sc = scale[g];
                         const bool small = sc.y < least;
                         const float f = k_factor * sc.x;
                         const float c = (small ? -28.f : sc.z + shift) - base_m;
                         const float back = small ? 268435456.f : sc.w * (unit * (1.f / kWeightTop));
-                        float sum0 = 0.f, sum1 = 0.f;
+                        const Pair ff = pair(f, f), cc = pair(c, c);
+                        Pair sum = pair(0.f, 0.f);
                         uint32_t hi[8];
                         [[maybe_unused]] uint32_t lo[8];
 #pragma unroll
                         for (int i = 0; i < 16; i += 2) {
-                            const float2 t = fma_pair(x[i], x[i + 1], f, c);
+                            const float2 t = unpair(fma_pair(pair(x[i], x[i + 1]), ff, cc));
                             float p0 = ex2(t.x), p1 = ex2(t.y);
                             if constexpr (kCut) {
                                 p0 = g * 16 + i < visible ? p0 : 0.f;
                                 p1 = g * 16 + i + 1 < visible ? p1 : 0.f;
                             }
-                            add_pair(sum0, sum1, p0, p1);
+                            const Pair pp = pair(p0, p1);
+                            sum = add_pair(sum, pp);
                             if constexpr (kHalves == 2) {
-                                split_pair(p0, p1, hi[i / 2], lo[i / 2]);
+                                split_packed(pp, minus_one, hi[i / 2], lo[i / 2]);
                             } else {
                                 const __half2 h = __floats2half2_rn(p0, p1);
                                 hi[i / 2] = *reinterpret_cast<const uint32_t*>(&h);
                             }
                         }
-                        l = fmaf(sum0 + sum1, kCut && g * 16 >= visible ? 0.f : back, l);
+                        const float2 sums = unpair(sum);
+                        l = fmaf(sums.x + sums.y, kCut && g * 16 >= visible ? 0.f : back, l);
                         // over the scores just read: 16 columns hold 8 of high halves, 8 of low
                         tmem_store8(s_at + g * 16, hi);
                         if constexpr (kHalves == 2) tmem_store8(s_at + g * 16 + 8, lo);
@@ -715,7 +751,8 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_kernel(const AttentionPar
     } else {
         // ================================================================ products
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(S::kProductRegs));
-        if (warp == 12 && lane == 0) {
+        if (warp == 12) {
+            // the warp runs in step and one elected lane issues: the descriptors stay in uniform registers
             constexpr uint32_t kIdescS = umma_idesc_f16<kM, kN>();
             constexpr uint32_t kIdescO = umma_idesc_f16<kM, D>() | (1u << 16);  // B is MN-major
             // descriptors' low bits are addresses / 16: adding moves them
@@ -726,24 +763,25 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_kernel(const AttentionPar
             Segment seg;
             bool ok = true;
             while (ok && cursor.next(seg)) {
-                const int most = seg.k1 - seg.k0;
-                const int n0 = tiles_for(seg, 0), n1 = tiles_for(seg, 1);
+                const int most = __shfl_sync(0xffffffffu, seg.k1 - seg.k0, 0);
+                const int n0 = __shfl_sync(0xffffffffu, tiles_for(seg, 0), 0), n1 = __shfl_sync(0xffffffffu, tiles_for(seg, 1), 0);
                 for (int j = 0; ok && j <= most; ++j) {
                     const int sj = (slot + j) % kStages, sp = (slot + j + kStages - 1) % kStages;  // this tile's, the last's
-                    if (j < most) ok = wait_one(k_full + sj, ((slot + j) / kStages) & 1);
-                    if (ok && j) ok = wait_one(v_full + sp, ((slot + j - 1) / kStages) & 1);
+                    if (j < most) ok = wait(k_full + sj, ((slot + j) / kStages) & 1);
+                    if (ok && j) ok = wait(v_full + sp, ((slot + j - 1) / kStages) & 1);
                     for (int w = 0; ok && w < 2; ++w) {
                         const int n = w ? n1 : n0;
                         if (j > n || n == 0) continue;
                         const uint32_t s_at = tmem + w * kN, o_at = tmem + 2 * kN + w * D;
                         if (j == 0) {
-                            if (!(ok = wait_one(q_full + w, (q_phase >> w) & 1))) break;
+                            if (!(ok = wait(q_full + w, (q_phase >> w) & 1))) break;
                             q_phase ^= 1u << w;
                         } else {
-                            if (!(ok = wait_one(p_full + w, (p_phase >> w) & 1))) break;
+                            if (!(ok = wait(p_full + w, (p_phase >> w) & 1))) break;
                             p_phase ^= 1u << w;
                         }
                         tmem_fence_after();
+                        if (elect()) {
                         if (j) {
                             const uint64_t vd = v_desc + uint64_t(sp * (S::kTileBytes >> 4));
 #pragma unroll
@@ -765,10 +803,15 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_kernel(const AttentionPar
                                             half != kHalves - 1 || i != 0);
                         }
                         mma_commit(s_full + w);
+                        }
+                        __syncwarp();
                     }
                     if (!ok) break;
-                    if (j < most) mma_commit(k_empty + sj);
-                    if (j) mma_commit(v_empty + sp);
+                    if (elect()) {
+                        if (j < most) mma_commit(k_empty + sj);
+                        if (j) mma_commit(v_empty + sp);
+                    }
+                    __syncwarp();
                 }
                 slot += most;
             }
