@@ -8,14 +8,17 @@
 // outputs), so a long context with few rows is shared like many short ones; the device plans
 // this itself from row_offsets and starts.
 //
-// Roles of a CTA (16 warps):
+// Roles of a CTA (three more warps idle):
 //  * warps 8-11 widen K and V codes to FP16 tiles in shared memory (exact; K token-major,
 //    V token-major too: the tensor core reads it transposed), with their blocks' scales;
-//  * one thread of warp 12 issues the products: S = Q K^T into tensor memory, O = P V
-//    with P from tensor memory;
+//  * one lane of warp 12 issues the products: S = Q K^T into tensor memory, O = P V with
+//    P from tensor memory;
 //  * warps 0-3 and 4-7 own one tile each, a thread per vector: running softmax of S's
-//    row, weights written over S in place, O's rows added up.
-// While one tile's threads work on their S, the tensor core runs the other's O and S.
+//    row, weights written over S in place, O's rows added up. (Two threads per vector,
+//    with half of the tokens and dims each, measured 13-15 % slower: they have to tell each
+//    other their largest scores, and a thread then has too few registers.)
+// S has kBuffers places (3 x 128 columns beside two O of 64, 2 beside two O of 128), used in
+// turn by both tiles: with three, a tile's next S is ready before its threads ask for it.
 //
 // Outputs: FP32 ones are added up in registers, tile by tile; BF16 ones stay in tensor
 // memory over an item's tiles.
@@ -37,7 +40,7 @@ namespace kv8 {
 namespace {
 
 constexpr int kCtas = 148;
-constexpr int kThreads = 512;
+constexpr int kWidenWarp = 8, kProductWarp = 12, kThreads = 512;
 constexpr int kM = 128;       // vectors of a tile
 constexpr int kN = 128;       // tokens of a K/V tile
 // Scale rows in flight. Row j + 4 is written after P V of tile j + 1 completed (its V slot
@@ -59,14 +62,16 @@ struct Shape {
     static constexpr int kV = kK + kStages * kTileBytes;
     static constexpr int kScales = kV + kStages * kTileBytes;           // [slots][groups] K, V, log2 V, 1 / V
     static constexpr int kBars = kScales + kScaleSlots * kGroups * 16;
-    static constexpr int kPlan = kBars + 32 * 8;                        // planning, and a few words
-    static constexpr int kSmem = kPlan + (kThreads + 1) * 4 + (kThreads + 1) * 8 + 2 * 16 * 8 + 64;
+    static constexpr int kPlan = kBars + 32 * 8;
+    static constexpr int kSmem = kPlan + (kThreads + 1) * 12 + 2 * 32 * 8;
     static constexpr int kAlloc = kSmem + 1024;                         // alignment slack
-    // registers a thread of each role: together the 512 x 128 of the launch
-    static constexpr int kSoftmaxRegs = D == 64 ? 168 : kHalves == 1 ? 168 : 184;
+    static constexpr int kBuffers = D == 64 ? 3 : 2;                    // places of S
+    // registers a thread of each role: together those of the launch, 512 x 128
+    static constexpr int kSoftmaxRegs = kHalves == 2 && D == 128 ? 184 : 168;
     static constexpr int kWidenRegs = D == 64 ? 96 : kHalves == 1 ? 104 : 80;
     static constexpr int kProductRegs = 512 - 2 * kSoftmaxRegs - kWidenRegs;
-    static constexpr uint32_t kTmemCols = 512;                          // S: 2 x 128, O: 2 x D
+    static constexpr int kAhead = kHalves == 2 && D == 128 ? 1 : 2;     // K and V codes loaded ahead, or one of them
+    static constexpr uint32_t kTmemCols = 512;                          // S: kBuffers x 128, O: 2 x D
 };
 static_assert(Shape<float, 128>::kAlloc <= 232448 && Shape<__nv_bfloat16, 128>::kAlloc <= 232448);
 
@@ -171,19 +176,28 @@ __device__ __forceinline__ void split_packed(Pair p, Pair minus_one, uint32_t& h
     lo = *reinterpret_cast<const uint32_t*>(&l);
 }
 
-// Two or four values of a row, or zeros.
-__device__ __forceinline__ void load_few(const float* p, bool on, float (&x)[2]) {
-    const float2 v = on ? *reinterpret_cast<const float2*>(p) : make_float2(0.f, 0.f);
-    x[0] = v.x, x[1] = v.y;
+// Registers a thread of this warpgroup from here on; the launch gives 128.
+template <int N>
+__device__ __forceinline__ void set_registers() {
+    if constexpr (N > 128) {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
+    } else {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
+    }
 }
-__device__ __forceinline__ void load_few(const __nv_bfloat16* p, bool on, float (&x)[2]) {
-    const uint32_t v = on ? *reinterpret_cast<const uint32_t*>(p) : 0u;
-    x[0] = __uint_as_float(v << 16), x[1] = __uint_as_float(v & 0xffff0000u);
+
+__device__ __forceinline__ void copy_row16(uint32_t to, const void* from, bool live) {  // zeros where not live
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(live ? 16 : 0) : "memory");
 }
-template <class T>
-__device__ __forceinline__ void load_few(const T* p, bool on, float (&x)[4]) {
-    x[0] = x[1] = x[2] = x[3] = 0.f;
-    if (on) load4(p, x);
+
+// The values of a 16-byte word.
+__device__ __forceinline__ void widen_word(uint4 w, float (&x)[4]) {
+    x[0] = __uint_as_float(w.x), x[1] = __uint_as_float(w.y), x[2] = __uint_as_float(w.z), x[3] = __uint_as_float(w.w);
+}
+__device__ __forceinline__ void widen_word(uint4 w, float (&x)[8]) {
+    const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x[2 * i] = __uint_as_float(u[i] << 16), x[2 * i + 1] = __uint_as_float(u[i] & 0xffff0000u);
 }
 
 // One item's tiles k0 .. k1 - 1 (of `tiles`), and what it covers.
@@ -252,23 +266,25 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_kernel(const AttentionPar
     float4* scales = reinterpret_cast<float4*>(sm + S::kScales);
     uint64_t* bars = reinterpret_cast<uint64_t*>(sm + S::kBars);
     uint64_t *k_full = bars, *k_empty = bars + 2, *v_full = bars + 4, *v_empty = bars + 6;
-    uint64_t *q_full = bars + 8, *s_full = bars + 10, *p_full = bars + 12;  // per tile
-    uint64_t *scales_full = bars + 14, *joined = bars + 18;                 // per scale slot; per tile
-    uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(bars + 20);
-    int* failed = reinterpret_cast<int*>(bars + 21);
-    int* last = reinterpret_cast<int*>(bars + 22);  // [2] whether this CTA joins the parts, per tile
+    uint64_t *q_full = bars + 8, *p_full = bars + 10, *o_full = bars + 12, *joined = bars + 14, *q_free = bars + 16;  // per tile
+    uint64_t *s_full = bars + 18, *scales_full = bars + 21;  // per place of S; per row of scales
+    uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(bars + 25);
+    int* failed = reinterpret_cast<int*>(bars + 26);
+    int* last = reinterpret_cast<int*>(bars + 27);  // [2] whether this CTA joins the parts, per tile
     int64_t* units_before = reinterpret_cast<int64_t*>(sm + S::kPlan);       // [kThreads + 1]
-    int64_t* sums = units_before + kThreads + 1;                             // [16], [16]
-    int* blocks_before = reinterpret_cast<int*>(sums + 32);                  // [kThreads + 1]
+    int64_t* sums = units_before + kThreads + 1;                         // [32], [32]
+    int* blocks_before = reinterpret_cast<int*>(sums + 64);                  // [kThreads + 1]
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
 
-    if (warp == 12) tmem_alloc(tmem_holder, S::kTmemCols);
+    if (warp == kProductWarp) tmem_alloc(tmem_holder, S::kTmemCols);
     if (tid == 0) {
         for (int i = 0; i < 2; ++i) {
             mbar_init(k_full + i, 4), mbar_init(v_full + i, 4);
             mbar_init(k_empty + i, 1), mbar_init(v_empty + i, 1);
-            mbar_init(q_full + i, kM), mbar_init(s_full + i, 1), mbar_init(p_full + i, kM), mbar_init(joined + i, kM);
+            mbar_init(q_full + i, 4), mbar_init(p_full + i, 4), mbar_init(o_full + i, 1);
+            mbar_init(joined + i, 4), mbar_init(q_free + i, 4);
         }
+        for (int i = 0; i < S::kBuffers; ++i) mbar_init(s_full + i, 1);
         for (int i = 0; i < kScaleSlots; ++i) mbar_init(scales_full + i, 1);
         *failed = 0;
         fence_barrier_init();
@@ -328,7 +344,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_kernel(const AttentionPar
                 mine += Cursor::units_of(start, rows, block, block_rows);
             }
         }
-        const int64_t before = scan(mine, sums + 16);
+        const int64_t before = scan(mine, sums + 32);
         units_before[tid] = before;
         if (tid == kThreads - 1) units_before[kThreads] = before + mine;
         __syncthreads();
@@ -374,27 +390,35 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_kernel(const AttentionPar
     // Bounded wait of one thread, or of a whole warp (whose lanes then agree). After a wait
     // that expired every role leaves its loops at its next wait.
     auto wait_one = [&](uint64_t* bar, uint32_t parity) {
-        if (*reinterpret_cast<volatile int*>(failed)) return false;
-        if (mbar_wait_bounded(bar, parity)) return true;
+        for (int i = 0; i < 64; ++i)  // before the clock is read, which takes longer than most waits
+            if (mbar_try_wait(bar, parity)) return true;
+        const uint64_t start = global_ns();
+        while (!*reinterpret_cast<volatile int*>(failed) && global_ns() - start < kWaitNanoseconds)
+            if (mbar_try_wait(bar, parity)) return true;
         *reinterpret_cast<volatile int*>(failed) = 1;
         raise_error(p.error, kErrTimeout);
         return false;
     };
     auto wait = [&](uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, wait_one(bar, parity)) != 0; };
 
-    if (warp < 8) {
-        // ================================================================ softmax, one thread per vector
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(S::kSoftmaxRegs));
+    if (warp < kWidenWarp) {
+        // ================================================================ softmax, a thread per vector
+        set_registers<S::kSoftmaxRegs>();
         const int w = warp >> 2, v = tid & (kM - 1);
         const uint32_t lanes = uint32_t((warp & 3) * 32) << 16;
-        const uint32_t s_at = tmem + w * kN + lanes, o_at = tmem + 2 * kN + w * D + lanes;
+        const uint32_t o_at = tmem + S::kBuffers * kN + w * D + lanes;
+        unsigned char* q_tile = sm + S::kQ + w * kHalves * S::kTileBytes;
         const float sign = p.scale < 0.f ? -1.f : 1.f;  // the sign goes to q: scores' factors stay positive
-        uint32_t phase = 0, join_phase = 0;
-        int slot = 0;
+        uint32_t o_phase = 0, join_phase = 0, free_phase = 1;
+        int slot = 0, used = 0;  // K/V tiles and S places that earlier segments took
         Segment seg;
         bool ok = true;
+        auto arrive = [&](uint64_t* bar) {  // of the warp
+            __syncwarp();
+            if (lane == 0) mbar_arrive(bar);
+        };
         while (ok && cursor.next(seg)) {
-            const int tiles = tiles_for(seg, w), most = seg.k1 - seg.k0;
+            const int n0 = tiles_for(seg, 0), n1 = tiles_for(seg, 1), tiles = w ? n1 : n0, most = seg.k1 - seg.k0;
             const int row = w * tile_rows + v / group;
             const bool live = v < tile_rows * group && row < seg.rows;
             const int position = seg.position + row;
@@ -402,73 +426,101 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_kernel(const AttentionPar
             int unit_log = -110;
 #pragma unroll
             for (int d = 0; d < D; ++d) o[d] = 0.f;
+            if (!(ok = wait(q_free + w, free_phase))) break;  // the tile's other warps have left its query buffer
+            free_phase ^= 1;
             if (tiles) {
-                // ---- query rows as FP16 halves, K-major with the 128-byte swizzle: the warp reads its 32
-                // vectors one by one, D / 32 values a lane, four in flight
-                constexpr int kPer = D / 32;
-                const int v0 = v & ~31;
-#pragma unroll 1
-                for (int r = 0; r < 32; r += 4) {
-                    float x[4][kPer];
+                // ---- query rows as FP16 halves, K-major with the 128-byte swizzle. A warp brings its rows, as they
+                // are, to where their halves go, then a lane takes its row to registers and writes the halves back
+                constexpr int kWords = D * int(sizeof(T)) / 16, kEach = 16 / int(sizeof(T)), kCols = D / 64;
+                const int r0 = v & ~31;
+                const uint64_t from = reinterpret_cast<uint64_t>(
+                    live ? static_cast<const T*>(p.q) + int64_t(seg.row0 + row) * p.q_stride + (seg.head * group + v % group) * D
+                         : nullptr);
+                auto place = [&](int r, int word) {  // of a row's raw 16-byte word
+                    const int piece = word / 8;      // 128 bytes: a column block of a half
+                    return piece / kCols * S::kTileBytes + piece % kCols * (kM * 128) + int(sw128_offset(r, word % 8));
+                };
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const int vec = v0 + r + i, of = w * tile_rows + vec / group;
-                        const bool on = vec < tile_rows * group && of < seg.rows;
-                        const T* q = static_cast<const T*>(p.q) + int64_t(seg.row0 + of) * p.q_stride +
-                                     (seg.head * group + vec % group) * D + lane * kPer;
-                        load_few(q, on, x[i]);
+                for (int i = 0; i < kWords; ++i) {
+                    const int x = i * 32 + lane, r = x / kWords, word = x % kWords;
+                    const uint64_t at = __shfl_sync(0xffffffffu, from, r);
+                    copy_row16(smem_u32(q_tile) + place(r0 + r, word),
+                               at ? reinterpret_cast<const char*>(at) + word * 16 : static_cast<const char*>(p.q), at != 0);
+                }
+                asm volatile("cp.async.commit_group;\n\tcp.async.wait_group 0;" ::: "memory");
+                __syncwarp();
+                uint4 raw[kWords];
+                float amax = 0.f;
+#pragma unroll
+                for (int i = 0; i < kWords; ++i) {
+                    raw[i] = *reinterpret_cast<const uint4*>(q_tile + place(v, i));
+                    float x[kEach];
+                    widen_word(raw[i], x);
+#pragma unroll
+                    for (int c = 0; c < kEach; ++c) amax = fmaxf(amax, fabsf(x[c]));
+                }
+                float factor, inverse;
+                row_factor(amax, factor, inverse);
+                k_factor = inverse * (p.scale * sign) * kLog2e;
+                factor *= sign;
+                __syncwarp();  // every lane has read its words
+#pragma unroll
+                for (int i = 0; i < D; i += 8) {
+                    uint32_t hi[4], lo[4];
+                    float x[8];
+                    if constexpr (kEach == 8) {
+                        widen_word(raw[i / 8], x);
+                    } else {
+                        widen_word(raw[i / 4], *reinterpret_cast<float(*)[4]>(x));
+                        widen_word(raw[i / 4 + 1], *reinterpret_cast<float(*)[4]>(x + 4));
                     }
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        float amax = fabsf(x[i][0]);
-#pragma unroll
-                        for (int c = 1; c < kPer; ++c) amax = fmaxf(amax, fabsf(x[i][c]));
-                        amax = warp_max(amax);
-                        float factor, inverse;
-                        row_factor(amax, factor, inverse);
-                        if (lane == r + i) k_factor = inverse * (p.scale * sign) * kLog2e;
-                        factor *= sign;
-                        const int d = lane * kPer;
-                        unsigned char* to = sm + S::kQ + w * kHalves * S::kTileBytes + (d / 64) * (kM * 128) +
-                                            sw128_offset(v0 + r + i, (d % 64) / 8) + (d % 8) * 2;
-#pragma unroll
-                        for (int c = 0; c < kPer; c += 2) {
-                            uint32_t hi, lo;
-                            split_pair(x[i][c] * factor, x[i][c + 1] * factor, hi, lo);
-                            *reinterpret_cast<uint32_t*>(to + 2 * c) = hi;
-                            if constexpr (kHalves == 2) *reinterpret_cast<uint32_t*>(to + S::kTileBytes + 2 * c) = lo;
-                        }
-                    }
+                    for (int c = 0; c < 4; ++c) split_pair(x[2 * c] * factor, x[2 * c + 1] * factor, hi[c], lo[c]);
+                    unsigned char* to = q_tile + i / 64 * (kM * 128) + sw128_offset(v, i % 64 / 8);
+                    *reinterpret_cast<uint4*>(to) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+                    if constexpr (kHalves == 2)
+                        *reinterpret_cast<uint4*>(to + S::kTileBytes) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
                 }
                 fence_proxy_async_shared();
-                mbar_arrive(q_full + w);
+                arrive(q_full + w);
             }
-            // O's row of this thread
-            auto add_outputs = [&] {
-                constexpr int kColumns = S::kAdd && D == 128 ? 16 : 32;
+            // O's row of this thread, times `by`
+            auto add_outputs = [&](float by) {
 #pragma unroll
-                for (int i = 0; i < D; i += kColumns) {
-                    float x[kColumns];
+                for (int i = 0; i < D; i += 32) {
+                    float x[32];
                     tmem_load(o_at + i, x);
+                    const Pair bb = pair(by, by);
 #pragma unroll
-                    for (int j = 0; j < kColumns; j += 2) {
-                        const float2 v = unpair(add_pair(pair(o[i + j], o[i + j + 1]), pair(x[j], x[j + 1])));
-                        o[i + j] = v.x, o[i + j + 1] = v.y;
+                    for (int j = 0; j < 32; j += 2) {
+                        const float2 s = unpair(fma_pair(pair(x[j], x[j + 1]), bb, pair(o[i + j], o[i + j + 1])));
+                        o[i + j] = s.x, o[i + j + 1] = s.y;
                     }
                 }
             };
             for (int j = 0; j < tiles; ++j) {
-                if (!(ok = wait(s_full + w, phase))) break;
-                phase ^= 1;
+                // S places in order: j = 0 of both tiles, j = 1, ..., each as far as it goes
+                const int place = used + (w ? min(j + 1, n0) + j : j + min(j, n1));
+                if (!(ok = wait(s_full + place % S::kBuffers, (place / S::kBuffers) & 1))) break;
                 tmem_fence_after();
-                if (S::kAdd && j) add_outputs();
+                const uint32_t s_at = tmem + place % S::kBuffers * kN + lanes;
+                bool behind = j > 0;  // O of the tile before is still to come
+                auto wait_outputs = [&] {
+                    if (behind) {
+                        ok = wait(o_full + w, o_phase);
+                        o_phase ^= 1;
+                        behind = false;
+                        tmem_fence_after();
+                    }
+                    return ok;
+                };
                 const int sl = (slot + j) % kScaleSlots;
                 if (!(ok = wait(scales_full + sl, ((slot + j) / kScaleSlots) & 1))) break;
                 const float4* scale = scales + sl * kGroups;
-                const int t0 = (seg.k0 + j) * kN;
-                const int visible = live ? min(max(position + 1 - t0, 0), kN) : 0;
+                // tokens of the tile that the row sees (padding vectors are zero queries: all, so that they
+                // bring no masks into their warp)
+                const int visible = live ? min(max(position + 1 - (seg.k0 + j) * kN, 0), kN) : kN;
                 const bool cut = __any_sync(0xffffffffu, visible < kN);
-                // largest score, largest weight times scale
                 // f(x, g) for every group of 16 scores, `at_once` of them per load
                 auto each_group = [&](auto at_once, auto f) {
                     constexpr int kAtOnce = decltype(at_once)::value;
@@ -481,6 +533,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_kernel(const AttentionPar
                     }
                 };
                 using One = std::integral_constant<int, 1>;
+                float moved = 1.f;  // factor of the outputs so far
                 // the tile's weights; kCut: some row of the warp does not see all of its tokens
                 auto weigh = [&](auto is_cut) {
                     constexpr bool kCut = decltype(is_cut)::value;
@@ -507,25 +560,25 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_kernel(const AttentionPar
                             const float t = largest_of(x, g);
                             if (t != -INFINITY) reach = fmaxf(reach, scale[g].y * ex2(t - m_new));
                         });
-                        float by = 1.f;
                         if (top > m + kSlack || reach >= 2.f * unit) {
                             const float decay = m_new == -INFINITY ? 1.f : ex2(m - m_new);
                             const float largest = fminf(fmaxf(fmaxf(unit * decay, reach), kUnitFloor), 8.507059e37f);
                             unit_log = (__float_as_int(largest) >> 23) - 127;
-                            by = decay * (unit * pow2(-unit_log));
+                            moved = decay * (unit * pow2(-unit_log));
                             l *= decay;
                             m = m_new, unit = pow2(unit_log);
                         }
                         if constexpr (S::kAdd) {
 #pragma unroll
-                            for (int d = 0; d < D; ++d) o[d] *= by;
+                            for (int d = 0; d < D; ++d) o[d] *= moved;
                         } else if (j) {
+                            if (!wait_outputs()) return;
 #pragma unroll 1
                             for (int i = 0; i < D; i += 16) {
                                 float x[16];
                                 tmem_load(o_at + i, x);
 #pragma unroll
-                                for (int c = 0; c < 16; ++c) x[c] *= by;
+                                for (int c = 0; c < 16; ++c) x[c] *= moved;
                                 tmem_store8(o_at + i, *reinterpret_cast<uint32_t(*)[8]>(x));
                                 tmem_store8(o_at + i + 8, *reinterpret_cast<uint32_t(*)[8]>(x + 8));
                             }
@@ -559,12 +612,12 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_kernel(const AttentionPar
                             if constexpr (kHalves == 2) {
                                 split_packed(pp, minus_one, hi[i / 2], lo[i / 2]);
                             } else {
-                                const __half2 h = __floats2half2_rn(p0, p1);
-                                hi[i / 2] = *reinterpret_cast<const uint32_t*>(&h);
+                                const __half2 packed = __floats2half2_rn(p0, p1);
+                                hi[i / 2] = *reinterpret_cast<const uint32_t*>(&packed);
                             }
                         }
-                        const float2 sums = unpair(sum);
-                        l = fmaf(sums.x + sums.y, kCut && g * 16 >= visible ? 0.f : back, l);
+                        const float2 both = unpair(sum);
+                        l = fmaf(both.x + both.y, kCut && g * 16 >= visible ? 0.f : back, l);
                         // over the scores just read: 16 columns hold 8 of high halves, 8 of low
                         tmem_store8(s_at + g * 16, hi);
                         if constexpr (kHalves == 2) tmem_store8(s_at + g * 16 + 8, lo);
@@ -575,24 +628,31 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_kernel(const AttentionPar
                 } else {
                     weigh(std::false_type{});
                 }
+                // the last tile's O, its weights relative to the reference before this tile
+                if (!ok || !wait_outputs()) break;
+                if (S::kAdd && j) add_outputs(moved);
                 tmem_wait_store();
                 tmem_fence_before();
-                mbar_arrive(p_full + w);
+                arrive(p_full + w);
             }
-            if (ok && tiles && (ok = wait(s_full + w, phase))) {
-                phase ^= 1;
+            if (ok && tiles && (ok = wait(o_full + w, o_phase))) {
+                o_phase ^= 1;
                 tmem_fence_after();
-                add_outputs();
+                add_outputs(1.f);
                 tmem_fence_before();
             }
+            used += n0 + n1;
             slot += most;
             if (!ok) break;
             const float u = unit * (1.f / kWeightTop);
             // rows out through this tile's query buffer (its products are done): the warp's 32 rows,
-            // 16-byte words XOR-ed by the row against bank conflicts, then row by row
+            // 16-byte words XOR-ed by the row against bank conflicts, then word by word
             auto write_rows = [&](float r) {
                 constexpr int kWords = D * int(sizeof(T)) / 16, kEach = 16 / int(sizeof(T));
-                unsigned char* stage = sm + S::kQ + w * kHalves * S::kTileBytes + (v & ~31) * (kWords * 16);
+                unsigned char* stage = q_tile + (warp & 3) * 32 * (kWords * 16);
+                const uint64_t to_row = reinterpret_cast<uint64_t>(
+                    live ? static_cast<T*>(p.out) + int64_t(seg.row0 + row) * p.out_stride + (seg.head * group + v % group) * D
+                         : nullptr);
 #pragma unroll
                 for (int i = 0; i < kWords; ++i) {
                     T* to = reinterpret_cast<T*>(stage + lane * (kWords * 16) + (i ^ (lane & 7)) * 16);
@@ -601,20 +661,18 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_kernel(const AttentionPar
                         store4(to + c, o[i * kEach + c] * r, o[i * kEach + c + 1] * r, o[i * kEach + c + 2] * r, o[i * kEach + c + 3] * r);
                 }
                 __syncwarp();
-#pragma unroll 4
-                for (int i = lane; i < 32 * kWords; i += 32) {
-                    const int from = i / kWords, word = i % kWords, vec = (v & ~31) + from, of = w * tile_rows + vec / group;
-                    if (vec < tile_rows * group && of < seg.rows) {
-                        T* out = static_cast<T*>(p.out) + int64_t(seg.row0 + of) * p.out_stride +
-                                 (seg.head * group + vec % group) * D;
-                        reinterpret_cast<uint4*>(out)[word] =
+#pragma unroll
+                for (int i = 0; i < kWords; ++i) {
+                    const int x = i * 32 + lane, from = x / kWords, word = x % kWords;
+                    const uint64_t at = __shfl_sync(0xffffffffu, to_row, from);
+                    if (at)
+                        reinterpret_cast<uint4*>(at)[word] =
                             *reinterpret_cast<const uint4*>(stage + from * (kWords * 16) + (word ^ (from & 7)) * 16);
-                    }
                 }
-                __syncwarp();
             };
             if (seg.k0 == 0 && seg.k1 == seg.tiles) {
                 if (tiles) write_rows(l == 0.f ? 0.f : u / l);
+                arrive(q_free + w);
                 continue;
             }
             // ---- a part of the item: to the workspace; the last CTA to arrive joins them. Slot 0 of
@@ -623,14 +681,18 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_kernel(const AttentionPar
             unsigned* counters = static_cast<unsigned*>(p.workspace);
             float* parts = reinterpret_cast<float*>(static_cast<unsigned char*>(p.workspace) + kCtas * 2 * 4 + 96);
             auto part = [&](int cta, int which) { return parts + ((int64_t(cta) * 2 + which) * 2 + w) * kPart; };
-            float* mine = part(blockIdx.x, seg.k0 == 0);
+            auto state = [&](int cta, int which) { return parts + (((int64_t(cta) * 2 + which) * 2 + w) * kPart + D * kM + v * 2); };
+            {
+                float* mine = part(blockIdx.x, seg.k0 == 0);
 #pragma unroll
-            for (int d = 0; d < D; d += 4)
-                *reinterpret_cast<float4*>(mine + d * kM + v * 4) = make_float4(o[d] * u, o[d + 1] * u, o[d + 2] * u, o[d + 3] * u);
-            *reinterpret_cast<float2*>(mine + D * kM + v * 2) = make_float2(m, l);
+                for (int d = 0; d < D; d += 4)
+                    *reinterpret_cast<float4*>(mine + d * kM + v * 4) =
+                        make_float4(o[d] * u, o[d + 1] * u, o[d + 2] * u, o[d + 3] * u);
+                *reinterpret_cast<float2*>(state(blockIdx.x, seg.k0 == 0)) = make_float2(m, l);
+            }
             __threadfence();
-            auto meet = [&] {  // the tile's 128 threads
-                mbar_arrive(joined + w);
+            auto meet = [&] {  // the tile's four warps
+                arrive(joined + w);
                 ok = wait(joined + w, join_phase);
                 join_phase ^= 1;
                 return ok;
@@ -650,7 +712,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_kernel(const AttentionPar
                 for (int d = 0; d < D; ++d) o[d] = 0.f;
                 for (int i = 0; i < n; ++i) {
                     const float* from = part(c0 + i, i == 0);
-                    const float2 ml = __ldcg(reinterpret_cast<const float2*>(from + D * kM + v * 2));
+                    const float2 ml = __ldcg(reinterpret_cast<const float2*>(state(c0 + i, i == 0)));
                     const float big = fmaxf(m, ml.x);
                     const float a = m == big ? 1.f : ex2(m - big), b = ml.x == big ? 1.f : ex2(ml.x - big);
                     l = l * a + ml.y * b;
@@ -665,10 +727,11 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_kernel(const AttentionPar
                 write_rows(l == 0.f ? 0.f : 1.f / l);
             }
             if (!meet()) break;  // `last` may be written again
+            arrive(q_free + w);
         }
-    } else if (warp < 12) {
+    } else if (warp < kProductWarp) {
         // ================================================================ codes -> FP16 tiles
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(S::kWidenRegs));
+        set_registers<S::kWidenRegs>();
         const int t = tid & 127, bt = p.cache.block_tokens;
         constexpr int kWords = kN * D / 16 / 128;  // 16-byte words of a thread per tile
         constexpr int kChunks = D / 16;            // words of a token
@@ -685,17 +748,17 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_kernel(const AttentionPar
             const int len = seg.position + seg.rows;
             // Lane g < 8 finds the block of tile k's 16 tokens from 16 g on: the offset of their K
             // rows (V's are one block of rows on) and their scales. Codes and scales are loaded a tile
-            // ahead, offsets two.
+            // ahead, offsets two (kAhead 1: K codes while V's are stored, and V's while K's are).
             int64_t offset = 0;
             float2 scale, next_scale;
-            uint4 code[2][kWords];
+            uint4 code[S::kAhead][kWords];
             auto find = [&](int k) {
                 const int tile = k * kGroups + lane;
                 next_scale = make_float2(0.f, 0.f);
                 if (lane < kGroups && k < seg.k1 && tile * kGroupTokens < len) {
                     const int block = block_id(p.cache, table, p.table_stride, tile / in_page, p.error);
                     offset = tile_offset(p.cache, block, seg.head, 0, D) + tile % in_page * (kGroupTokens * D);
-                    if (warp == 8)
+                    if (warp == kWidenWarp)
                         next_scale = *reinterpret_cast<const float2*>(p.cache.scales + block * p.cache.scale_stride + 2 * seg.head);
                 }
             };
@@ -705,19 +768,22 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_kernel(const AttentionPar
                 for (int i = 0; i < kWords; ++i) {
                     const int group_of = first_token / kGroupTokens + i * (kN / kWords) / kGroupTokens;
                     const int64_t at = __shfl_sync(0xffffffffu, offset, group_of);
-                    code[part][i] = make_uint4(0, 0, 0, 0);
+                    code[part % S::kAhead][i] = make_uint4(0, 0, 0, 0);
                     if (first_token + i * (kN / kWords) < left)
-                        code[part][i] = __ldg(reinterpret_cast<const uint4*>(p.cache.pages + at + part * bt * D + own));
+                        code[part % S::kAhead][i] = __ldg(reinterpret_cast<const uint4*>(p.cache.pages + at + part * bt * D + own));
                 }
             };
             find(seg.k0);
             load(seg.k0, 0);
-            load(seg.k0, 1);
-            scale = next_scale;
-            find(seg.k0 + 1);
+            if constexpr (S::kAhead == 2) {
+                load(seg.k0, 1);
+                scale = next_scale;
+                find(seg.k0 + 1);
+            }
             for (int k = seg.k0; ok && k < seg.k1; ++k, ++slot) {
                 const int stage = slot % kStages;
                 const uint32_t parity = ((slot / kStages) & 1) ^ 1;
+                if constexpr (S::kAhead == 1) scale = next_scale;
                 if (t < kGroups)
                     scales[slot % kScaleSlots * kGroups + t] =
                         make_float4(scale.x, scale.y, __log2f(scale.y), scale.y == 0.f ? 0.f : 1.f / scale.y);
@@ -729,7 +795,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_kernel(const AttentionPar
                     unsigned char* tile = sm + (part ? S::kV : S::kK) + stage * S::kTileBytes;
 #pragma unroll
                     for (int i = 0; i < kWords; ++i) {
-                        const uint4 c = code[part][i];
+                        const uint4 c = code[part % S::kAhead][i];
                         uint32_t h[8];
                         widen4<F>(c.x, h[0], h[1]);
                         widen4<F>(c.y, h[2], h[3]);
@@ -742,85 +808,107 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_kernel(const AttentionPar
                     fence_proxy_async_shared();
                     __syncwarp();
                     if (lane == 0) mbar_arrive((part ? v_full : k_full) + stage);
-                    load(k + 1, part);
+                    if constexpr (S::kAhead == 2) {
+                        load(k + 1, part);
+                    } else if (part == 0) {
+                        load(k, 1);
+                    } else {
+                        find(k + 1);
+                        load(k + 1, 0);
+                    }
                 }
-                scale = next_scale;
-                find(k + 2);
+                if constexpr (S::kAhead == 2) {
+                    scale = next_scale;
+                    find(k + 2);
+                }
             }
         }
     } else {
         // ================================================================ products
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(S::kProductRegs));
-        if (warp == 12) {
+        set_registers<S::kProductRegs>();
+        if (warp == kProductWarp) {
             // the warp runs in step and one elected lane issues: the descriptors stay in uniform registers
             constexpr uint32_t kIdescS = umma_idesc_f16<kM, kN>();
             constexpr uint32_t kIdescO = umma_idesc_f16<kM, D>() | (1u << 16);  // B is MN-major
             // descriptors' low bits are addresses / 16: adding moves them
             const uint64_t q_desc = smem_desc(sm + S::kQ), k_desc = smem_desc(sm + S::kK);
             const uint64_t v_desc = mn_desc(smem_u32(sm + S::kV), kN * 128);
-            int slot = 0;
+            int slot = 0, used = 0;  // as in the softmax
             uint32_t q_phase = 0, p_phase = 0;  // one bit per tile
             Segment seg;
             bool ok = true;
             while (ok && cursor.next(seg)) {
                 const int most = __shfl_sync(0xffffffffu, seg.k1 - seg.k0, 0);
                 const int n0 = __shfl_sync(0xffffffffu, tiles_for(seg, 0), 0), n1 = __shfl_sync(0xffffffffu, tiles_for(seg, 1), 0);
-                for (int j = 0; ok && j <= most; ++j) {
-                    const int sj = (slot + j) % kStages, sp = (slot + j + kStages - 1) % kStages;  // this tile's, the last's
-                    if (j < most) ok = wait(k_full + sj, ((slot + j) / kStages) & 1);
-                    if (ok && j) ok = wait(v_full + sp, ((slot + j - 1) / kStages) & 1);
-                    for (int w = 0; ok && w < 2; ++w) {
-                        const int n = w ? n1 : n0;
-                        if (j > n || n == 0) continue;
-                        const uint32_t s_at = tmem + w * kN, o_at = tmem + 2 * kN + w * D;
-                        if (j == 0) {
-                            if (!(ok = wait(q_full + w, (q_phase >> w) & 1))) break;
-                            q_phase ^= 1u << w;
-                        } else {
-                            if (!(ok = wait(p_full + w, (p_phase >> w) & 1))) break;
-                            p_phase ^= 1u << w;
-                        }
+                // (tile, K/V tile) pairs in order: `s` the next S, `o` the next O, kBuffers behind it
+                struct Next {
+                    int w, j;
+                    __device__ __forceinline__ void skip(int n0, int n1, int most) {
+                        while (j < most && j >= (w ? n1 : n0)) step();
+                    }
+                    __device__ __forceinline__ void step() { w ^= 1, j += w == 0; }
+                };
+                Next s{0, 0}, o{0, 0};
+                s.skip(n0, n1, most), o.skip(n0, n1, most);
+                for (int i = 0; ok && i < n0 + n1 + S::kBuffers; ++i) {
+                    if (i >= S::kBuffers) {
+                        const int stage = (slot + o.j) % kStages, place = (used + i - S::kBuffers) % S::kBuffers;
+                        ok = wait(p_full + o.w, (p_phase >> o.w) & 1) && wait(v_full + stage, ((slot + o.j) / kStages) & 1);
+                        if (!ok) break;
+                        p_phase ^= 1u << o.w;
                         tmem_fence_after();
+                        const uint32_t s_at = tmem + place * kN, o_at = tmem + S::kBuffers * kN + o.w * D;
+                        const uint64_t vd = v_desc + uint64_t(stage * (S::kTileBytes >> 4));
+                        const bool keep = !S::kAdd && o.j > 0, leave = o.w || o.j >= n1;  // leave: V's last use
                         if (elect()) {
-                        if (j) {
-                            const uint64_t vd = v_desc + uint64_t(sp * (S::kTileBytes >> 4));
 #pragma unroll
                             for (int half = kHalves - 1; half >= 0; --half)
 #pragma unroll
-                                for (int i = 0; i < kN / 16; ++i)
-                                    mma_f16_ts(o_at, s_at + i * 16 + half * 8, vd + uint64_t(i * (2048 >> 4)), kIdescO,
-                                               half != kHalves - 1 || i != 0 || (!S::kAdd && j > 1));
-                        }
-                        if (j < n) {
-                            const uint64_t kd = k_desc + uint64_t(sj * (S::kTileBytes >> 4));
-                            const uint64_t qd = q_desc + uint64_t(w * kHalves * (S::kTileBytes >> 4));
-#pragma unroll
-                            for (int half = kHalves - 1; half >= 0; --half)
-#pragma unroll
-                                for (int i = 0; i < D / 16; ++i)
-                                    mma_f16(s_at, qd + uint64_t(half * (S::kTileBytes >> 4) + (i / 4) * (kM * 128 >> 4) + i % 4 * 2),
-                                            kd + uint64_t((i / 4) * (kN * 128 >> 4) + i % 4 * 2), kIdescS,
-                                            half != kHalves - 1 || i != 0);
-                        }
-                        mma_commit(s_full + w);
+                                for (int c = 0; c < kN / 16; ++c)
+                                    mma_f16_ts(o_at, s_at + c * 16 + half * 8, vd + uint64_t(c * (2048 >> 4)), kIdescO,
+                                               half != kHalves - 1 || c != 0 || keep);
+                            mma_commit(o_full + o.w);
+                            if (leave) mma_commit(v_empty + stage);
                         }
                         __syncwarp();
+                        o.step(), o.skip(n0, n1, most);
                     }
-                    if (!ok) break;
-                    if (elect()) {
-                        if (j < most) mma_commit(k_empty + sj);
-                        if (j) mma_commit(v_empty + sp);
+                    if (i < n0 + n1) {
+                        const int stage = (slot + s.j) % kStages, place = (used + i) % S::kBuffers;
+                        if (s.j == 0) {
+                            ok = wait(q_full + s.w, (q_phase >> s.w) & 1);
+                            q_phase ^= 1u << s.w;
+                        }
+                        ok = ok && wait(k_full + stage, ((slot + s.j) / kStages) & 1);
+                        if (!ok) break;
+                        tmem_fence_after();
+                        const uint32_t s_at = tmem + place * kN;
+                        const uint64_t kd = k_desc + uint64_t(stage * (S::kTileBytes >> 4));
+                        const uint64_t qd = q_desc + uint64_t(s.w * kHalves * (S::kTileBytes >> 4));
+                        const bool leave = s.w || s.j >= n1;
+                        if (elect()) {
+#pragma unroll
+                            for (int half = kHalves - 1; half >= 0; --half)
+#pragma unroll
+                                for (int c = 0; c < D / 16; ++c)
+                                    mma_f16(s_at, qd + uint64_t(half * (S::kTileBytes >> 4) + (c / 4) * (kM * 128 >> 4) + c % 4 * 2),
+                                            kd + uint64_t((c / 4) * (kN * 128 >> 4) + c % 4 * 2), kIdescS,
+                                            half != kHalves - 1 || c != 0);
+                            mma_commit(s_full + place);
+                            if (leave) mma_commit(k_empty + stage);
+                        }
+                        __syncwarp();
+                        s.step(), s.skip(n0, n1, most);
                     }
-                    __syncwarp();
                 }
-                slot += most;
+                slot += most, used += n0 + n1;
             }
         }
         __syncwarp();
     }
     tmem_fence_before();
     __syncthreads();
-    if (warp == 12) {
+    if (warp == kProductWarp) {
         tmem_fence_after();
         tmem_dealloc(tmem, S::kTmemCols);
     }
