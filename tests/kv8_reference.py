@@ -119,8 +119,9 @@ def bound(out, weight, size, top, length, dim, bf16):
     2^-22 from its halves (FP16's half step 2^-11 instead for BF16 outputs). It counts twice: in the sum and in the
     normaliser, which also add `length` terms in FP32 (2^-23 each). BF16 outputs are rounded once more (2^-8).
 
-    The halves also have a smallest step: weights times block scales are held in units in which the largest is 2^12,
-    and FP16 rounds to multiples of 2^-24 at best, so each is off by up to 2^-25 / 2^12 = 2^-37 of the largest, times
-    a code. `length` of those add up, also where the largest itself meets a code of 0 (top = largest * top code)."""
+    The halves also have a smallest step: weights times block scales are held in units of which the largest counts 2^8
+    or more, and FP16 rounds to multiples of 2^-24 at best, so each is off by up to 2^-25 / 2^8 = 2^-33 of the largest,
+    times a code. `length` of those add up, also where the largest itself meets a code of 0 (top = largest * top
+    code)."""
     e = size * (2 ** -22 + dim * 2 ** -23 + 2 ** -21) + 2 ** -21 + (2 ** -11 if bf16 else 2 ** -22)
-    return weight * (2 * e + length * 2 ** -22) + top * length * 2 ** -37 + (out.abs() * 2 ** -8 if bf16 else 0) + 1e-37
+    return weight * (2 * e + length * 2 ** -22) + top * length * 2 ** -33 + (out.abs() * 2 ** -8 if bf16 else 0) + 1e-37

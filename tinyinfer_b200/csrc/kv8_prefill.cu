@@ -49,7 +49,12 @@ constexpr int kScaleSlots = 4;
 constexpr int kSetup = 2;     // an item's start and end cost about this many tiles
 constexpr int kGroupTokens = 16;  // tokens that share a block's scales at least
 constexpr int kGroups = kN / kGroupTokens;
-constexpr float kWeightTop = 4096.f, kSlack = 2.f, kUnitFloor = 7.70371977754894e-34f;  // as in kv8_warp.cuh
+// A weight times V scale of `unit` is 2^8 in FP16, and may grow to 2^15 before the reference
+// score and the unit move (kRoom): a move costs a third of a tile's softmax, and with room for
+// 2^2 some row of a warp asked for one in most tiles. FP16's smallest half step, 2^-25, is
+// 2^-33 of the largest.
+constexpr int kTopLog = 8;
+constexpr float kRoom = 7.f;
 
 template <class T, int D>
 struct Shape {
@@ -422,7 +427,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_kernel(const AttentionPar
             const int row = w * tile_rows + v / group;
             const bool live = v < tile_rows * group && row < seg.rows;
             const int position = seg.position + row;
-            float o[D], m = -INFINITY, l = 0.f, unit = kUnitFloor, k_factor = 0.f;
+            float o[D], m = -INFINITY, l = 0.f, k_factor = 0.f;
             int unit_log = -110;
 #pragma unroll
             for (int d = 0; d < D; ++d) o[d] = 0.f;
@@ -548,25 +553,23 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_kernel(const AttentionPar
                         for (int i = 2; i < 16; i += 2) big = max3(big, x[i], x[i + 1]);
                         return kCut && g * 16 >= visible ? -INFINITY : big * (k_factor * scale[g].x);
                     };
-                    float top = -INFINITY, most_scale = 0.f;
+                    float top = -INFINITY, reach = -INFINITY;  // largest score, and log2 of weight times V scale plus m
                     each_group(Some{}, [&](float (&x)[16], int g) {
-                        top = fmaxf(top, largest_of(x, g));
-                        most_scale = fmaxf(most_scale, kCut && g * 16 >= visible ? 0.f : scale[g].y);
+                        const float t = largest_of(x, g);
+                        top = fmaxf(top, t);
+                        reach = fmaxf(reach, t + scale[g].z);
                     });
-                    if (__any_sync(0xffffffffu, top > m + kSlack || most_scale >= 2.f * unit)) {
-                        const float m_new = fmaxf(m, top);
-                        float reach = 0.f;  // largest weight times scale
-                        each_group(One{}, [&](float (&x)[16], int g) {
-                            const float t = largest_of(x, g);
-                            if (t != -INFINITY) reach = fmaxf(reach, scale[g].y * ex2(t - m_new));
-                        });
-                        if (top > m + kSlack || reach >= 2.f * unit) {
-                            const float decay = m_new == -INFINITY ? 1.f : ex2(m - m_new);
-                            const float largest = fminf(fmaxf(fmaxf(unit * decay, reach), kUnitFloor), 8.507059e37f);
-                            unit_log = (__float_as_int(largest) >> 23) - 127;
-                            moved = decay * (unit * pow2(-unit_log));
+                    const bool high = reach - m > float(unit_log) + kRoom || top > m + 60.f;
+                    if (__any_sync(0xffffffffu, high)) {
+                        if (high) {
+                            const float m_new = fmaxf(m, top);
+                            const float decay = m == -INFINITY ? 0.f : ex2(m - m_new);
+                            // the largest so far, in whole powers of two; within the exponents of floats
+                            const float most = fmaxf(m == -INFINITY ? -110.f : float(unit_log) + (m - m_new), reach - m_new);
+                            const int next = int(floorf(fminf(fmaxf(most, -110.f), 120.f)));
+                            moved = m == -INFINITY ? 0.f : ex2(m - m_new + float(unit_log - next));
                             l *= decay;
-                            m = m_new, unit = pow2(unit_log);
+                            m = m_new, unit_log = next;
                         }
                         if constexpr (S::kAdd) {
 #pragma unroll
@@ -584,17 +587,18 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_kernel(const AttentionPar
                             }
                         }
                     }
-                    // weight * V scale = 2^(score - m + log2 scale - log2 unit + 12). A scale below unit * 2^-40
+                    // weight * V scale = 2^(score - m + log2 scale - log2 unit + 8). A scale below unit * 2^-40
                     // counts as that: its weights are zero in FP16 either way, but l needs them
-                    const float base_m = m == -INFINITY ? 0.f : m, shift = 12.f - float(unit_log);
+                    const float base_m = m == -INFINITY ? 0.f : m, shift = float(kTopLog - unit_log);
+                    const float unit = pow2(unit_log);
                     [[maybe_unused]] const Pair minus_one = pair(-1.f, -1.f);
                     const float least = fmaxf(unit * 9.094947e-13f, 1.17549435e-38f);
                     each_group(Some{}, [&](float (&x)[16], int g) {
                         const float4 sc = scale[g];
                         const bool small = sc.y < least;
                         const float f = k_factor * sc.x;
-                        const float c = (small ? -28.f : sc.z + shift) - base_m;
-                        const float back = small ? 268435456.f : sc.w * (unit * (1.f / kWeightTop));
+                        const float c = (small ? float(kTopLog - 40) : sc.z + shift) - base_m;
+                        const float back = small ? 4294967296.f : sc.w * (unit * (1.f / (1 << kTopLog)));
                         const Pair ff = pair(f, f), cc = pair(c, c);
                         Pair sum = pair(0.f, 0.f);
                         uint32_t hi[8];
@@ -644,7 +648,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_kernel(const AttentionPar
             used += n0 + n1;
             slot += most;
             if (!ok) break;
-            const float u = unit * (1.f / kWeightTop);
+            const float u = pow2(unit_log - kTopLog);
             // rows out through this tile's query buffer (its products are done): the warp's 32 rows,
             // 16-byte words XOR-ed by the row against bank conflicts, then word by word
             auto write_rows = [&](float r) {

@@ -20,10 +20,10 @@
 //
 // The state is a running softmax: m (the reference score), l (sum of weights), and outputs
 // in units of `unit`, a power of two at most the largest weight times scale so far, so that
-// the weights fill FP16's range. FP16 has room for weights 8 times 2^12 (`unit` is below the
-// largest by up to 2), so m and unit move only when a score passes m by 2 (in powers of
+// the weights fill FP16's range. FP16 has room for weights 2^7 times 2^8 (`unit` is below the
+// largest by up to 2), so m and unit move only when a score passes m by 6 (in powers of
 // two) or a scale reaches twice the unit: moving them every time that the maximum grew cost a
-// fifth of the instructions.
+// fifth of the instructions. FP16's smallest half step, 2^-25, is 2^-33 of the largest.
 #pragma once
 #include "kv8.cuh"
 
@@ -34,8 +34,8 @@ constexpr int kTile = 16;                  // tokens of a tile: the K of one pro
 constexpr int kTiles = 2;                  // tiles of a unit: their products overlap, and votes and shuffles halve
 constexpr int kUnit = kTile * kTiles;
 constexpr int kChain = 4;                  // units per chain of tensor-op sums (FP32 outputs)
-constexpr float kWeightTop = 4096.f;       // a weight of `unit` is 2^12 in FP16
-constexpr float kSlack = 2.f;              // a score may pass m by this (weights up to 2^2)
+constexpr float kWeightTop = 256.f;        // a weight of `unit` is 2^8 in FP16
+constexpr float kSlack = 6.f;              // a score may pass m by this (weights up to 2^6)
 constexpr float kUnitFloor = 7.70371977754894e-34f;  // 2^-110: below every scale the append makes
 
 template <class T, int F, int D>
