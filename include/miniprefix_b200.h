@@ -303,9 +303,10 @@ typedef struct {
  * Every row's k is rotated by its position, and k and v go to slot position %
  * block_tokens of block tables[i][position / block_tokens]. With q, the rotated q goes
  * to q_out (which may be q itself). Rotation of a pair (a, b): (a cos - b sin, b cos
- * + a sin) with row `position` of cos / sin ([max_positions][rotary_dim / 2]), in 64
- * bits, rounded once; dims at or past rotary_dim pass unrotated (rotary_dim 0: no
- * rotation, cos and sin unused).
+ * + a sin) with row `position` of cos / sin ([max_positions][rotary_dim / 2]); dims at or
+ * past rotary_dim pass unrotated (rotary_dim 0: no rotation, cos and sin unused). q is
+ * rotated in FP32 (a rounded product and a fused multiply-add); k codes come from the exact
+ * rotated value.
  *
  * The scale of a block written from its slot 0 on is the smallest power of two with
  * which the largest new magnitude fits the format (at least 2^-100); what the block

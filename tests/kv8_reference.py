@@ -56,14 +56,15 @@ def rotate(x, cos, sin, rotary, layout):
     return y
 
 
-def to_type(x, dtype):
-    """64 bits -> dtype in one rounding (by way of 32 bits rounded to odd for BF16)."""
-    f = x.float()
-    if dtype == torch.float32:
-        return f
-    f = torch.where(f.double().abs() > x.abs(), torch.nextafter(f, torch.zeros_like(f)), f)
-    odd = (f.view(torch.int32) | 1).view(torch.float32)
-    return torch.where(f.double() == x, f, odd).to(dtype)
+def rotation_bound(x, rotated, cos, sin, rotary, layout, bf16):
+    """How far an FP32 rotation a c - (b s) may be from the 64-bit one: half a step (2^-24) of the rounded product b s,
+    and half a step of the sum, which is as large as the result plus the first error; BF16 outputs are rounded once
+    more (half a step: 2^-8 of the value)."""
+    products = rotate(x.abs(), torch.zeros_like(cos), sin.abs(), rotary, layout).abs()  # |b s| in a's place, |a s| in b's
+    products[..., rotary:] = 0
+    exact = products * 2 ** -24 + rotated.abs() * 2 ** -24 * (1 + 2 ** -20)
+    exact[..., rotary:] = 0
+    return exact + products * 2 ** -46 + (rotated.abs() + exact) * 2 ** -8 * (1 if bf16 else 0) + 1e-44
 
 
 def append(pages, scales, fmt, k, v, tables, offsets, starts):

@@ -1,7 +1,7 @@
 """8-bit paged K/V cache operators against plain 64-bit forms (kv8_reference.py).
 
-Codes, scales and rotated queries have to be equal; attention outputs lie within
-kv8_reference.bound, which counts the roundings. Blocks that no table names and slots
+Codes and scales have to be equal; rotated queries and attention outputs lie within
+kv8_reference.rotation_bound and kv8_reference.bound, which count the roundings. Blocks that no table names and slots
 behind a sequence's last token hold NaN codes (E4M3) and NaN scales, buffers have
 strides above their rows and sentinels behind them.
 """
@@ -302,9 +302,11 @@ class Appender:
                                                  pages[differ][:4].tolist(), cache.store[differ][:4].tolist())
         assert torch.equal(scales.view(torch.int32), cache.scale_store.view(torch.int32))
         if with_q:
-            want = ref.to_type(ref.rotate(q, c, s, self.rotary, self.layout), store.dtype).reshape(rows, -1)
-            assert torch.equal(q_out[:rows, : self.heads * d], want)
-            before[:rows, : self.heads * d] = want
+            want = ref.rotate(q, c, s, self.rotary, self.layout)
+            got = q_out[:rows, : self.heads * d].double().reshape(rows, -1, d)
+            assert bool(((got - want).abs() <= ref.rotation_bound(q, want, c, s, self.rotary, self.layout,
+                                                                  self.dtype == "bf16")).all())
+            before[:rows, : self.heads * d] = q_out[:rows, : self.heads * d]
         assert torch.equal(before.view(torch.int16), q_out.view(torch.int16)), "wrote outside the rows"
         return q_out[:rows, : self.heads * d]
 

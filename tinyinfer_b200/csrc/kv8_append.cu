@@ -2,72 +2,88 @@
 //
 // Rotation of a pair (a, b) at position p with c = cos[p][i], s = sin[p][i]: (a c - b s,
 // b c + a s), the reference's rope_append step (miniprefix/src/backend/cuda/
-// llama_runner.cu:20-32). A code is the nearest multiple of the block's scale, so a
-// rotated value next to the border of two codes must not be rounded on the way: the
-// products of two floats are exact in 64 bits, and the sum is rounded there once.
+// llama_runner.cu:20-32). A rotated q is one product and one fused multiply-add.
 //
-// The unit of work is (block, kv head, K or V): its scale needs the largest magnitude of
-// all its new tokens, so one warp takes a whole tile, twice (magnitude, then codes; the
-// second read hits L1).
+// A k code is the nearest multiple of the block's scale to the exact rotated value, so a
+// value next to the border of two codes must not be rounded on the way. The FP32 value
+// a c - (b s) is off by at most e = 2^-23 (|b s| + |value|); where value - e and value + e
+// have the same code, that is the code. Where not (one value in some 10^4)
+// the lane computes its codes again in 64 bits, in which the products are exact; likewise
+// for the scale, and for tiles with values outside the range in which e holds. (Everything in
+// 64 bits measured 24 us for 8192 rows of 9 + 3 + 3 heads x 64 FP32, and 290 us for 20447 rows of
+// 32 + 8 + 8 heads x 128 BF16: its conversions bound it.)
+//
+// Bound by HBM. A CTA takes up to 16 packed rows: all its threads rotate their q, and its
+// warps write the tiles of the blocks that begin among its rows (a tile's first appended row
+// is in one CTA only). A tile is (block, kv head, K or V); its scale needs the largest
+// magnitude of all its new tokens, so one warp takes it whole, 8 or 16 tokens in registers at
+// a time, twice: magnitude, then codes. Fewer rows per CTA when there are few (one for a
+// decode step), so that all SMs take part.
 #include "kv8.cuh"
 
 namespace mpb {
 namespace kv8 {
 namespace {
 
-constexpr int kThreads = 128;
-
-// double -> float rounded to odd, so that a later rounding to fewer bits equals one
-// rounding of the double.
-__device__ __forceinline__ float to_odd(double x) {
-    const float f = __double2float_rz(x);
-    return double(f) == x || isnan(x) ? f : __int_as_float(__float_as_int(f) | 1);
-}
-
-__device__ __forceinline__ float rounded(double x, float) { return __double2float_rn(x); }
-__device__ __forceinline__ float rounded(double x, __nv_bfloat16) { return to_odd(x); }  // store4 rounds it
+constexpr int kThreads = 256;
+constexpr int kMaxRows = 16;  // rows of a CTA
+constexpr float kHuge = 8.5e37f;  // 2^126: FP32 products and sums below it are finite
 
 // A lane's eight values of one head row: two groups of four, at i0 and i1. Chunk c of
 // the rotated dims holds four whole pairs; later chunks pass through.
 struct Chunk {
     int i0, i1, pair;  // pair: index of the first of the four rotation pairs, -1: none
 };
-__device__ __forceinline__ Chunk chunk_of(int c, int rotary, int interleaved) {
+template <bool kInterleaved>
+__device__ __forceinline__ Chunk chunk_of(int c, int rotary) {
     if (8 * c >= rotary) return {8 * c, 8 * c + 4, -1};
-    return interleaved ? Chunk{8 * c, 8 * c + 4, 4 * c} : Chunk{4 * c, rotary / 2 + 4 * c, 4 * c};
+    return kInterleaved ? Chunk{8 * c, 8 * c + 4, 4 * c} : Chunk{4 * c, rotary / 2 + 4 * c, 4 * c};
 }
 
-// The chunk's eight values, rotated by row `position` of the tables, in 64 bits.
+// The chunk's eight values as they are in memory.
 template <class T>
-__device__ __forceinline__ void load_rotated(const T* row, Chunk ch, int interleaved, const float* cos,
-                                             const float* sin, int rotary, int position, double (&r)[8]) {
-    float x[4], y[4];
-    load4(row + ch.i0, x);
-    load4(row + ch.i1, y);
-    if (ch.pair < 0) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) r[i] = x[i], r[4 + i] = y[i];
-        return;
+struct Raw {
+    using Word = std::conditional_t<sizeof(T) == 4, float4, uint2>;  // four values
+    Word a, b;
+    __device__ __forceinline__ void load(const T* row, Chunk ch) {
+        a = *reinterpret_cast<const Word*>(row + ch.i0);
+        b = *reinterpret_cast<const Word*>(row + ch.i1);
     }
-    float c[4], s[4];
-    const size_t at = size_t(position) * (rotary / 2) + ch.pair;
-    load4(cos + at, c);
-    load4(sin + at, s);
-    if (interleaved) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const double a = i < 2 ? x[2 * i] : y[2 * i - 4], b = i < 2 ? x[2 * i + 1] : y[2 * i - 3];
-            r[2 * i] = a * double(c[i]) - b * double(s[i]);
-            r[2 * i + 1] = b * double(c[i]) + a * double(s[i]);
-        }
-    } else {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const double a = x[i], b = y[i];
-            r[i] = a * double(c[i]) - b * double(s[i]);
-            r[4 + i] = b * double(c[i]) + a * double(s[i]);
-        }
+    __device__ __forceinline__ void widen(float (&x)[8]) const {
+        widen4f(a, x);
+        widen4f(b, x + 4);
     }
+    static __device__ __forceinline__ void widen4f(float4 w, float* x) { x[0] = w.x, x[1] = w.y, x[2] = w.z, x[3] = w.w; }
+    static __device__ __forceinline__ void widen4f(uint2 w, float* x) {
+        x[0] = __uint_as_float(w.x << 16), x[1] = __uint_as_float(w.x & 0xffff0000u);
+        x[2] = __uint_as_float(w.y << 16), x[3] = __uint_as_float(w.y & 0xffff0000u);
+    }
+};
+
+// What a rotation reads: the tables' row of a position.
+struct Angles {
+    const float *cos, *sin;
+    int half;
+    __device__ __forceinline__ void load(int position, int pair, float (&c)[4], float (&s)[4]) const {
+        const size_t at = size_t(position) * half + pair;
+        load4(cos + at, c);
+        load4(sin + at, s);
+    }
+};
+
+// Rotates a chunk in FP32; returns the largest magnitude of its rounded products.
+template <bool kInterleaved>
+__device__ __forceinline__ float rotate(float (&x)[8], const float (&c)[4], const float (&s)[4]) {
+    float cross = 0.f;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        float &a = x[kInterleaved ? 2 * i : i], &b = x[kInterleaved ? 2 * i + 1 : 4 + i];
+        const float bs = __fmul_rn(b, s[i]), as = __fmul_rn(a, s[i]);
+        cross = fmaxf(cross, fmaxf(fabsf(bs), fabsf(as)));
+        a = __fmaf_rn(a, c[i], -bs);
+        b = __fmaf_rn(b, c[i], as);
+    }
+    return cross;
 }
 
 // Exponent of the smallest power of two that holds `amax` (finite): 127 = 0.9921875 *
@@ -80,28 +96,28 @@ __device__ __forceinline__ int scale_exponent(float amax) {
     return max(x, -100);
 }
 
-// Four values in units of the scale as codes.
+// Codes of two values in units of the scale, in the low two bytes. INT8: adding 1.5 * 2^23
+// rounds to an integer (ties to even) whose low byte is the code; |value| <= 127.5.
 template <int F>
-__device__ __forceinline__ uint32_t encode4(const double (&r)[8], int at, double inv) {
-    uint32_t w = 0;
+__device__ __forceinline__ uint32_t encode2(float a, float b) {
     if constexpr (F == MP_KV8_INT8) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const double y = r[at + i] * inv;
-            const int c = isnan(y) ? 0 : __double2int_rn(fmin(fmax(y, -127.0), 127.0));
-            w |= uint32_t(c & 255) << (8 * i);
-        }
+        return __byte_perm(__float_as_uint(__fadd_rn(a, 12582912.f)), __float_as_uint(__fadd_rn(b, 12582912.f)), 0x0040) &
+               0xffffu;
     } else {
-#pragma unroll
-        for (int i = 0; i < 4; i += 2) {
-            float a = to_odd(r[at + i] * inv), b = to_odd(r[at + i + 1] * inv);
-            a = isnan(a) ? 0.f : a, b = isnan(b) ? 0.f : b;
-            uint16_t h;
-            asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(h) : "f"(b), "f"(a));
-            w |= uint32_t(h) << (8 * i);
-        }
+        uint16_t h;
+        asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(h) : "f"(b), "f"(a));
+        return h;
     }
-    return w;
+}
+template <int F>
+__device__ __forceinline__ uint32_t encode4(float a, float b, float c, float d) {
+    if constexpr (F == MP_KV8_INT8) {
+        const uint32_t x = __byte_perm(__float_as_uint(__fadd_rn(a, 12582912.f)), __float_as_uint(__fadd_rn(b, 12582912.f)), 0x0040);
+        const uint32_t y = __byte_perm(__float_as_uint(__fadd_rn(c, 12582912.f)), __float_as_uint(__fadd_rn(d, 12582912.f)), 0x0040);
+        return __byte_perm(x, y, 0x5410);
+    } else {
+        return encode2<F>(a, b) | encode2<F>(c, d) << 16;
+    }
 }
 
 // Four held codes times `ratio` (a power of two below 1), rounded to codes again.
@@ -110,34 +126,128 @@ __device__ __forceinline__ uint32_t recode4(uint32_t w, float ratio) {
     uint32_t lo, hi;
     widen4<F>(w, lo, hi);
     const float2 a = __half22float2(*reinterpret_cast<__half2*>(&lo)), b = __half22float2(*reinterpret_cast<__half2*>(&hi));
-    const double r[8] = {a.x, a.y, b.x, b.y, 0, 0, 0, 0};
-    return encode4<F>(r, 0, double(ratio));
+    return encode4<F>(a.x * ratio, a.y * ratio, b.x * ratio, b.y * ratio);
 }
 
-template <class T, int F, int D>
+// ---------------------------------------------------------------- in 64 bits
+// One value of a row: dim `d`, rotated.
+template <class T, bool kInterleaved>
+__device__ double exact_value(const T* row, int d, const Angles& angles, int rotary, int position) {
+    const double x = double(float(row[d]));
+    if (d >= rotary) return x;
+    const int half = rotary / 2;
+    const int i = kInterleaved ? d / 2 : d % half;
+    const bool second = kInterleaved ? d & 1 : d >= half;
+    const int other = kInterleaved ? d ^ 1 : second ? d - half : d + half;
+    const double y = double(float(row[other]));
+    const double c = double(angles.cos[size_t(position) * half + i]), s = double(angles.sin[size_t(position) * half + i]);
+    return second ? x * c + y * s : x * c - y * s;
+}
+
+// Its code; NaN is 0, infinity the largest. (A 64-bit value rounds to odd in 32 bits first, so
+// that rounding those to a code is one rounding.)
+template <int F>
+__device__ uint32_t exact_code(double v, float inv) {
+    if (isnan(v)) return 0;
+    const double y = v * double(inv);
+    if constexpr (F == MP_KV8_INT8) {
+        return uint32_t(__double2int_rn(fmin(fmax(y, -127.0), 127.0)) & 255);
+    } else {
+        float f = __double2float_rz(y);
+        if (double(f) != y) f = __int_as_float(__float_as_int(f) | 1);
+        return encode2<F>(f, 0.f) & 255u;
+    }
+}
+
+// A chunk's codes: those at i0 and at i1.
+template <class T, int F, bool kInterleaved>
+__device__ __noinline__ uint2 exact_codes(const T* row, int i0, int i1, Angles angles, int rotary, int position, float inv) {
+    uint32_t w[2] = {0, 0};
+#pragma unroll 1
+    for (int i = 0; i < 8; ++i) {
+        const int d = i < 4 ? i0 + i : i1 + i - 4;
+        const uint32_t c = exact_code<F>(exact_value<T, kInterleaved>(row, d, angles, rotary, position), inv) << (8 * (i & 3));
+        if (i < 4) {
+            w[0] |= c;
+        } else {
+            w[1] |= c;
+        }
+    }
+    return make_uint2(w[0], w[1]);
+}
+
+// A warp's tile: the largest finite magnitude, rounded to 32 bits; *odd: some value is not finite.
+template <class T, bool kInterleaved>
+__device__ __noinline__ float exact_largest(const T* at, int64_t stride, int n, int dims, Angles angles, int rotary,
+                                            int position, int lane, bool* odd) {
+    float amax = 0.f;
+    bool bad = false;
+#pragma unroll 1
+    for (int i = lane; i < n * dims; i += 32) {
+        const int t = i / dims;
+        const float f = fabsf(__double2float_rn(exact_value<T, kInterleaved>(at + t * stride, i % dims, angles, rotary, position + t)));
+        const bool finite = f <= 3.402823466e38f;
+        bad |= !finite;
+        amax = finite ? fmaxf(amax, f) : amax;
+    }
+    *odd = __any_sync(0xffffffffu, bad);
+    return warp_max(amax);
+}
+
+// ---------------------------------------------------------------- a tile, by one warp
+template <class T, int F, int D, bool kInterleaved>
 __device__ __forceinline__ void append_tile(const AppendParams& p, const T* rows, int64_t stride, int head, int part,
                                             int block, int slot0, int n, int position, int lane) {
     constexpr int kLanes = D / 8;        // lanes of one token
     constexpr int kStep = 32 / kLanes;   // tokens a warp reads at once
-    const int c = lane % kLanes, sub = lane / kLanes;
-    const int rotary = part ? 0 : p.rotary_dim;
-    const Chunk ch = chunk_of(c, rotary, p.interleaved);
+    constexpr int kUnitTokens = sizeof(T) == 4 && D == 128 ? 8 : 16;  // in registers at a time
+    constexpr int kSteps = kUnitTokens / kStep;                       // a lane's share
+    const int sub = lane / kLanes, rotary = part ? 0 : p.rotary_dim;
+    const Angles angles{p.cos, p.sin, rotary / 2};
+    const Chunk ch = chunk_of<kInterleaved>(lane % kLanes, rotary);
     const T* at = rows + head * D;
-    float amax = 0.f;
-    bool odd = false;
-    for (int t = sub; t < n; t += kStep) {
-        double r[8];
-        load_rotated(at + t * stride, ch, p.interleaved, p.cos, p.sin, rotary, position + t, r);
+    Raw<T> raw[kSteps];
+    auto load = [&](int first) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const float f = fabsf(__double2float_rn(r[i]));
-            const bool finite = f <= 3.402823466e38f;
-            odd |= !finite;
-            amax = finite ? fmaxf(amax, f) : amax;
+        for (int i = 0; i < kSteps; ++i)
+            if (first + i * kStep + sub < n) raw[i].load(at + (first + i * kStep + sub) * stride, ch);
+    };
+    // a token's values; what any of them may be off by (0: they are exact), and their largest magnitude
+    auto values = [&](const Raw<T>& r, int t, float (&x)[8], float& e, float& top) {
+        r.widen(x);
+        e = 0.f;
+        if (ch.pair >= 0) {
+            float c[4], s[4];
+            angles.load(position + t, ch.pair, c, s);
+            e = rotate<kInterleaved>(x, c, s);
+        }
+        top = 0.f;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) top = fmaxf(top, fabsf(x[j]));
+        if (ch.pair >= 0) e = (e + top) * 1.1920929e-7f;
+    };
+    // bounds of the largest magnitude; `sum` becomes NaN if a value is not finite
+    float most = 0.f, least = 0.f, sum = 0.f;
+    for (int first = 0; first < n; first += kUnitTokens) {
+        load(first);
+#pragma unroll
+        for (int i = 0; i < kSteps; ++i) {
+            const int t = first + i * kStep + sub;
+            if (t >= n) break;
+            float x[8], e, top;
+            values(raw[i], t, x, e, top);
+            most = fmaxf(most, top + e);
+            least = fmaxf(least, top - e);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) sum = fmaf(x[j], 0.f, sum);
         }
     }
-    amax = warp_max(amax);
-    int x = scale_exponent<F>(amax);
+    const bool wide = __any_sync(0xffffffffu, !(most < kHuge) || isnan(sum));  // e does not hold, or not finite
+    most = warp_max(most), least = warp_max(least);
+    bool odd = false;
+    int x = scale_exponent<F>(least);
+    if (wide || x != scale_exponent<F>(most))
+        x = scale_exponent<F>(exact_largest<T, kInterleaved>(at, stride, n, D, angles, rotary, position, lane, &odd));
     float* scale = p.cache.scales + int64_t(block) * p.cache.scale_stride + head * 2 + part;
     unsigned char* tile = p.cache.pages + tile_offset(p.cache, block, head, part, D);
     if (slot0 > 0) {
@@ -159,69 +269,137 @@ __device__ __forceinline__ void append_tile(const AppendParams& p, const T* rows
         __syncwarp();
     }
     if (lane == 0) *scale = pow2(x);
-    const double inv = double(pow2(-x));
-    for (int t = sub; t < n; t += kStep) {
-        double r[8];
-        load_rotated(at + t * stride, ch, p.interleaved, p.cos, p.sin, rotary, position + t, r);
-        unsigned char* to = tile + (slot0 + t) * D;
-        *reinterpret_cast<uint32_t*>(to + ch.i0) = encode4<F>(r, 0, inv);
-        *reinterpret_cast<uint32_t*>(to + ch.i1) = encode4<F>(r, 4, inv);
+    const float inv = pow2(-x);
+    for (int first = 0; first < n; first += kUnitTokens) {
+        if (n > kUnitTokens) load(first);  // else still there
+#pragma unroll
+        for (int i = 0; i < kSteps; ++i) {
+            const int t = first + i * kStep + sub;
+            if (t >= n) break;
+            float x[8], e, top;
+            values(raw[i], t, x, e, top);
+            uint32_t w[2];
+            bool near = wide;  // a border of codes lies within what a value may be off by
+            if (ch.pair < 0) {
+#pragma unroll
+                for (int j = 0; j < 2; ++j)
+                    w[j] = encode4<F>(x[4 * j] * inv, x[4 * j + 1] * inv, x[4 * j + 2] * inv, x[4 * j + 3] * inv);
+            } else {
+                const float d = fmaf(e, inv, 9.094947e-13f);  // 2^-40: products that lost bits below FP32's exponents
+#pragma unroll
+                for (int j = 0; j < 2; ++j) {
+                    const float* v = x + 4 * j;
+                    w[j] = encode4<F>(fmaf(v[0], inv, -d), fmaf(v[1], inv, -d), fmaf(v[2], inv, -d), fmaf(v[3], inv, -d));
+                    near |= w[j] != encode4<F>(fmaf(v[0], inv, d), fmaf(v[1], inv, d), fmaf(v[2], inv, d), fmaf(v[3], inv, d));
+                }
+            }
+            if (near) {
+                const uint2 exact = exact_codes<T, F, kInterleaved>(at + t * stride, ch.i0, ch.i1, angles, rotary, position + t, inv);
+                w[0] = exact.x, w[1] = exact.y;
+            }
+            unsigned char* to = tile + (slot0 + t) * D;
+            *reinterpret_cast<uint32_t*>(to + ch.i0) = w[0];
+            *reinterpret_cast<uint32_t*>(to + ch.i1) = w[1];
+        }
     }
-    if (__any_sync(0xffffffffu, odd) && lane == 0) raise_error(p.error, kErrValue);
+    if (odd && lane == 0) raise_error(p.error, kErrValue);
 }
 
-// One CTA per packed row: it rotates the row's q, and the first row of each touched block
-// writes the block's tiles.
-template <class T, int F, int D>
-__global__ void __launch_bounds__(kThreads) append_kernel(const AppendParams p) {
-    pdl_enter();
-    __shared__ int s_seq;
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    const int row = blockIdx.x;
-    if (tid == 0) s_seq = 0;
-    __syncthreads();
-    // the row's sequence: the number of sequences that end at or before it
-    int before = 0;
-    for (int i = tid; i < p.count; i += kThreads) before += p.row_offsets[i + 1] <= row;
-    before = __reduce_add_sync(0xffffffffu, before);
-    if (lane == 0) atomicAdd(&s_seq, before);
-    __syncthreads();
-    const int seq = s_seq;
-    if (seq >= p.count) return;  // behind the last sequence
-    const int begin = p.row_offsets[seq], end = min(p.row_offsets[seq + 1], p.rows), start = p.starts[seq];
+// A packed row's place: its sequence (-1: behind the last, or out of range) and position.
+struct Place {
+    int seq, position, end;  // end: the sequence's last row + 1
+};
+
+// By one warp: the row's sequence is the first that ends behind it, found 32 ways at a time.
+__device__ __forceinline__ Place find_row(const AppendParams& p, int row, int lane) {
+    int low = 0, high = p.count;
+    while (high - low > 32) {
+        const int step = (high - low + 31) / 32, i = low + (lane + 1) * step - 1;
+        const int k = __popc(__ballot_sync(0xffffffffu, i < high && p.row_offsets[i + 1] <= row));
+        low += k * step;
+        high = min(high, low + step);
+    }
+    low += __popc(__ballot_sync(0xffffffffu, low + lane < high && p.row_offsets[low + lane + 1] <= row));
+    if (low >= p.count) return {-1, 0, 0};
+    const int begin = p.row_offsets[low], end = min(p.row_offsets[low + 1], p.rows), start = p.starts[low];
     const int64_t position = int64_t(start) + row - begin;
     if (row < begin || row >= end || start < 0 || position >= int64_t(p.table_stride) * p.cache.block_tokens ||
         (p.rotary_dim && position >= p.max_positions)) {
-        if (tid == 0) raise_error(p.error, kErrBounds);
-        return;
+        if (lane == 0) raise_error(p.error, kErrBounds);
+        return {-1, 0, 0};
     }
-    const int pos = int(position), bt = p.cache.block_tokens, slot = pos % bt;
-    if (p.q) {
-        const T* q = static_cast<const T*>(p.q) + row * p.q_stride;
-        T* out = static_cast<T*>(p.q_out) + row * p.q_out_stride;
-        for (int i = tid; i < p.heads * (D / 8); i += kThreads) {
-            const int head = i / (D / 8), c = i % (D / 8);
-            const Chunk ch = chunk_of(c, p.rotary_dim, p.interleaved);
-            double r[8];
-            load_rotated(q + head * D, ch, p.interleaved, p.cos, p.sin, p.rotary_dim, pos, r);
-            store4(out + head * D + ch.i0, rounded(r[0], T{}), rounded(r[1], T{}), rounded(r[2], T{}), rounded(r[3], T{}));
-            store4(out + head * D + ch.i1, rounded(r[4], T{}), rounded(r[5], T{}), rounded(r[6], T{}), rounded(r[7], T{}));
+    return {low, int(position), end};
+}
+
+template <class T, int F, int D, bool kInterleaved>
+__global__ void __launch_bounds__(kThreads, 3) append_kernel(const AppendParams p, int rows_each, uint32_t per_row_inverse) {
+    constexpr int kChunks = D / 8;
+    __shared__ Place places[kMaxRows];
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    pdl_enter();
+    const int row0 = blockIdx.x * rows_each, rows = min(rows_each, p.rows - row0);
+    for (int i = warp; i < rows; i += kThreads / 32) {
+        const Place at = find_row(p, row0 + i, lane);
+        if (lane == 0) places[i] = at;
+    }
+    __syncthreads();
+    // ---- tiles of the blocks whose first appended row is here
+    const int bt = p.cache.block_tokens, tiles = 2 * p.cache.kv_heads;
+    int turn = warp;  // tiles go round the warps
+    for (int i = 0; i < rows; ++i) {
+        const Place at = places[i];
+        const int slot = at.position % bt;
+        if (at.seq < 0) continue;
+        if (slot && row0 + i != p.row_offsets[at.seq]) continue;
+        const int row = row0 + i;
+        const int block = p.tables[int64_t(at.seq) * p.table_stride + at.position / bt];
+        int n = min(bt - slot, at.end - row);
+        if (p.rotary_dim) n = min(n, p.max_positions - at.position);  // rows past the tables report themselves
+        if (unsigned(block) >= unsigned(p.cache.max_blocks)) {
+            if (tid == 0) raise_error(p.error, kErrBounds);
+            continue;
         }
+        for (; turn < tiles; turn += kThreads / 32) {
+            const int head = turn >> 1, part = turn & 1;
+            const T* x = static_cast<const T*>(part ? p.v : p.k);
+            const int64_t stride = part ? p.v_stride : p.k_stride;
+            append_tile<T, F, D, kInterleaved>(p, x + row * stride, stride, head, part, block, slot, n, at.position, lane);
+        }
+        turn -= tiles;
     }
-    if (row != begin && slot != 0) return;
-    const int block = p.tables[int64_t(seq) * p.table_stride + pos / bt];
-    int n = min(bt - slot, end - row);
-    if (p.rotary_dim) n = min(n, p.max_positions - pos);  // rows past the tables report themselves
-    if (unsigned(block) >= unsigned(p.cache.max_blocks)) {
-        if (tid == 0) raise_error(p.error, kErrBounds);
-        return;
-    }
-    for (int i = warp; i < 2 * p.cache.kv_heads; i += kThreads / 32) {
-        const int head = i >> 1, part = i & 1;
-        if (part == 0) {
-            append_tile<T, F, D>(p, static_cast<const T*>(p.k) + row * p.k_stride, p.k_stride, head, 0, block, slot, n, pos, lane);
-        } else {
-            append_tile<T, F, D>(p, static_cast<const T*>(p.v) + row * p.v_stride, p.v_stride, head, 1, block, slot, n, pos, lane);
+    // ---- q: a chunk of a head of a row per thread, kFly of them in flight
+    if (!p.q) return;
+    constexpr int kFly = 4;
+    const int per_row = p.heads * kChunks, total = rows * per_row;
+    const Chunk ch = chunk_of<kInterleaved>(tid % kChunks, p.rotary_dim);  // kThreads is a multiple of kChunks
+    const Angles angles{p.cos, p.sin, p.rotary_dim / 2};
+    for (int first = tid; first < total; first += kFly * kThreads) {
+        Raw<T> raw[kFly];
+        int row[kFly], head[kFly];
+#pragma unroll
+        for (int i = 0; i < kFly; ++i) {
+            const int x = first + i * kThreads;
+            row[i] = x < total ? int(__umulhi(x, per_row_inverse)) : 0;
+            head[i] = (x - row[i] * per_row) / kChunks;
+            if (x >= total || places[row[i]].seq < 0) {
+                row[i] = -1;
+            } else {
+                raw[i].load(static_cast<const T*>(p.q) + (row0 + row[i]) * p.q_stride + head[i] * D, ch);
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < kFly; ++i) {
+            if (row[i] < 0) continue;
+            float x[8];
+            raw[i].widen(x);
+            if (ch.pair >= 0) {
+                float c[4], s[4];
+                angles.load(places[row[i]].position, ch.pair, c, s);
+                rotate<kInterleaved>(x, c, s);
+            }
+            T* to = static_cast<T*>(p.q_out) + (row0 + row[i]) * p.q_out_stride + head[i] * D;
+            store4(to + ch.i0, x[0], x[1], x[2], x[3]);
+            store4(to + ch.i1, x[4], x[5], x[6], x[7]);
         }
     }
 }
@@ -230,8 +408,13 @@ __global__ void __launch_bounds__(kThreads) append_kernel(const AppendParams p) 
 
 cudaError_t launch_append(const AppendParams& p, int type, int format, int head_dim, cudaStream_t stream) {
     return dispatch(type, format, head_dim, [&](auto t, auto f, auto d) {
-        return launch_pdl(append_kernel<decltype(t), decltype(f)::value, decltype(d)::value>, dim3(p.rows),
-                          dim3(kThreads), 0, stream, p);
+        const int each = std::clamp(p.rows / (2 * 148), 1, kMaxRows);
+        using T = decltype(t);
+        constexpr int kFormat = decltype(f)::value, kDim = decltype(d)::value;
+        // x / per_row = high half of x * inverse while x * per_row < 2^32: x < 16 * per_row, per_row <= 2^14
+        const uint32_t per_row = p.heads * (kDim / 8), inverse = uint32_t(((uint64_t(1) << 32) + per_row - 1) / per_row);
+        return launch_pdl(p.interleaved ? append_kernel<T, kFormat, kDim, true> : append_kernel<T, kFormat, kDim, false>,
+                          dim3((p.rows + each - 1) / each), dim3(kThreads), 0, stream, p, each, inverse);
     });
 }
 
