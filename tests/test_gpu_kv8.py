@@ -239,6 +239,33 @@ def test_prefill_shapes(built, counts, starts):
     check_prefill(cache, 9, tables_for(lengths, 16, cache.c.max_blocks, 13), counts, starts, "f32")
 
 
+@pytest.mark.parametrize("heads,kv_heads,dim,dtype", [(9, 3, 64, "f32"), (32, 8, 128, "bf16"), (16, 2, 128, "f32"),
+                                                      (8, 8, 64, "bf16")])
+def test_prefill_many_items_per_sm(built, heads, kv_heads, dim, dtype):
+    """Several items of unlike shapes one after the other on every SM: blocks whose rows fill one tile of vectors or
+    two, tiles of which one sees fewer tokens, items that end on the next SM."""
+    rows = 2 * (128 * kv_heads // heads)
+    counts = [1, rows, rows // 2 + 1, 3, 2 * rows + 5, rows // 2] * 24
+    starts = [(37 * i) % 700 for i in range(len(counts))]
+    lengths = [s + c for s, c in zip(starts, counts)]
+    cache = Cache(sum(-(-n // 16) for n in lengths), kv_heads, dim, 16, "int8")
+    check_prefill(cache, heads, tables_for(lengths, 16, cache.c.max_blocks, 44), counts, starts, dtype)
+
+
+@pytest.mark.parametrize("low", [-40, -100])
+def test_prefill_tiny_value_scales(built, low):
+    """Blocks whose V scale is far below the others' count in the sum of weights alone."""
+    counts, starts = [60, 9], [300, 0]
+    cache = Cache(40, 3, 64, 16, "int8")
+    tables = tables_for([360, 9], 16, 40, 45)
+    fill(cache, tables, [360, 9], 46, (-6, -6))
+    cache.scales[tables[0, 2:20:3].long(), :, 1] = 2.0 ** low
+    cache.scales[tables[1, 0].long(), 1, 1] = 0.0
+    q, out = prefill(cache, 9, tables, counts, starts, "f32", q=torch.randn(69, 576, device=DEV) * 6)
+    check_rows(cache, 9, q[:60], out[:60], tables[0].tolist(), 360, 0.125, False)
+    check_rows(cache, 9, q[60:], out[60:], tables[1].tolist(), 9, 0.125, False)
+
+
 def test_prefill_ranges(built):
     """Block scales far apart, queries of any size next to each other."""
     counts, starts = [70, 5], [50, 200]

@@ -13,11 +13,11 @@
 // 64 bits measured 24 us for 8192 rows of 9 + 3 + 3 heads x 64 FP32, and 290 us for 20447 rows of
 // 32 + 8 + 8 heads x 128 BF16: its conversions bound it.)
 //
-// Bound by HBM. A CTA takes up to 16 packed rows: all its threads rotate their q, and its
+// Bound by HBM. A CTA takes up to 8 packed rows: all its threads rotate their q, and its
 // warps write the tiles of the blocks that begin among its rows (a tile's first appended row
 // is in one CTA only). A tile is (block, kv head, K or V); its scale needs the largest
-// magnitude of all its new tokens, so one warp takes it whole, 8 or 16 tokens in registers at
-// a time, twice: magnitude, then codes. Fewer rows per CTA when there are few (one for a
+// magnitude of all its new tokens, so one warp takes it whole, 16 tokens (8 of head_dim 128) in
+// registers at a time, twice: magnitude, then codes. Fewer rows per CTA when there are few (one for a
 // decode step), so that all SMs take part.
 #include "kv8.cuh"
 
@@ -25,8 +25,7 @@ namespace mpb {
 namespace kv8 {
 namespace {
 
-constexpr int kThreads = 256;
-constexpr int kMaxRows = 16;  // rows of a CTA
+constexpr int kMaxRows = 8;  // rows of a CTA (16 and 4 were no faster)
 constexpr float kHuge = 8.5e37f;  // 2^126: FP32 products and sums below it are finite
 
 // A lane's eight values of one head row: two groups of four, at i0 and i1. Chunk c of
@@ -197,57 +196,67 @@ __device__ __noinline__ float exact_largest(const T* at, int64_t stride, int n, 
 // ---------------------------------------------------------------- a tile, by one warp
 template <class T, int F, int D, bool kInterleaved>
 __device__ __forceinline__ void append_tile(const AppendParams& p, const T* rows, int64_t stride, int head, int part,
-                                            int block, int slot0, int n, int position, int lane) {
+                                            const int32_t* entry, int slot0, int n, int position, int lane) {
     constexpr int kLanes = D / 8;        // lanes of one token
     constexpr int kStep = 32 / kLanes;   // tokens a warp reads at once
-    constexpr int kUnitTokens = sizeof(T) == 4 && D == 128 ? 8 : 16;  // in registers at a time
-    constexpr int kSteps = kUnitTokens / kStep;                       // a lane's share
+    constexpr int kSteps = 4, kUnitTokens = kSteps * kStep;  // a lane's tokens at a time, and the warp's
     const int sub = lane / kLanes, rotary = part ? 0 : p.rotary_dim;
     const Angles angles{p.cos, p.sin, rotary / 2};
     const Chunk ch = chunk_of<kInterleaved>(lane % kLanes, rotary);
     const T* at = rows + head * D;
+    // a lane's values of kSteps tokens, rotated; what any of a token's may be off by (0: they are exact)
+    float x[kSteps][8], e[kSteps];
     Raw<T> raw[kSteps];
     auto load = [&](int first) {
 #pragma unroll
-        for (int i = 0; i < kSteps; ++i)
-            if (first + i * kStep + sub < n) raw[i].load(at + (first + i * kStep + sub) * stride, ch);
-    };
-    // a token's values; what any of them may be off by (0: they are exact), and their largest magnitude
-    auto values = [&](const Raw<T>& r, int t, float (&x)[8], float& e, float& top) {
-        r.widen(x);
-        e = 0.f;
-        if (ch.pair >= 0) {
-            float c[4], s[4];
-            angles.load(position + t, ch.pair, c, s);
-            e = rotate<kInterleaved>(x, c, s);
+        for (int i = 0; i < kSteps; ++i) {
+            const int t = first + i * kStep + sub;
+            raw[i] = {};
+            if (t < n) raw[i].load(at + t * stride, ch);
         }
-        top = 0.f;
-#pragma unroll
-        for (int j = 0; j < 8; ++j) top = fmaxf(top, fabsf(x[j]));
-        if (ch.pair >= 0) e = (e + top) * 1.1920929e-7f;
     };
+    auto turn = [&](int first) {
+        if (ch.pair >= 0) {
+            float c[kSteps][4], s[kSteps][4];
+#pragma unroll
+            for (int i = 0; i < kSteps; ++i) angles.load(position + min(first + i * kStep + sub, n - 1), ch.pair, c[i], s[i]);
+#pragma unroll
+            for (int i = 0; i < kSteps; ++i) {
+                raw[i].widen(x[i]);
+                e[i] = rotate<kInterleaved>(x[i], c[i], s[i]);
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < kSteps; ++i) raw[i].widen(x[i]), e[i] = 0.f;
+        }
+    };
+    load(0);
+    const int block = *entry;  // in flight with the values
     // bounds of the largest magnitude; `sum` becomes NaN if a value is not finite
     float most = 0.f, least = 0.f, sum = 0.f;
     for (int first = 0; first < n; first += kUnitTokens) {
-        load(first);
+        if (first) load(first);
+        turn(first);
 #pragma unroll
         for (int i = 0; i < kSteps; ++i) {
-            const int t = first + i * kStep + sub;
-            if (t >= n) break;
-            float x[8], e, top;
-            values(raw[i], t, x, e, top);
-            most = fmaxf(most, top + e);
-            least = fmaxf(least, top - e);
+            float top = 0.f;
 #pragma unroll
-            for (int j = 0; j < 8; ++j) sum = fmaf(x[j], 0.f, sum);
+            for (int j = 0; j < 8; ++j) top = fmaxf(top, fabsf(x[i][j])), sum = fmaf(x[i][j], 0.f, sum);
+            if (ch.pair >= 0) e[i] = (e[i] + top) * 1.1920929e-7f;
+            most = fmaxf(most, top + e[i]);
+            least = fmaxf(least, top - e[i]);
         }
     }
     const bool wide = __any_sync(0xffffffffu, !(most < kHuge) || isnan(sum));  // e does not hold, or not finite
     most = warp_max(most), least = warp_max(least);
+    if (unsigned(block) >= unsigned(p.cache.max_blocks)) {
+        if (lane == 0) raise_error(p.error, kErrBounds);
+        return;
+    }
     bool odd = false;
-    int x = scale_exponent<F>(least);
-    if (wide || x != scale_exponent<F>(most))
-        x = scale_exponent<F>(exact_largest<T, kInterleaved>(at, stride, n, D, angles, rotary, position, lane, &odd));
+    int power = scale_exponent<F>(least);
+    if (wide || power != scale_exponent<F>(most))
+        power = scale_exponent<F>(exact_largest<T, kInterleaved>(at, stride, n, D, angles, rotary, position, lane, &odd));
     float* scale = p.cache.scales + int64_t(block) * p.cache.scale_stride + head * 2 + part;
     unsigned char* tile = p.cache.pages + tile_offset(p.cache, block, head, part, D);
     if (slot0 > 0) {
@@ -255,10 +264,10 @@ __device__ __forceinline__ void append_tile(const AppendParams& p, const T* rows
         const int bits = __float_as_int(held), e = (bits >> 23) - 127;
         if ((bits & 0x807fffff) != 0 || e < -126 || e > 127) {
             odd = true;  // not a power of two: the held codes stay as they are under the new scale
-        } else if (e >= x) {
-            x = e;
+        } else if (e >= power) {
+            power = e;
         } else {
-            const float ratio = e - x < -126 ? 0.f : pow2(e - x);
+            const float ratio = e - power < -126 ? 0.f : pow2(e - power);
             for (int i = lane; i < slot0 * D / 16; i += 32) {
                 uint4* w = reinterpret_cast<uint4*>(tile) + i;
                 const uint4 v = *w;
@@ -268,29 +277,36 @@ __device__ __forceinline__ void append_tile(const AppendParams& p, const T* rows
         }
         __syncwarp();
     }
-    if (lane == 0) *scale = pow2(x);
-    const float inv = pow2(-x);
+    if (lane == 0) *scale = pow2(power);
+    const float inv = pow2(-power);
     for (int first = 0; first < n; first += kUnitTokens) {
-        if (n > kUnitTokens) load(first);  // else still there
+        if (n > kUnitTokens) {  // else still there
+            load(first);
+            turn(first);
+        }
 #pragma unroll
         for (int i = 0; i < kSteps; ++i) {
             const int t = first + i * kStep + sub;
-            if (t >= n) break;
-            float x[8], e, top;
-            values(raw[i], t, x, e, top);
+            if (t >= n) continue;
             uint32_t w[2];
             bool near = wide;  // a border of codes lies within what a value may be off by
             if (ch.pair < 0) {
 #pragma unroll
-                for (int j = 0; j < 2; ++j)
-                    w[j] = encode4<F>(x[4 * j] * inv, x[4 * j + 1] * inv, x[4 * j + 2] * inv, x[4 * j + 3] * inv);
+                for (int j = 0; j < 8; j += 4)
+                    w[j / 4] = encode4<F>(x[i][j] * inv, x[i][j + 1] * inv, x[i][j + 2] * inv, x[i][j + 3] * inv);
             } else {
-                const float d = fmaf(e, inv, 9.094947e-13f);  // 2^-40: products that lost bits below FP32's exponents
+                if (n > kUnitTokens) {
+                    float top = 0.f;
 #pragma unroll
-                for (int j = 0; j < 2; ++j) {
-                    const float* v = x + 4 * j;
-                    w[j] = encode4<F>(fmaf(v[0], inv, -d), fmaf(v[1], inv, -d), fmaf(v[2], inv, -d), fmaf(v[3], inv, -d));
-                    near |= w[j] != encode4<F>(fmaf(v[0], inv, d), fmaf(v[1], inv, d), fmaf(v[2], inv, d), fmaf(v[3], inv, d));
+                    for (int j = 0; j < 8; ++j) top = fmaxf(top, fabsf(x[i][j]));
+                    e[i] = (e[i] + top) * 1.1920929e-7f;
+                }
+                const float d = fmaf(e[i], inv, 9.094947e-13f);  // 2^-40: products that lost bits below FP32's exponents
+#pragma unroll
+                for (int j = 0; j < 8; j += 4) {
+                    const float* v = x[i] + j;
+                    w[j / 4] = encode4<F>(fmaf(v[0], inv, -d), fmaf(v[1], inv, -d), fmaf(v[2], inv, -d), fmaf(v[3], inv, -d));
+                    near |= w[j / 4] != encode4<F>(fmaf(v[0], inv, d), fmaf(v[1], inv, d), fmaf(v[2], inv, d), fmaf(v[3], inv, d));
                 }
             }
             if (near) {
@@ -310,37 +326,48 @@ struct Place {
     int seq, position, end;  // end: the sequence's last row + 1
 };
 
-// By one warp: the row's sequence is the first that ends behind it, found 32 ways at a time.
-__device__ __forceinline__ Place find_row(const AppendParams& p, int row, int lane) {
-    int low = 0, high = p.count;
-    while (high - low > 32) {
-        const int step = (high - low + 31) / 32, i = low + (lane + 1) * step - 1;
-        const int k = __popc(__ballot_sync(0xffffffffu, i < high && p.row_offsets[i + 1] <= row));
-        low += k * step;
-        high = min(high, low + step);
+// By one warp, a row per lane from `row0` on (rows <= 32): a row's sequence is the first that
+// ends behind it. With sequences of one length it is known for row0; else it is found 32
+// ways at a time. From there on step by step.
+__device__ __forceinline__ Place find_rows(const AppendParams& p, int row0, int rows, int lane) {
+    int low = int(int64_t(row0) * p.count / p.rows);
+    const int guess = low, start_there = p.starts[low];
+    if (p.row_offsets[low] > row0 || p.row_offsets[low + 1] <= row0) {
+        low = 0;
+        int high = p.count;
+        while (high - low > 32) {
+            const int step = (high - low + 31) / 32, i = low + (lane + 1) * step - 1;
+            const int k = __popc(__ballot_sync(0xffffffffu, i < high && p.row_offsets[i + 1] <= row0));
+            low += k * step;
+            high = min(high, low + step);
+        }
+        low += __popc(__ballot_sync(0xffffffffu, low + lane < high && p.row_offsets[low + lane + 1] <= row0));
     }
-    low += __popc(__ballot_sync(0xffffffffu, low + lane < high && p.row_offsets[low + lane + 1] <= row));
+    const int row = row0 + lane;
+    if (lane >= rows) return {-1, 0, 0};
+    int end = 0;
+    while (low < p.count && (end = p.row_offsets[low + 1]) <= row) ++low;
     if (low >= p.count) return {-1, 0, 0};
-    const int begin = p.row_offsets[low], end = min(p.row_offsets[low + 1], p.rows), start = p.starts[low];
+    const int begin = p.row_offsets[low], start = low == guess ? start_there : p.starts[low];
     const int64_t position = int64_t(start) + row - begin;
-    if (row < begin || row >= end || start < 0 || position >= int64_t(p.table_stride) * p.cache.block_tokens ||
+    if (row < begin || start < 0 || position >= int64_t(p.table_stride) * p.cache.block_tokens ||
         (p.rotary_dim && position >= p.max_positions)) {
-        if (lane == 0) raise_error(p.error, kErrBounds);
+        raise_error(p.error, kErrBounds);
         return {-1, 0, 0};
     }
-    return {low, int(position), end};
+    return {low, int(position), min(end, p.rows)};
 }
 
-template <class T, int F, int D, bool kInterleaved>
-__global__ void __launch_bounds__(kThreads, 3) append_kernel(const AppendParams p, int rows_each, uint32_t per_row_inverse) {
+template <class T, int F, int D, bool kInterleaved, int kThreads>
+__global__ void __launch_bounds__(kThreads, kThreads == 128 ? 5 : 2) append_kernel(const AppendParams p, int rows_each, uint32_t per_row_inverse) {
     constexpr int kChunks = D / 8;
     __shared__ Place places[kMaxRows];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     pdl_enter();
     const int row0 = blockIdx.x * rows_each, rows = min(rows_each, p.rows - row0);
-    for (int i = warp; i < rows; i += kThreads / 32) {
-        const Place at = find_row(p, row0 + i, lane);
-        if (lane == 0) places[i] = at;
+    if (warp == 0) {
+        const Place at = find_rows(p, row0, rows, lane);
+        if (lane < rows) places[lane] = at;
     }
     __syncthreads();
     // ---- tiles of the blocks whose first appended row is here
@@ -352,18 +379,14 @@ __global__ void __launch_bounds__(kThreads, 3) append_kernel(const AppendParams 
         if (at.seq < 0) continue;
         if (slot && row0 + i != p.row_offsets[at.seq]) continue;
         const int row = row0 + i;
-        const int block = p.tables[int64_t(at.seq) * p.table_stride + at.position / bt];
+        const int32_t* entry = p.tables + int64_t(at.seq) * p.table_stride + at.position / bt;
         int n = min(bt - slot, at.end - row);
         if (p.rotary_dim) n = min(n, p.max_positions - at.position);  // rows past the tables report themselves
-        if (unsigned(block) >= unsigned(p.cache.max_blocks)) {
-            if (tid == 0) raise_error(p.error, kErrBounds);
-            continue;
-        }
         for (; turn < tiles; turn += kThreads / 32) {
             const int head = turn >> 1, part = turn & 1;
             const T* x = static_cast<const T*>(part ? p.v : p.k);
             const int64_t stride = part ? p.v_stride : p.k_stride;
-            append_tile<T, F, D, kInterleaved>(p, x + row * stride, stride, head, part, block, slot, n, at.position, lane);
+            append_tile<T, F, D, kInterleaved>(p, x + row * stride, stride, head, part, entry, slot, n, at.position, lane);
         }
         turn -= tiles;
     }
@@ -411,10 +434,19 @@ cudaError_t launch_append(const AppendParams& p, int type, int format, int head_
         const int each = std::clamp(p.rows / (2 * 148), 1, kMaxRows);
         using T = decltype(t);
         constexpr int kFormat = decltype(f)::value, kDim = decltype(d)::value;
-        // x / per_row = high half of x * inverse while x * per_row < 2^32: x < 16 * per_row, per_row <= 2^14
+        // x / per_row = high half of x * inverse while x * per_row < 2^32: x < 8 * per_row, per_row <= 2^14
         const uint32_t per_row = p.heads * (kDim / 8), inverse = uint32_t(((uint64_t(1) << 32) + per_row - 1) / per_row);
-        return launch_pdl(p.interleaved ? append_kernel<T, kFormat, kDim, true> : append_kernel<T, kFormat, kDim, false>,
-                          dim3((p.rows + each - 1) / each), dim3(kThreads), 0, stream, p, each, inverse);
+        // A row alone: 8 warps, so that its tiles are written side by side (5 rows, 256 rows: 4.1 and 5.1 us,
+        // 5.3 and 5.9 with 4 warps). More rows: 4 warps, of which more CTAs overlap (8192 rows of FP32:
+        // 17 us, 20 with 8 warps).
+        auto launch = [&](auto kernel, int threads) {
+            return launch_pdl(kernel, dim3((p.rows + each - 1) / each), dim3(threads), 0, stream, p, each, inverse);
+        };
+        if (each == 1)
+            return p.interleaved ? launch(append_kernel<T, kFormat, kDim, true, 256>, 256)
+                                 : launch(append_kernel<T, kFormat, kDim, false, 256>, 256);
+        return p.interleaved ? launch(append_kernel<T, kFormat, kDim, true, 128>, 128)
+                             : launch(append_kernel<T, kFormat, kDim, false, 128>, 128);
     });
 }
 

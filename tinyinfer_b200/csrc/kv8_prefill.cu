@@ -273,9 +273,10 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_kernel(const AttentionPar
     uint64_t *k_full = bars, *k_empty = bars + 2, *v_full = bars + 4, *v_empty = bars + 6;
     uint64_t *q_full = bars + 8, *p_full = bars + 10, *o_full = bars + 12, *joined = bars + 14, *q_free = bars + 16;  // per tile
     uint64_t *s_full = bars + 18, *scales_full = bars + 21;  // per place of S; per row of scales
-    uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(bars + 25);
-    int* failed = reinterpret_cast<int*>(bars + 26);
-    int* last = reinterpret_cast<int*>(bars + 27);  // [2] whether this CTA joins the parts, per tile
+    uint64_t* done = bars + 25;                              // a segment's products
+    uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(bars + 26);
+    int* failed = reinterpret_cast<int*>(bars + 27);
+    int* last = reinterpret_cast<int*>(bars + 28);  // [2] whether this CTA joins the parts, per tile
     int64_t* units_before = reinterpret_cast<int64_t*>(sm + S::kPlan);       // [kThreads + 1]
     int64_t* sums = units_before + kThreads + 1;                         // [32], [32]
     int* blocks_before = reinterpret_cast<int*>(sums + 64);                  // [kThreads + 1]
@@ -291,6 +292,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_kernel(const AttentionPar
         }
         for (int i = 0; i < S::kBuffers; ++i) mbar_init(s_full + i, 1);
         for (int i = 0; i < kScaleSlots; ++i) mbar_init(scales_full + i, 1);
+        mbar_init(done, 1);
         *failed = 0;
         fence_barrier_init();
     }
@@ -431,7 +433,10 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_kernel(const AttentionPar
             int unit_log = -110;
 #pragma unroll
             for (int d = 0; d < D; ++d) o[d] = 0.f;
-            if (!(ok = wait(q_free + w, free_phase))) break;  // the tile's other warps have left its query buffer
+            // The segment before is done, and the tile's other warps have left its query buffer. (A tile
+            // with fewer tokens, or none, would else run ahead, and S's places and the scales are waited for
+            // by the parity of their phase: one phase ahead passes for the one before.)
+            if (!(ok = wait(q_free + w, free_phase)) || !(ok = wait(done, free_phase))) break;
             free_phase ^= 1;
             if (tiles) {
                 // ---- query rows as FP16 halves, K-major with the 128-byte swizzle. A warp brings its rows, as they
@@ -487,8 +492,8 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_kernel(const AttentionPar
                         *reinterpret_cast<uint4*>(to + S::kTileBytes) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
                 }
                 fence_proxy_async_shared();
-                arrive(q_full + w);
             }
+            arrive(q_full + w);
             // O's row of this thread, times `by`
             auto add_outputs = [&](float by) {
 #pragma unroll
@@ -559,7 +564,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_kernel(const AttentionPar
                         top = fmaxf(top, t);
                         reach = fmaxf(reach, t + scale[g].z);
                     });
-                    const bool high = reach - m > float(unit_log) + kRoom || top > m + 60.f;
+                    const bool high = reach - m > float(unit_log) + kRoom || top > m + 20.f;
                     if (__any_sync(0xffffffffu, high)) {
                         if (high) {
                             const float m_new = fmaxf(m, top);
@@ -587,18 +592,18 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_kernel(const AttentionPar
                             }
                         }
                     }
-                    // weight * V scale = 2^(score - m + log2 scale - log2 unit + 8). A scale below unit * 2^-40
-                    // counts as that: its weights are zero in FP16 either way, but l needs them
+                    // weight * V scale = 2^(score - m + log2 scale - log2 unit + 8). A scale below unit * 2^-60
+                    // counts as that: its weights (up to 2^20 * 2^-52) are zero in FP16 either way, but l needs them
                     const float base_m = m == -INFINITY ? 0.f : m, shift = float(kTopLog - unit_log);
                     const float unit = pow2(unit_log);
                     [[maybe_unused]] const Pair minus_one = pair(-1.f, -1.f);
-                    const float least = fmaxf(unit * 9.094947e-13f, 1.17549435e-38f);
+                    const float least = fmaxf(unit * 8.6736174e-19f, 1.17549435e-38f);
                     each_group(Some{}, [&](float (&x)[16], int g) {
                         const float4 sc = scale[g];
                         const bool small = sc.y < least;
                         const float f = k_factor * sc.x;
-                        const float c = (small ? float(kTopLog - 40) : sc.z + shift) - base_m;
-                        const float back = small ? 4294967296.f : sc.w * (unit * (1.f / (1 << kTopLog)));
+                        const float c = (small ? float(kTopLog - 60) : sc.z + shift) - base_m;
+                        const float back = small ? 4503599627370496.f : sc.w * (unit * (1.f / (1 << kTopLog)));
                         const Pair ff = pair(f, f), cc = pair(c, c);
                         Pair sum = pair(0.f, 0.f);
                         uint32_t hi[8];
@@ -838,7 +843,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_kernel(const AttentionPar
             const uint64_t q_desc = smem_desc(sm + S::kQ), k_desc = smem_desc(sm + S::kK);
             const uint64_t v_desc = mn_desc(smem_u32(sm + S::kV), kN * 128);
             int slot = 0, used = 0;  // as in the softmax
-            uint32_t q_phase = 0, p_phase = 0;  // one bit per tile
+            uint32_t q_phase = 0, p_phase = 0;  // p_phase: one bit per tile
             Segment seg;
             bool ok = true;
             while (ok && cursor.next(seg)) {
@@ -854,6 +859,8 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_kernel(const AttentionPar
                 };
                 Next s{0, 0}, o{0, 0};
                 s.skip(n0, n1, most), o.skip(n0, n1, most);
+                if (!(ok = wait(q_full, q_phase) && wait(q_full + 1, q_phase))) break;
+                q_phase ^= 1;
                 for (int i = 0; ok && i < n0 + n1 + S::kBuffers; ++i) {
                     if (i >= S::kBuffers) {
                         const int stage = (slot + o.j) % kStages, place = (used + i - S::kBuffers) % S::kBuffers;
@@ -879,11 +886,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_kernel(const AttentionPar
                     }
                     if (i < n0 + n1) {
                         const int stage = (slot + s.j) % kStages, place = (used + i) % S::kBuffers;
-                        if (s.j == 0) {
-                            ok = wait(q_full + s.w, (q_phase >> s.w) & 1);
-                            q_phase ^= 1u << s.w;
-                        }
-                        ok = ok && wait(k_full + stage, ((slot + s.j) / kStages) & 1);
+                        ok = wait(k_full + stage, ((slot + s.j) / kStages) & 1);
                         if (!ok) break;
                         tmem_fence_after();
                         const uint32_t s_at = tmem + place * kN;
@@ -905,6 +908,9 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_kernel(const AttentionPar
                         s.step(), s.skip(n0, n1, most);
                     }
                 }
+                if (!ok) break;
+                if (elect()) mma_commit(done);
+                __syncwarp();
                 slot += most, used += n0 + n1;
             }
         }
