@@ -21,7 +21,8 @@ namespace {
 
 constexpr int kCtas = 148;
 constexpr int kSmemBytes = 227 * 1024;
-constexpr int kMinUnits = 4;  // units per warp before another CTA takes part: joining CTAs costs more
+constexpr int kMinUnits = 2;  // units per warp before another CTA takes part: joining CTAs costs about as much
+constexpr int kWholeUnits = 2;  // units per warp up to which a CTA takes an item whole, if there are CTAs for all
 
 template <class T, int D>
 __host__ __device__ constexpr int warps_of() {
@@ -42,7 +43,7 @@ __host__ __device__ constexpr Layout layout_of(int warps, int heads, int head_di
     Layout l{};
     const int stage = 2 * kUnit * head_dim;  // [tile][K, V][16 tokens][head_dim]
     const int partial = heads * (head_dim + 4) * 4;
-    const int misc = (warps * 32 + 1 + warps) * 8 + 4 * 4;  // scan, joins
+    const int misc = (warps * 32 + 1 + warps) * 8 + (4 + warps) * 4;  // scan, joins
     const int fixed = warps * 2 * partial + warps * 2 * int(sizeof(Record)) + misc;
     int stages = (kSmemBytes - fixed) / (warps * (stage + kTiles * 8));
     stages = stages > 3 ? 3 : stages;
@@ -131,6 +132,7 @@ __global__ void __launch_bounds__(warps_of<T, D>() * 32, 1)
     int64_t* sums = reinterpret_cast<int64_t*>(smem + lay.misc);  // [kWarps] units of each warp's rows
     int64_t* before = sums + kWarps;                              // [kThreads + 1] units before each thread's rows
     int* joins = reinterpret_cast<int*>(before + kThreads + 1);   // [2] CTAs to join (0: none), [2] their records
+    int* longest_of = joins + 4;                                  // [kWarps] most units of a row of each warp
     if (lane < 2) records[2 * warp + lane].units = 0;
     if (tid < 2) joins[tid] = 0;
     pdl_enter();
@@ -146,40 +148,60 @@ __global__ void __launch_bounds__(warps_of<T, D>() * 32, 1)
         return 0;
     };
     auto units_of = [&](int row) { return row < p.count ? int((unsigned(tokens(row)) + kUnit - 1) / kUnit) : 0; };
-    {
-        int64_t mine = 0;
-        for (int i = 0; i < share; ++i) mine += units_of(tid * share + i);
-        int64_t upto = mine;  // inclusive scan over the warp
+    // A CTA per item where that is few units for every warp (no CTA waits for another, and
+    // there is nothing to search); else equal runs.
+    int64_t mine = 0;
+    int most = 0;
+    for (int i = 0; i < share; ++i) {
+        const int u = units_of(tid * share + i);
+        mine += u, most = max(most, u);
+    }
+    int64_t upto = mine;  // inclusive scan over the warp
 #pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const int64_t x = __shfl_up_sync(0xffffffffu, upto, o);
-            if (lane >= o) upto += x;
+    for (int o = 1; o < 32; o <<= 1) {
+        const int64_t x = __shfl_up_sync(0xffffffffu, upto, o);
+        if (lane >= o) upto += x;
+    }
+    most = __reduce_max_sync(0xffffffffu, most);
+    if (lane == 31) sums[warp] = upto, longest_of[warp] = most;
+    __syncthreads();
+    most = __reduce_max_sync(0xffffffffu, lane < kWarps ? longest_of[lane] : 0);
+    const bool whole = int64_t(p.count) * per <= int64_t(gridDim.x) && most <= kWholeUnits * kWarps;
+    int row = 0, item = 0, unit = 0;
+    int ctas, cta_units = 0, extra = 0;
+    int64_t cta_begin = 0, base = 0;  // CTA c's run: `base` units, one more for the first `extra` CTAs
+    if (whole) {
+        ctas = p.count * per;
+        if (int(blockIdx.x) < ctas) {
+            row = blockIdx.x / per, item = blockIdx.x % per;
+            cta_units = units_of(row);
         }
-        if (lane == 31) sums[warp] = upto;
-        __syncthreads();
+    } else {
         int64_t x = lane < warp ? sums[lane] : 0;
 #pragma unroll
         for (int o = 16; o; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
         before[tid] = x + upto - mine;
         if (tid == kThreads - 1) before[kThreads] = x + upto;
         __syncthreads();
+        const int64_t total = before[kThreads] * per;
+        const int64_t want = (total + kWarps * kMinUnits - 1) / (kWarps * kMinUnits);
+        ctas = int(want < int64_t(gridDim.x) ? want : int64_t(gridDim.x));
+        const int parts = max(ctas, 1);
+        base = total >> 32 ? total / parts : int64_t(uint32_t(total) / uint32_t(parts));
+        extra = int(total - base * parts);
+        cta_begin = blockIdx.x * base + min(int(blockIdx.x), extra);
+        if (int(blockIdx.x) < ctas) cta_units = int(base) + (int(blockIdx.x) < extra);
     }
-    const int64_t total = before[kThreads] * per;
-    const int64_t want = (total + kWarps * kMinUnits - 1) / (kWarps * kMinUnits);
-    const int ctas = int(want < int64_t(gridDim.x) ? want : int64_t(gridDim.x));
-    // worker w's run: `base` units, one more for the first `extra` workers
-    const int workers = max(ctas, 1) * kWarps;
-    const int64_t base = total >> 32 ? total / workers : int64_t(uint32_t(total) / uint32_t(workers));
-    const int extra = int(total - base * workers);
     auto cta_of = [&](int64_t unit) {
         const int64_t split = extra * (base + 1);
-        return int(unit < split ? unit / (base + 1) : extra + (unit - split) / base) / kWarps;
+        return int(unit < split ? unit / (base + 1) : extra + (unit - split) / base);
     };
-    const int worker = blockIdx.x * kWarps + warp;
-    const int64_t begin = worker * base + min(worker, extra);
-    const int run = int(blockIdx.x) < ctas ? int(base) + (worker < extra) : 0;
-    int row = 0, item = 0, unit = 0;
-    if (run > 0) {
+    // the warp's run, likewise
+    const int each = cta_units / kWarps, more = cta_units % kWarps, run = each + (warp < more);
+    const int64_t begin = cta_begin + warp * each + min(warp, more);
+    if (whole) {
+        unit = int(begin);
+    } else if (run > 0) {
         // the last thread whose rows begin at or before `begin`, then the row among its rows
         int t = (31 - __clz(__ballot_sync(0xffffffffu, before[lane * kWarps] * per <= begin))) * kWarps;
         t += 31 - __clz(__ballot_sync(0xffffffffu, lane < kWarps && before[t + min(lane, kWarps - 1)] * per <= begin));
