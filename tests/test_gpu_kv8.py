@@ -588,3 +588,56 @@ def test_streams_and_shared_workspaces(built):
                 check_rows(cache, 9, q[i: i + 1], out[i: i + 1], tables[i].tolist(), n, 0.125, False)
             else:
                 assert bool((out[i] == 0).all())
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("heads,kv_heads,dim,counts", [
+    (4, 4, 64, [30, 0, 3, 1]), (4, 4, 64, [30, 0, 5]), (5, 1, 128, [100, 45]), (5, 1, 128, [100, 46]),
+    (40, 2, 64, [20, 1]), (40, 2, 64, [23])])
+def test_prefill_small_calls(built, heads, kv_heads, dim, counts, dtype):
+    """Up to 148 items of a row, a kv head and 8 query heads (three of the rows belong to nobody), and one more."""
+    starts = [17 * i + (200 if i else 0) for i in range(len(counts))]
+    cache = Cache(40, kv_heads, dim, 32, "int8")
+    lengths = [s + c for s, c in zip(starts, counts)]
+    check_prefill(cache, heads, tables_for(lengths, 32, 40, 61), counts, starts, dtype)
+
+
+def test_prefill_bad_metadata_in_a_long_call(built):
+    """As for a few rows: the bad sequence is reported and left, the others are computed."""
+    cache = Cache(30, 3, 64, 16, "int8")
+    tables = tables_for([160, 160], 16, 30, 62, spare=0)
+    fill(cache, tables, [160, 160], 63)
+    word = torch.zeros(1, dtype=torch.int32, device=DEV)
+    for rows in (20, 100):
+        for start in (161 - rows, -1, 2 ** 31 - 2):
+            q, out = prefill(cache, 9, tables, [rows, rows], [160 - rows, start], "f32", error=word)
+            assert mp.kv8_status(word.data_ptr(), stream()) == mp.MP_ERR_BOUNDS
+            check_rows(cache, 9, q[:rows], out[:rows], tables[0].tolist(), 160, 0.125, False)
+            assert bool((out[rows:] == 7).all())
+
+
+def test_decode_and_prefill_share_a_workspace(built):
+    """Calls of both kinds, one after the other, leave a workspace as the next one needs it."""
+    cache = Cache(200, 3, 64, 16, "int8")
+    tables = tables_for([1500, 900], 16, 200, 64)
+    fill(cache, tables, [1500, 900], 65)
+    workspace = torch.zeros(max(mp.kv8_decode_workspace(cache.c, 9), mp.kv8_prefill_workspace(cache.c, 9)),
+                            dtype=torch.uint8, device=DEV)
+    both = dict(tables=tables.data_ptr(), workspace=workspace.data_ptr(), workspace_bytes=workspace.numel(), type=0,
+                heads=9, table_stride=tables.stride(0), count=2, scale=0.125, q_stride=576, out_stride=576)
+    lens = torch.tensor([1500, 900], dtype=torch.int32, device=DEV)
+    word = torch.zeros(1, dtype=torch.int32, device=DEV)
+    for rows in (10, 300, 20, 700):
+        q, out = values(2 * rows, 576, 66), torch.zeros(2 * rows, 576, device=DEV)
+        offsets = torch.tensor([0, rows, 2 * rows], dtype=torch.int32, device=DEV)
+        starts = lens - rows
+        mp.kv8_attention_prefill(cache.c, mp.Kv8PrefillArgs(q=q.data_ptr(), out=out.data_ptr(), rows=2 * rows,
+                                 row_offsets=offsets.data_ptr(), starts=starts.data_ptr(), **both), word.data_ptr(), stream())
+        one = torch.zeros(2, 576, device=DEV)
+        last = torch.stack([q[rows - 1], q[-1]])
+        mp.kv8_attention_decode(cache.c, mp.Kv8DecodeArgs(q=last.data_ptr(), out=one.data_ptr(),
+                                lengths=lens.data_ptr(), **both), word.data_ptr(), stream())
+        assert mp.kv8_status(word.data_ptr(), stream()) == mp.MP_OK
+        for i, n in enumerate((1500, 900)):
+            check_rows(cache, 9, q[i * rows: (i + 1) * rows], out[i * rows: (i + 1) * rows], tables[i].tolist(), n, 0.125, False)
+            check_rows(cache, 9, last[i: i + 1], one[i: i + 1], tables[i].tolist(), n, 0.125, False)

@@ -11,6 +11,9 @@
 namespace mpb {
 namespace kv8 {
 
+constexpr int kCtas = 148;            // one per SM
+constexpr int kPackedItems = kCtas;   // items up to which a prefill goes row by row (kv8_prefill.cu)
+constexpr int kCounterBytes = kCtas * 2 * 4 + 96;  // of the attentions' workspaces: zero between calls; partials follow
 constexpr unsigned kErrValue = 4u;  // error word bit: a value (or a held block's scale) that cannot be quantised
 
 struct Cache {
@@ -42,6 +45,7 @@ struct AttentionParams {
     const int32_t* starts;       // prefill
     void* workspace;
     int heads, table_stride, count, rows;
+    int sequences;  // launch_packed: of the prefill; count is its rows
     float scale;
     unsigned* error;
 };
@@ -49,6 +53,8 @@ struct AttentionParams {
 cudaError_t launch_append(const AppendParams& p, int type, int format, int head_dim, cudaStream_t stream);
 cudaError_t launch_decode(const AttentionParams& p, int type, int format, int head_dim, cudaStream_t stream);
 cudaError_t launch_prefill(const AttentionParams& p, int type, int format, int head_dim, cudaStream_t stream);
+// Prefill with at most kPackedItems (row, kv head, 8 query heads) items, row by row.
+cudaError_t launch_packed(AttentionParams p, int type, int format, int head_dim, cudaStream_t stream);
 size_t decode_workspace(int group, int head_dim);
 size_t prefill_workspace(int group, int head_dim);
 
@@ -86,6 +92,18 @@ __device__ __forceinline__ int block_id(const Cache& c, const int32_t* table, in
         return 0;
     }
     return b;
+}
+
+// Rows of a prefill's sequence i, 0 for one whose metadata is out of range.
+__device__ __forceinline__ int sequence_rows(const AttentionParams& p, int i, int& begin, int& start) {
+    begin = p.row_offsets[i], start = p.starts[i];
+    const int end = p.row_offsets[i + 1];
+    if (begin < 0 || end < begin || end > p.rows || (end > begin && start < 0) ||
+        int64_t(start) + (end - begin) > int64_t(p.table_stride) * p.cache.block_tokens) {
+        if (end != begin) raise_error(p.error, kErrBounds);
+        return 0;
+    }
+    return end - begin;
 }
 
 // 2^x as a float, x in -126 .. 127.

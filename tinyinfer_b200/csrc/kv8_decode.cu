@@ -1,4 +1,5 @@
-// mp_kv8_attention_decode: one query row per sequence over the 8-bit paged cache (sm_100a).
+// mp_kv8_attention_decode: one query row per sequence over the 8-bit paged cache (sm_100a);
+// and the rows of small mp_kv8_attention_prefill calls (kPacked).
 //
 // Bound by HBM: a token costs 2 head_dim bytes per kv head and 4 head_dim flops per query
 // head. The work is cut into units of 32 tokens of one (row, kv head, up to 8 query heads)
@@ -19,7 +20,6 @@ namespace mpb {
 namespace kv8 {
 namespace {
 
-constexpr int kCtas = 148;
 constexpr int kSmemBytes = 227 * 1024;
 constexpr int kMinUnits = 2;  // units per warp before another CTA takes part: joining CTAs costs about as much
 constexpr int kWholeUnits = 2;  // units per warp up to which a CTA takes an item whole, if there are CTAs for all
@@ -43,7 +43,7 @@ __host__ __device__ constexpr Layout layout_of(int warps, int heads, int head_di
     Layout l{};
     const int stage = 2 * kUnit * head_dim;  // [tile][K, V][16 tokens][head_dim]
     const int partial = heads * (head_dim + 4) * 4;
-    const int misc = (warps * 32 + 1 + warps) * 8 + (4 + warps) * 4;  // scan, joins
+    const int misc = (warps * 32 + 1 + warps) * 8 + (4 + warps + 2 * kPackedItems) * 4;  // scan, joins, packed rows
     const int fixed = warps * 2 * partial + warps * 2 * int(sizeof(Record)) + misc;
     int stages = (kSmemBytes - fixed) / (warps * (stage + kTiles * 8));
     stages = stages > 3 ? 3 : stages;
@@ -115,7 +115,7 @@ struct Joined {
     }
 };
 
-template <class T, int F, int D>
+template <class T, int F, int D, bool kPacked>
 __global__ void __launch_bounds__(warps_of<T, D>() * 32, 1)
     decode_kernel(const AttentionParams p) {
     constexpr int kWarps = warps_of<T, D>(), kThreads = kWarps * 32, kStage = 2 * kUnit * D;
@@ -141,7 +141,32 @@ __global__ void __launch_bounds__(warps_of<T, D>() * 32, 1)
     const int bt = p.cache.block_tokens;
     const int64_t longest = int64_t(p.table_stride) * bt;
     const int share = (p.count + kThreads - 1) / kThreads;
+    // Packed rows: each one's sequence, and tokens up to its position (0: no row, or out of range)
+    int *row_tokens = longest_of + kWarps, *row_seq = row_tokens + kPackedItems;
+    if constexpr (kPacked) {
+        if (tid < p.count) {
+            int low = 0, high = p.sequences;  // the first sequence that ends behind the row
+            while (low < high) {
+                const int i = (low + high) / 2;
+                if (p.row_offsets[i + 1] <= tid) {
+                    low = i + 1;
+                } else {
+                    high = i;
+                }
+            }
+            int n = 0;
+            if (low < p.sequences) {
+                int first, start;
+                const int rows = sequence_rows(p, low, first, start);
+                if (tid >= first && tid < first + rows) n = start + tid - first + 1;
+            }
+            row_tokens[tid] = n, row_seq[tid] = low;
+        }
+        __syncthreads();
+    }
+    auto table_of = [&](int row) { return p.tables + int64_t(kPacked ? row_seq[row] : row) * p.table_stride; };
     auto tokens = [&](int row) {
+        if constexpr (kPacked) return row_tokens[row];
         const int n = p.lengths[row];
         if (n >= 0 && n <= longest) return n;
         raise_error(p.error, kErrBounds);
@@ -250,8 +275,7 @@ __global__ void __launch_bounds__(warps_of<T, D>() * 32, 1)
                     w_scale = make_float2(0.f, 0.f);
                     if (tile * kTile < c_len && lane < kTiles * c_left) {
                         const int kh = c_item / subs;
-                        const int block = block_id(p.cache, p.tables + int64_t(c_row) * p.table_stride, p.table_stride,
-                                                   tile / in_page, p.error);
+                        const int block = block_id(p.cache, table_of(c_row), p.table_stride, tile / in_page, p.error);
                         w_scale = *reinterpret_cast<const float2*>(p.cache.scales + block * p.cache.scale_stride + 2 * kh);
                         w_at = p.cache.pages + tile_offset(p.cache, block, kh, 0, D) + tile % in_page * (kTile * D);
                     }
@@ -285,7 +309,10 @@ __global__ void __launch_bounds__(warps_of<T, D>() * 32, 1)
         __syncwarp();
 
         // rows without tokens, while the copies fly
-        for (int r = blockIdx.x * kWarps + warp; r < p.count; r += gridDim.x * kWarps)
+        // (packed: sequences that no row was found in have their metadata checked too)
+        for (int r = blockIdx.x * kThreads + tid, at, from; kPacked && r < p.sequences; r += gridDim.x * kThreads)
+            sequence_rows(p, r, at, from);
+        for (int r = blockIdx.x * kWarps + warp; !kPacked && r < p.count; r += gridDim.x * kWarps)
             if (tokens(r) == 0) {
                 T* out = static_cast<T*>(p.out) + r * p.out_stride;
                 for (int i = lane; i < p.heads * D / 4; i += 32) store4(out + 4 * i, 0.f, 0.f, 0.f, 0.f);
@@ -357,7 +384,7 @@ __global__ void __launch_bounds__(warps_of<T, D>() * 32, 1)
     __syncthreads();
 
     // ---- join the warps' partials: the warp of an item's first record in this CTA joins them
-    float* store = reinterpret_cast<float*>(static_cast<unsigned char*>(p.workspace) + kCtas * 4 + 48);
+    float* store = reinterpret_cast<float*>(static_cast<unsigned char*>(p.workspace) + kCounterBytes);
     unsigned* counters = static_cast<unsigned*>(p.workspace);
     auto same = [&](const Record& a, const Record& b) { return b.units && a.row == b.row && a.item == b.item; };
     auto output = [&](const Record& r) {
@@ -425,20 +452,30 @@ __global__ void __launch_bounds__(warps_of<T, D>() * 32, 1)
 }  // namespace
 
 size_t decode_workspace(int group, int head_dim) {
-    return kCtas * 4 + 48 + size_t(kCtas) * 2 * (group < 8 ? group : 8) * (head_dim + 4) * 4;
+    return kCounterBytes + size_t(kCtas) * 2 * (group < 8 ? group : 8) * (head_dim + 4) * 4;
 }
 
-cudaError_t launch_decode(const AttentionParams& p, int type, int format, int head_dim, cudaStream_t stream) {
+template <bool kPacked>
+static cudaError_t launch(const AttentionParams& p, int type, int format, int head_dim, cudaStream_t stream) {
     return dispatch(type, format, head_dim, [&](auto t, auto f, auto d) {
         using T = decltype(t);
         constexpr int kDim = decltype(d)::value, kWarps = warps_of<T, kDim>();
-        auto kernel = decode_kernel<T, decltype(f)::value, kDim>;
+        auto kernel = decode_kernel<T, decltype(f)::value, kDim, kPacked>;
         const int group = p.heads / p.cache.kv_heads;
         const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes);
         if (e != cudaSuccess) return e;
         return launch_pdl(kernel, dim3(kCtas), dim3(kWarps * 32), size_t(layout_of(kWarps, group < 8 ? group : 8, kDim).total),
                           stream, p);
     });
+}
+
+cudaError_t launch_decode(const AttentionParams& p, int type, int format, int head_dim, cudaStream_t stream) {
+    return launch<false>(p, type, format, head_dim, stream);
+}
+
+cudaError_t launch_packed(AttentionParams p, int type, int format, int head_dim, cudaStream_t stream) {
+    p.sequences = p.count, p.count = p.rows;
+    return launch<true>(p, type, format, head_dim, stream);
 }
 
 }  // namespace kv8

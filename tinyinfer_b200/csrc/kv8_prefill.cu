@@ -32,6 +32,8 @@
 //
 // Bound by the tensor core, exp2 and the softmax's other instructions alike: per 256
 // vectors x 128 tokens of FP32 at head_dim 64 each takes about 2050 cycles.
+#include <algorithm>
+
 #include "kv8.cuh"
 #include "umma.cuh"
 
@@ -39,7 +41,6 @@ namespace mpb {
 namespace kv8 {
 namespace {
 
-constexpr int kCtas = 148;
 constexpr int kWidenWarp = 8, kProductWarp = 12, kThreads = 512;
 constexpr int kM = 128;       // vectors of a tile
 constexpr int kN = 128;       // tokens of a K/V tile
@@ -219,17 +220,6 @@ struct Cursor {
     int64_t at;               // device-wide index of the next unit
     int left;
 
-    // rows of sequence i, 0 for one whose metadata is out of range
-    static __device__ __forceinline__ int rows_of(const AttentionParams& p, int i, int& begin, int& start) {
-        begin = p.row_offsets[i], start = p.starts[i];
-        const int end = p.row_offsets[i + 1];
-        if (begin < 0 || end < begin || end > p.rows || (end > begin && start < 0) ||
-            int64_t(start) + (end - begin) > int64_t(p.table_stride) * p.cache.block_tokens) {
-            if (end != begin) raise_error(p.error, kErrBounds);
-            return 0;
-        }
-        return end - begin;
-    }
     static __device__ __forceinline__ int units_of(int start, int rows, int block, int block_rows) {
         return kSetup + (start + min((block + 1) * block_rows, rows) + kN - 1) / kN;
     }
@@ -242,10 +232,10 @@ struct Cursor {
     }
     __device__ __forceinline__ bool advance(Segment& s) {
         if (left <= 0) return false;
-        int begin, start, rows = rows_of(*p, seq, begin, start);
+        int begin, start, rows = sequence_rows(*p, seq, begin, start);
         while (block * block_rows >= rows) {
             block = 0, head = 0, k = 0;
-            rows = rows_of(*p, ++seq, begin, start);
+            rows = sequence_rows(*p, ++seq, begin, start);
         }
         s.seq = seq, s.head = head;
         s.row0 = begin + block * block_rows;
@@ -320,7 +310,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_kernel(const AttentionPar
         int mine = 0;
         for (int i = 0; i < share; ++i)
             if (tid * share + i < p.count)
-                mine += (Cursor::rows_of(p, tid * share + i, begin, start) + block_rows - 1) / block_rows;
+                mine += (sequence_rows(p, tid * share + i, begin, start) + block_rows - 1) / block_rows;
         const int before = int(scan(mine, sums));
         blocks_before[tid] = before;
         if (tid == kThreads - 1) blocks_before[kThreads] = before + mine;
@@ -335,7 +325,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_kernel(const AttentionPar
             if (blocks_before[t + o] <= f) t += o;
         block = f - blocks_before[t];
         for (seq = t * share;; ++seq) {
-            const int n = (Cursor::rows_of(p, seq, begin, start) + block_rows - 1) / block_rows;
+            const int n = (sequence_rows(p, seq, begin, start) + block_rows - 1) / block_rows;
             if (block < n) return;
             block -= n;
         }
@@ -345,9 +335,9 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_kernel(const AttentionPar
         if (tid * each < blocks) {
             int seq, block;
             locate(tid * each, seq, block);
-            int rows = Cursor::rows_of(p, seq, begin, start);
+            int rows = sequence_rows(p, seq, begin, start);
             for (int i = 0; i < min(each, blocks - tid * each); ++i, ++block) {
-                while (block * block_rows >= rows) block = 0, rows = Cursor::rows_of(p, ++seq, begin, start);
+                while (block * block_rows >= rows) block = 0, rows = sequence_rows(p, ++seq, begin, start);
                 mine += Cursor::units_of(start, rows, block, block_rows);
             }
         }
@@ -375,8 +365,8 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_kernel(const AttentionPar
             if (units_before[t + o] * heads <= cursor.at) t += o;
         locate(t * each, cursor.seq, cursor.block);
         int64_t in = cursor.at - units_before[t] * heads;
-        for (int rows = Cursor::rows_of(p, cursor.seq, begin, start);; ++cursor.block) {
-            while (cursor.block * block_rows >= rows) cursor.block = 0, rows = Cursor::rows_of(p, ++cursor.seq, begin, start);
+        for (int rows = sequence_rows(p, cursor.seq, begin, start);; ++cursor.block) {
+            while (cursor.block * block_rows >= rows) cursor.block = 0, rows = sequence_rows(p, ++cursor.seq, begin, start);
             const int n = Cursor::units_of(start, rows, cursor.block, block_rows);
             if (in < int64_t(n) * heads) {
                 cursor.head = int(in) / n, cursor.k = int(in) % n;
@@ -688,7 +678,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_kernel(const AttentionPar
             // a CTA: the item began earlier, slot 1: it begins here. Vectors side by side.
             constexpr int64_t kPart = int64_t(kM) * (D + 2);
             unsigned* counters = static_cast<unsigned*>(p.workspace);
-            float* parts = reinterpret_cast<float*>(static_cast<unsigned char*>(p.workspace) + kCtas * 2 * 4 + 96);
+            float* parts = reinterpret_cast<float*>(static_cast<unsigned char*>(p.workspace) + kCounterBytes);
             auto part = [&](int cta, int which) { return parts + ((int64_t(cta) * 2 + which) * 2 + w) * kPart; };
             auto state = [&](int cta, int which) { return parts + (((int64_t(cta) * 2 + which) * 2 + w) * kPart + D * kM + v * 2); };
             {
@@ -926,11 +916,19 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_kernel(const AttentionPar
 
 }  // namespace
 
-size_t prefill_workspace(int, int head_dim) {
-    return kCtas * 2 * 4 + 96 + size_t(kCtas) * 4 * kM * (head_dim + 2) * 4;
+size_t prefill_workspace(int group, int head_dim) {
+    return std::max(decode_workspace(group, head_dim), kCounterBytes + size_t(kCtas) * 4 * kM * (head_dim + 2) * 4);
 }
 
 cudaError_t launch_prefill(const AttentionParams& p, int type, int format, int head_dim, cudaStream_t stream) {
+    // Few rows go one by one, as decode's do, while there is an SM for each (row, kv head, 8 query
+    // heads): their tokens are read once per row, but no tile of vectors has to be filled. 9 / 3
+    // heads, FP32, beside the tiles: 37 rows 7.4 us against 13.4 (at position 500 11.5 / 19.8);
+    // 49 rows 7.8 / 14.8, at 2000 21.7 / 30.0, at 16000 67.9 / 67.9. Twice as many would
+    // still gain a little on short contexts (98 rows 14.6 / 15.0, at 2000 27.2 / 31.6), and lose
+    // on long ones, where the time is the tokens that an SM passes over.
+    if (int64_t(p.rows) * p.cache.kv_heads * ((p.heads / p.cache.kv_heads + 7) / 8) <= kPackedItems)
+        return launch_packed(p, type, format, head_dim, stream);
     return dispatch(type, format, head_dim, [&](auto t, auto f, auto d) {
         using S = Shape<decltype(t), decltype(d)::value>;
         auto kernel = prefill_kernel<decltype(t), decltype(f)::value, decltype(d)::value>;
