@@ -258,19 +258,23 @@ int mp_paged_attention_status(void* stream);
  *   mp_kv8_attention_prefill  causal attention of packed chunks of rows.
  * A value is code * scale. Codes are INT8 (-127..127) or E4M3 (bytes of the 8-bit
  * float with 4 exponent and 3 mantissa bits, largest 448). The append chooses scales
- * that are powers of two; the attentions take any finite scale.
+ * that are powers of two; the attentions take any finite scale that is not negative.
  *
  * All arrays are device memory of the current device unless stated, and the metadata
  * (tables, lengths, row_offsets, starts) is read by the kernels only: no call copies
  * to the device, synchronises or allocates, so every call can be captured into a
- * graph and replayed with other metadata in the same buffers. Calls that share a
- * workspace must not overlap. A null or misaligned pointer, a pointer that is not
+ * graph and replayed with other metadata in the same buffers. A workspace may serve
+ * both attentions and any number of captured calls as long as no two of them run at
+ * the same time; after MP_ERR_TIMEOUT it must be zeroed again. Outputs must not overlap
+ * a call's other buffers, unless stated. A null or misaligned pointer, a pointer that is not
  * memory of the current device, and sizes outside the stated ranges are refused with
  * MP_ERR_INVALID (a geometry without a kernel with MP_ERR_UNSUPPORTED) before
  * anything is queued. What only the device can see goes to `device_error`
  * (optional, caller-owned device word, zeroed by the caller; mp_kv8_status reads
  * and clears it): bit 1 = a block id outside [0, max_blocks), metadata outside its
- * table, or a position outside the rotation tables; bit 2 = a copy wait expired;
+ * table, or a position outside the rotation tables, or more than 2^30 pieces of work for
+ * one SM (that sequence, or the call, is left out); bit 2 = a wait inside the
+ * prefill kernel expired (its outputs are incomplete);
  * bit 4 = an appended value was NaN or infinite, or the scale of a block that already
  * held tokens was no power of two. */
 #define MP_KV8_INT8 0
@@ -302,7 +306,7 @@ typedef struct {
  *
  * Every row's k is rotated by its position, and k and v go to slot position %
  * block_tokens of block tables[i][position / block_tokens]. With q, the rotated q goes
- * to q_out (which may be q itself). Rotation of a pair (a, b): (a cos - b sin, b cos
+ * to q_out (which may be q itself, with its stride). Rotation of a pair (a, b): (a cos - b sin, b cos
  * + a sin) with row `position` of cos / sin ([max_positions][rotary_dim / 2]); dims at or
  * past rotary_dim pass unrotated (rotary_dim 0: no rotation, cos and sin unused). q is
  * rotated in FP32 (a rounded product and a fused multiply-add); k codes come from the exact
@@ -331,7 +335,7 @@ typedef struct {
     int32_t rotary_dim;         /* a multiple of 8, 0 .. head_dim */
     int32_t rope_layout;        /* MP_ROPE_* */
     int32_t max_positions;
-    int32_t table_stride;
+    int32_t table_stride;       /* table_stride * block_tokens <= 2^26 */
     int32_t count; /* 1 .. 65536 */
     int32_t rows;
 } mp_kv8_append_args;
@@ -359,7 +363,9 @@ int mp_kv8_attention_decode(const mp_kv8_cache* cache, const mp_kv8_decode_args*
 
 /* Causal attention of packed chunks of rows (row_offsets, starts, rows as for the
  * append): the row at position p attends to tokens 0 .. p of its sequence, which are in
- * the pages already (the chunk's own rows among them: append first). */
+ * the pages already (the chunk's own rows among them: append first). Calls with at most
+ * 148 (row, kv head, 8 query heads) in their `rows` go row by row, others as tiles of
+ * rows on the tensor cores, with the same error bounds. */
 typedef struct {
     const void* q;
     void* out;

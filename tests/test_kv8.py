@@ -155,3 +155,8 @@ def test_reference_rounding_and_scales(fmt):
         s = ref.scale_for(amax, fmt)
         assert limit * s >= float(torch.tensor(amax, dtype=torch.float64).float())
         assert s == 2.0 ** -100 or limit * s / 2 < amax
+
+
+@pytest.mark.parametrize("op", list(CALLS))
+def test_tables_beyond_the_index_range_are_refused(built, op):
+    refused(op, mp.MP_ERR_INVALID, table_stride=(1 << 26) // 16 + 1)

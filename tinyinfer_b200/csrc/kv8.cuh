@@ -14,6 +14,9 @@ namespace kv8 {
 constexpr int kCtas = 148;            // one per SM
 constexpr int kPackedItems = kCtas;   // items up to which a prefill goes row by row (kv8_prefill.cu)
 constexpr int kCounterBytes = kCtas * 2 * 4 + 96;  // of the attentions' workspaces: zero between calls; partials follow
+// Limits that keep a plan's 32-bit indexes in range: tokens of a table (checked by the host), and
+// units of a CTA's run (checked by the device: minutes of work).
+constexpr int64_t kMostTokens = int64_t(1) << 26, kMostUnits = int64_t(1) << 30;
 constexpr unsigned kErrValue = 4u;  // error word bit: a value (or a held block's scale) that cannot be quantised
 
 struct Cache {
@@ -177,13 +180,6 @@ __device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], 
     asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
         : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-}
-
-// Transpose of an 8 x 8 matrix of 16-bit elements over the warp.
-__device__ __forceinline__ uint32_t transpose8x8(uint32_t a) {
-    uint32_t d;
-    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(a));
-    return d;
 }
 
 // Four 8 x 8 matrices of 16-bit elements from shared memory, transposed: lane l gives

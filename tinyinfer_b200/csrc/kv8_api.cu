@@ -36,6 +36,8 @@ int check_rows(const mp_kv8_cache* c, int type, int heads, int count, int table_
         return refuse(MP_ERR_INVALID, "kv8: heads is not 1 to 64 times kv_heads, or above 1024");
     if (count < 1 || count > 65536 || table_stride < 1)
         return refuse(MP_ERR_INVALID, "kv8: count or table_stride out of range");
+    if (int64_t(table_stride) * c->block_tokens > kv8::kMostTokens)
+        return refuse(MP_ERR_INVALID, "kv8: a table of more than 2^26 tokens");
     return MP_OK;
 }
 
@@ -201,7 +203,7 @@ extern "C" int mp_kv8_status(uint32_t* device_error, void* stream_ptr) {
     if (e == cudaSuccess) e = cudaStreamSynchronize(stream);
     if (e == cudaSuccess && bits) e = cudaMemsetAsync(device_error, 0, sizeof(bits), stream);
     if (e != cudaSuccess) return finish(e);
-    if (bits & kErrTimeout) return refuse(MP_ERR_TIMEOUT, "kv8: a copy wait expired");
+    if (bits & kErrTimeout) return refuse(MP_ERR_TIMEOUT, "kv8: a wait expired");
     if (bits & kErrBounds) return refuse(MP_ERR_BOUNDS, "kv8: block id, metadata or position out of range");
     if (bits & kv8::kErrValue) return refuse(MP_ERR_NONFINITE, "kv8: value or block scale that cannot be quantised");
     return MP_OK;

@@ -1,15 +1,22 @@
 // mp_kv8_attention_decode: one query row per sequence over the 8-bit paged cache (sm_100a);
 // and the rows of small mp_kv8_attention_prefill calls (kPacked).
 //
-// Bound by HBM: a token costs 2 head_dim bytes per kv head and 4 head_dim flops per query
-// head. The work is cut into units of 32 tokens of one (row, kv head, up to 8 query heads)
-// item; all items' units, in order, are dealt out in equal runs to the warps of one CTA
-// per SM, however long the sequences are. The lengths are device memory, so every CTA adds
-// them up itself (a block scan) and finds where its warps' runs begin.
+// A token costs 2 head_dim bytes per kv head and 4 head_dim flops per query head. The work
+// is cut into units of 32 tokens of one (row, kv head, up to 8 query heads) item; all items'
+// units, in order, are dealt out in equal runs to one CTA per SM and its warps, however
+// long the sequences are, or a CTA takes an item whole. The lengths are device memory,
+// so every CTA adds them up itself (a block scan) and finds where its warps' runs begin.
 //
-// A warp is a pipeline of its own: a ring of units in shared memory that tensor copies fill
-// (K and V tiles of a page are one piece, so a 16-token page is one box; its rows are swizzled against bank conflicts) and the warp-level tensor ops of kv8_warp.cuh empty. 16 warps keep up to 192 KB in flight per SM, and no two
-// warps wait for one another before the end.
+// A warp is a pipeline of its own: a ring of units in shared memory that cp.async fills
+// (rows swizzled against bank conflicts) and the warp-level tensor ops of kv8_warp.cuh
+// empty. 16 warps keep up to 192 KB in flight per SM, and no two warps wait for one another
+// before the end. (The copy engine's tiles, issued by a lane, cost the warp more instructions
+// than 16-byte copies by all lanes: 74 us against 52 for 256 rows of 2048 tokens.)
+//
+// Bound by instructions: about 480 a unit on a scheduler with 4 warps (2 or 3 for head_dim 128),
+// where the ring without arithmetic takes 40 us for 256 x 2048 tokens of 9 / 3 heads x 64; with it
+// 53 us in FP32 (3.8 TB/s), 48 in BF16. Wider heads come nearer to HBM: 64 x 4096 tokens of
+// 32 / 8 heads x 128 100 us (5.4 TB/s).
 //
 // An item that ends in a later run leaves partials (max, sum, outputs): a CTA's warps join theirs
 // through shared memory, CTAs through the workspace: the last CTA to arrive on the counter of
@@ -21,8 +28,14 @@ namespace kv8 {
 namespace {
 
 constexpr int kSmemBytes = 227 * 1024;
-constexpr int kMinUnits = 2;  // units per warp before another CTA takes part: joining CTAs costs about as much
-constexpr int kWholeUnits = 2;  // units per warp up to which a CTA takes an item whole, if there are CTAs for all
+// Units per warp before another CTA takes part (1 is no faster; with 4, one row of 32768 tokens took
+// 20.7 us instead of 17.9).
+constexpr int kMinUnits = 2;
+// Units per warp that a CTA may take beyond its equal share to have an item whole, if there is a CTA for
+// each: no CTA then waits for another. Against runs: one row of 333 tokens 8.9 us (12.2), 3 x 1000 11.8
+// (12.8), 49 x 2000 16.6 (21.7), 64 x 4096 of 16 / 2 heads x 128 40.0 (43.8). With 2, 24 x 3000 takes
+// 20.8 us, 19.6 with 4; with 6, 16 rows at position 4000 take 22.4, 20.1 with 4.
+constexpr int kWholeUnits = 4;
 
 template <class T, int D>
 __host__ __device__ constexpr int warps_of() {
@@ -173,8 +186,7 @@ __global__ void __launch_bounds__(warps_of<T, D>() * 32, 1)
         return 0;
     };
     auto units_of = [&](int row) { return row < p.count ? int((unsigned(tokens(row)) + kUnit - 1) / kUnit) : 0; };
-    // A CTA per item where that is few units for every warp (no CTA waits for another, and
-    // there is nothing to search); else equal runs.
+    // A CTA per item, or equal runs
     int64_t mine = 0;
     int most = 0;
     for (int i = 0; i < share; ++i) {
@@ -191,7 +203,11 @@ __global__ void __launch_bounds__(warps_of<T, D>() * 32, 1)
     if (lane == 31) sums[warp] = upto, longest_of[warp] = most;
     __syncthreads();
     most = __reduce_max_sync(0xffffffffu, lane < kWarps ? longest_of[lane] : 0);
-    const bool whole = int64_t(p.count) * per <= int64_t(gridDim.x) && most <= kWholeUnits * kWarps;
+    bool whole = int64_t(p.count) * per <= int64_t(gridDim.x);
+    if (whole) {  // few rows: 32 bits hold their units
+        const int all = int(__reduce_add_sync(0xffffffffu, lane < kWarps ? unsigned(sums[lane]) : 0u)) * per;
+        whole = most <= all / int(gridDim.x) + kWholeUnits * kWarps;
+    }
     int row = 0, item = 0, unit = 0;
     int ctas, cta_units = 0, extra = 0;
     int64_t cta_begin = 0, base = 0;  // CTA c's run: `base` units, one more for the first `extra` CTAs
@@ -214,6 +230,10 @@ __global__ void __launch_bounds__(warps_of<T, D>() * 32, 1)
         const int parts = max(ctas, 1);
         base = total >> 32 ? total / parts : int64_t(uint32_t(total) / uint32_t(parts));
         extra = int(total - base * parts);
+        if (base >= kMostUnits) {
+            raise_error(p.error, kErrBounds);
+            return;
+        }
         cta_begin = blockIdx.x * base + min(int(blockIdx.x), extra);
         if (int(blockIdx.x) < ctas) cta_units = int(base) + (int(blockIdx.x) < extra);
     }

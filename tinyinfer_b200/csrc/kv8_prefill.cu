@@ -356,7 +356,8 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_kernel(const AttentionPar
         return int(unit < split ? unit / (base + 1) : extra + (unit - split) / base);
     };
     Cursor cursor{&p, block_rows, 0, 0, 0, 0, 0, 0};
-    cursor.left = int(blockIdx.x) < ctas ? int(base) + (int(blockIdx.x) < extra) : 0;
+    if (base >= kMostUnits) raise_error(p.error, kErrBounds);
+    cursor.left = int(blockIdx.x) < ctas && base < kMostUnits ? int(base) + (int(blockIdx.x) < extra) : 0;
     if (cursor.left) {
         cursor.at = blockIdx.x * base + min(int(blockIdx.x), extra);
         int t = 0;
@@ -924,7 +925,7 @@ cudaError_t launch_prefill(const AttentionParams& p, int type, int format, int h
     // Few rows go one by one, as decode's do, while there is an SM for each (row, kv head, 8 query
     // heads): their tokens are read once per row, but no tile of vectors has to be filled. 9 / 3
     // heads, FP32, beside the tiles: 37 rows 7.4 us against 13.4 (at position 500 11.5 / 19.8);
-    // 49 rows 7.8 / 14.8, at 2000 21.7 / 30.0, at 16000 67.9 / 67.9. Twice as many would
+    // 49 rows 8.0 / 14.8, at 2000 17.0 / 30.0, at 16000 62.7 / 67.9. Twice as many would
     // still gain a little on short contexts (98 rows 14.6 / 15.0, at 2000 27.2 / 31.6), and lose
     // on long ones, where the time is the tokens that an SM passes over.
     if (int64_t(p.rows) * p.cache.kv_heads * ((p.heads / p.cache.kv_heads + 7) / 8) <= kPackedItems)
