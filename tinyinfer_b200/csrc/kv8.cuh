@@ -87,14 +87,16 @@ __device__ __forceinline__ int64_t tile_offset(const Cache& c, int block, int he
 
 // Block id of `page` in a table row; an id or page out of range sets the bounds bit
 // and gives block 0, so that no access leaves the cache.
-__device__ __forceinline__ int block_id(const Cache& c, const int32_t* table, int table_stride, int page,
-                                        unsigned* error) {
-    const int b = page < table_stride ? table[page] : -1;
+__device__ __forceinline__ int checked_id(const Cache& c, int b, unsigned* error) {
     if (unsigned(b) >= unsigned(c.max_blocks)) {
         raise_error(error, kErrBounds);
         return 0;
     }
     return b;
+}
+__device__ __forceinline__ int block_id(const Cache& c, const int32_t* table, int table_stride, int page,
+                                        unsigned* error) {
+    return checked_id(c, page < table_stride ? table[page] : -1, error);
 }
 
 // Rows of a prefill's sequence i, 0 for one whose metadata is out of range.

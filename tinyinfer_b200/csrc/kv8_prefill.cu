@@ -10,7 +10,9 @@
 //
 // Roles of a CTA (three more warps idle):
 //  * warps 8-11 widen K and V codes to FP16 tiles in shared memory (exact; K token-major,
-//    V token-major too: the tensor core reads it transposed), with their blocks' scales;
+//    V token-major too: the tensor core reads it transposed), with their blocks' scales. The codes
+//    come by cp.async: loaded into registers a tile ahead, they waited for one another in the
+//    little L1 that the tiles leave (8 x 1024 rows of 32 / 8 heads x 128 BF16: 452 us, now 383);
 //  * one lane of warp 12 issues the products: S = Q K^T into tensor memory, O = P V with
 //    P from tensor memory;
 //  * warps 0-3 and 4-7 own one tile each, a thread per vector: running softmax of S's
@@ -66,17 +68,18 @@ struct Shape {
     static constexpr int kQ = 0;                                        // [2 tiles][halves]
     static constexpr int kK = kQ + 2 * kHalves * kTileBytes;
     static constexpr int kV = kK + kStages * kTileBytes;
-    static constexpr int kScales = kV + kStages * kTileBytes;           // [slots][groups] K, V, log2 V, 1 / V
+    static constexpr int kRing = D == 64 ? 3 : 1;                       // tiles of codes in flight, as they are
+    static constexpr int kRaw = kV + kStages * kTileBytes;              // [ring][K, V][words of a thread][128 threads]
+    static constexpr int kRawScales = kRaw + kRing * 2 * kN * D;        // [ring][groups] K, V
+    static constexpr int kScales = kRawScales + kRing * kGroups * 8;    // [slots][groups] K, V, log2 V, 1 / V
     static constexpr int kBars = kScales + kScaleSlots * kGroups * 16;
-    static constexpr int kPlan = kBars + 32 * 8;
-    static constexpr int kSmem = kPlan + (kThreads + 1) * 12 + 2 * 32 * 8;
+    static constexpr int kPlan = kQ;                                    // before the queries come
+    static constexpr int kSmem = kBars + 32 * 8;
     static constexpr int kAlloc = kSmem + 1024;                         // alignment slack
     static constexpr int kBuffers = D == 64 ? 3 : 2;                    // places of S
     // registers a thread of each role: together those of the launch, 512 x 128
-    static constexpr int kSoftmaxRegs = kHalves == 2 && D == 128 ? 184 : 168;
-    static constexpr int kWidenRegs = D == 64 ? 96 : kHalves == 1 ? 104 : 80;
+    static constexpr int kSoftmaxRegs = 184, kWidenRegs = 72;
     static constexpr int kProductRegs = 512 - 2 * kSoftmaxRegs - kWidenRegs;
-    static constexpr int kAhead = kHalves == 2 && D == 128 ? 1 : 2;     // K and V codes loaded ahead, or one of them
     static constexpr uint32_t kTmemCols = 512;                          // S: kBuffers x 128, O: 2 x D
 };
 static_assert(Shape<float, 128>::kAlloc <= 232448 && Shape<__nv_bfloat16, 128>::kAlloc <= 232448);
@@ -194,6 +197,15 @@ __device__ __forceinline__ void set_registers() {
 
 __device__ __forceinline__ void copy_row16(uint32_t to, const void* from, bool live) {  // zeros where not live
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(live ? 16 : 0) : "memory");
+}
+
+__device__ __forceinline__ void copy_scales(uint32_t to, const float* from, bool live) {  // zeros where not live
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;" ::"r"(to), "l"(from), "r"(live ? 8 : 0) : "memory");
+}
+// All but the youngest N groups of this thread's copies are done.
+template <int N>
+__device__ __forceinline__ void wait_copies() {
+    asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
 
 // The values of a 16-byte word.
@@ -737,6 +749,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_kernel(const AttentionPar
         constexpr int kChunks = D / 16;            // words of a token
         const int first_token = t / kChunks, chunk = t % kChunks, in_page = bt / kGroupTokens;
         const int own = first_token % kGroupTokens * D + chunk * 16;
+        const uint32_t raw = smem_u32(sm + S::kRaw) + t * 16, raw_scales = smem_u32(sm + S::kRawScales);
         // the word's 16 FP16 values in a tile: two 16-byte chunks of the token's row
         const int to0 = (chunk / 4) * (kN * 128) + int(sw128_offset(first_token, 2 * (chunk % 4)));
         const int to1 = (chunk / 4) * (kN * 128) + int(sw128_offset(first_token, 2 * (chunk % 4) + 1));
@@ -746,56 +759,62 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_kernel(const AttentionPar
         while (ok && cursor.next(seg)) {
             const int32_t* table = p.tables + int64_t(seg.seq) * p.table_stride;
             const int len = seg.position + seg.rows;
-            // Lane g < 8 finds the block of tile k's 16 tokens from 16 g on: the offset of their K
-            // rows (V's are one block of rows on) and their scales. Codes and scales are loaded a tile
-            // ahead, offsets two (kAhead 1: K codes while V's are stored, and V's while K's are).
+            // Codes and scales are copied kRing tiles ahead; a thread copies what it widens itself. The
+            // blocks of four tiles at a time are found by the lanes, 8 pieces of 16 tokens each: their
+            // K rows' offsets (V's are one block of rows on); table entries are read four tiles earlier.
+            const int first = slot - seg.k0;
             int64_t offset = 0;
-            float2 scale, next_scale;
-            uint4 code[S::kAhead][kWords];
-            auto find = [&](int k) {
-                const int tile = k * kGroups + lane;
-                next_scale = make_float2(0.f, 0.f);
-                if (lane < kGroups && k < seg.k1 && tile * kGroupTokens < len) {
-                    const int block = block_id(p.cache, table, p.table_stride, tile / in_page, p.error);
-                    offset = tile_offset(p.cache, block, seg.head, 0, D) + tile % in_page * (kGroupTokens * D);
-                    if (warp == kWidenWarp)
-                        next_scale = *reinterpret_cast<const float2*>(p.cache.scales + block * p.cache.scale_stride + 2 * seg.head);
-                }
+            int block = 0, entry, rest;
+            auto peek = [&](int k) {
+                const int piece = k * kGroups + lane, page = piece / in_page;
+                entry = 0, rest = piece - page * in_page;
+                if (piece < seg.k1 * kGroups && piece * kGroupTokens < len) entry = page < p.table_stride ? table[page] : -1;
             };
-            auto load = [&](int k, int part) {
-                const int left = k < seg.k1 ? len - k * kN : 0;  // tokens of the tile
+            auto copy = [&](int k, int part) {
+                if (k < seg.k1) {
+                    const int place = (first + k) % S::kRing, in = (k - seg.k0) % 4 * kGroups, left = len - k * kN;
+                    if (part == 0) {
+                        if (in == 0) {
+                            block = checked_id(p.cache, entry, p.error);
+                            offset = tile_offset(p.cache, block, seg.head, 0, D) + rest * (kGroupTokens * D);
+                            peek(k + 4);
+                        }
+                        const int from = __shfl_sync(0xffffffffu, block, in + lane % kGroups);
+                        if (t < kGroups)
+                            copy_scales(raw_scales + (place * kGroups + t) * 8, p.cache.scales + from * p.cache.scale_stride + 2 * seg.head,
+                                        t * kGroupTokens < left);
+                    }
 #pragma unroll
-                for (int i = 0; i < kWords; ++i) {
-                    const int group_of = first_token / kGroupTokens + i * (kN / kWords) / kGroupTokens;
-                    const int64_t at = __shfl_sync(0xffffffffu, offset, group_of);
-                    code[part % S::kAhead][i] = make_uint4(0, 0, 0, 0);
-                    if (first_token + i * (kN / kWords) < left)
-                        code[part % S::kAhead][i] = __ldg(reinterpret_cast<const uint4*>(p.cache.pages + at + part * bt * D + own));
+                    for (int i = 0; i < kWords; ++i) {
+                        const int64_t at = __shfl_sync(0xffffffffu, offset, in + first_token / kGroupTokens + i * (kN / kWords) / kGroupTokens);
+                        const bool live = first_token + i * (kN / kWords) < left;
+                        copy_row16(raw + ((place * 2 + part) * kWords + i) * 2048, p.cache.pages + (live ? at + part * bt * D + own : 0), live);
+                    }
                 }
+                asm volatile("cp.async.commit_group;" ::: "memory");  // one per tile and part, empty ones included
             };
-            find(seg.k0);
-            load(seg.k0, 0);
-            if constexpr (S::kAhead == 2) {
-                load(seg.k0, 1);
-                scale = next_scale;
-                find(seg.k0 + 1);
-            }
+            peek(seg.k0);
+            for (int k = seg.k0; k < seg.k0 + S::kRing; ++k) copy(k, 0), copy(k, 1);
             for (int k = seg.k0; ok && k < seg.k1; ++k, ++slot) {
                 const int stage = slot % kStages;
                 const uint32_t parity = ((slot / kStages) & 1) ^ 1;
-                if constexpr (S::kAhead == 1) scale = next_scale;
-                if (t < kGroups)
+                const int place = slot % S::kRing;
+                wait_copies<2 * S::kRing - 1>();
+                if (t < kGroups) {
+                    const float2 scale = *reinterpret_cast<const float2*>(sm + S::kRawScales + (place * kGroups + t) * 8);
                     scales[slot % kScaleSlots * kGroups + t] =
                         make_float4(scale.x, scale.y, __log2f(scale.y), scale.y == 0.f ? 0.f : 1.f / scale.y);
+                }
                 __syncwarp();
                 if (t == 0) mbar_arrive(scales_full + slot % kScaleSlots);
 #pragma unroll
                 for (int part = 0; part < 2; ++part) {
                     if (!(ok = wait((part ? v_empty : k_empty) + stage, parity))) break;
+                    if (part) wait_copies<2 * S::kRing - 1>();
                     unsigned char* tile = sm + (part ? S::kV : S::kK) + stage * S::kTileBytes;
 #pragma unroll
                     for (int i = 0; i < kWords; ++i) {
-                        const uint4 c = code[part % S::kAhead][i];
+                        const uint4 c = *reinterpret_cast<const uint4*>(sm + S::kRaw + ((place * 2 + part) * kWords + i) * 2048 + t * 16);
                         uint32_t h[8];
                         widen4<F>(c.x, h[0], h[1]);
                         widen4<F>(c.y, h[2], h[3]);
@@ -808,21 +827,11 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_kernel(const AttentionPar
                     fence_proxy_async_shared();
                     __syncwarp();
                     if (lane == 0) mbar_arrive((part ? v_full : k_full) + stage);
-                    if constexpr (S::kAhead == 2) {
-                        load(k + 1, part);
-                    } else if (part == 0) {
-                        load(k, 1);
-                    } else {
-                        find(k + 1);
-                        load(k + 1, 0);
-                    }
-                }
-                if constexpr (S::kAhead == 2) {
-                    scale = next_scale;
-                    find(k + 2);
+                    copy(k + S::kRing, part);
                 }
             }
         }
+        asm volatile("cp.async.wait_all;" ::: "memory");
     } else {
         // ================================================================ products
         set_registers<S::kProductRegs>();
