@@ -129,6 +129,25 @@ __device__ __forceinline__ void tmem_load(uint32_t taddr, float (&r)[32]) {
           "=f"(r[24]), "=f"(r[25]), "=f"(r[26]), "=f"(r[27]), "=f"(r[28]), "=f"(r[29]), "=f"(r[30]), "=f"(r[31])
         : "r"(taddr));
 }
+__device__ __forceinline__ void tmem_load(uint32_t taddr, float (&r)[64]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x64.b32 {"
+        "%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15,"
+        "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31,"
+        "%32, %33, %34, %35, %36, %37, %38, %39, %40, %41, %42, %43, %44, %45, %46, %47,"
+        "%48, %49, %50, %51, %52, %53, %54, %55, %56, %57, %58, %59, %60, %61, %62, %63"
+        "}, [%64];\n\t"
+        "tcgen05.wait::ld.sync.aligned;"
+        : "=f"(r[0]), "=f"(r[1]), "=f"(r[2]), "=f"(r[3]), "=f"(r[4]), "=f"(r[5]), "=f"(r[6]), "=f"(r[7]),
+          "=f"(r[8]), "=f"(r[9]), "=f"(r[10]), "=f"(r[11]), "=f"(r[12]), "=f"(r[13]), "=f"(r[14]), "=f"(r[15]),
+          "=f"(r[16]), "=f"(r[17]), "=f"(r[18]), "=f"(r[19]), "=f"(r[20]), "=f"(r[21]), "=f"(r[22]), "=f"(r[23]),
+          "=f"(r[24]), "=f"(r[25]), "=f"(r[26]), "=f"(r[27]), "=f"(r[28]), "=f"(r[29]), "=f"(r[30]), "=f"(r[31]),
+          "=f"(r[32]), "=f"(r[33]), "=f"(r[34]), "=f"(r[35]), "=f"(r[36]), "=f"(r[37]), "=f"(r[38]), "=f"(r[39]),
+          "=f"(r[40]), "=f"(r[41]), "=f"(r[42]), "=f"(r[43]), "=f"(r[44]), "=f"(r[45]), "=f"(r[46]), "=f"(r[47]),
+          "=f"(r[48]), "=f"(r[49]), "=f"(r[50]), "=f"(r[51]), "=f"(r[52]), "=f"(r[53]), "=f"(r[54]), "=f"(r[55]),
+          "=f"(r[56]), "=f"(r[57]), "=f"(r[58]), "=f"(r[59]), "=f"(r[60]), "=f"(r[61]), "=f"(r[62]), "=f"(r[63])
+        : "r"(taddr));
+}
 // One lane of the (converged) warp.
 __device__ __forceinline__ bool elect() {
     uint32_t one;
@@ -550,7 +569,9 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_kernel(const AttentionPar
                 // the tile's weights; kCut: some row of the warp does not see all of its tokens
                 auto weigh = [&](auto is_cut) {
                     constexpr bool kCut = decltype(is_cut)::value;
-                    using Some = std::integral_constant<int, kCut || (S::kAdd && D == 128) ? 1 : 2>;
+                    // (64 scores at once: BF16, head_dim 64, 16 x 512 rows at position 3584 take 185 us, 198 with
+                    // 32; in the other shapes too few registers are left: FP32 259 and 249, head_dim 128 405 and 383)
+                    using Some = std::integral_constant<int, kCut || (S::kAdd && D == 128) ? 1 : !S::kAdd && D == 64 ? 4 : 2>;
                     auto largest_of = [&](float (&x)[16], int g) {  // scaled
                         if constexpr (kCut) {
 #pragma unroll
