@@ -250,6 +250,7 @@ struct Cursor {
     int seq, block, head, k;  // k: unit of the item, kSetup + tile
     int64_t at;               // device-wide index of the next unit
     int left;
+    int begin, start, rows;   // of sequence `seq`
 
     static __device__ __forceinline__ int units_of(int start, int rows, int block, int block_rows) {
         return kSetup + (start + min((block + 1) * block_rows, rows) + kN - 1) / kN;
@@ -263,7 +264,6 @@ struct Cursor {
     }
     __device__ __forceinline__ bool advance(Segment& s) {
         if (left <= 0) return false;
-        int begin, start, rows = sequence_rows(*p, seq, begin, start);
         while (block * block_rows >= rows) {
             block = 0, head = 0, k = 0;
             rows = sequence_rows(*p, ++seq, begin, start);
@@ -386,7 +386,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_kernel(const AttentionPar
         const int64_t split = extra * (base + 1);
         return int(unit < split ? unit / (base + 1) : extra + (unit - split) / base);
     };
-    Cursor cursor{&p, block_rows, 0, 0, 0, 0, 0, 0};
+    Cursor cursor{&p, block_rows};
     if (base >= kMostUnits) raise_error(p.error, kErrBounds);
     cursor.left = int(blockIdx.x) < ctas && base < kMostUnits ? int(base) + (int(blockIdx.x) < extra) : 0;
     if (cursor.left) {
@@ -397,9 +397,11 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_kernel(const AttentionPar
             if (units_before[t + o] * heads <= cursor.at) t += o;
         locate(t * each, cursor.seq, cursor.block);
         int64_t in = cursor.at - units_before[t] * heads;
-        for (int rows = sequence_rows(p, cursor.seq, begin, start);; ++cursor.block) {
-            while (cursor.block * block_rows >= rows) cursor.block = 0, rows = sequence_rows(p, ++cursor.seq, begin, start);
-            const int n = Cursor::units_of(start, rows, cursor.block, block_rows);
+        cursor.rows = sequence_rows(p, cursor.seq, cursor.begin, cursor.start);
+        for (;; ++cursor.block) {
+            while (cursor.block * block_rows >= cursor.rows)
+                cursor.block = 0, cursor.rows = sequence_rows(p, ++cursor.seq, cursor.begin, cursor.start);
+            const int n = Cursor::units_of(cursor.start, cursor.rows, cursor.block, block_rows);
             if (in < int64_t(n) * heads) {
                 cursor.head = int(in) / n, cursor.k = int(in) % n;
                 break;
