@@ -320,7 +320,7 @@ typedef struct {
  * is then off by at most half its block's scale when appended, and by less than one
  * scale after any number of re-roundings (each scale is at least twice the one
  * before). NaN is stored as 0 and infinity as the largest code, with the error bit.
- * A block takes new rows from one sequence per call; slots past a sequence's last
+ * A block takes new rows from one place of one table per call; slots past a sequence's last
  * token keep their bytes. */
 typedef struct {
     const void *q, *k, *v; /* q optional */

@@ -641,3 +641,60 @@ def test_decode_and_prefill_share_a_workspace(built):
         for i, n in enumerate((1500, 900)):
             check_rows(cache, 9, q[i * rows: (i + 1) * rows], out[i * rows: (i + 1) * rows], tables[i].tolist(), n, 0.125, False)
             check_rows(cache, 9, last[i: i + 1], one[i: i + 1], tables[i].tolist(), n, 0.125, False)
+
+
+@pytest.mark.parametrize("scale", [0.0, -0.125])
+@pytest.mark.parametrize("rows,dtype", [(4, "f32"), (90, "f32"), (90, "bf16")])
+def test_any_factor_of_the_scores(built, rows, dtype, scale):
+    """A factor of 0 weighs all tokens alike, a negative one turns the order round; in every kernel."""
+    lengths = [333, rows]
+    cache = Cache(40, 3, 64, 16, "int8")
+    tables = tables_for(lengths, 16, 40, 67)
+    fill(cache, tables, lengths, 68)
+    q, out = decode(cache, 9, tables, lengths, dtype, scale=scale)
+    for i, n in enumerate(lengths):
+        check_rows(cache, 9, q[i: i + 1], out[i: i + 1], tables[i].tolist(), n, scale, dtype == "bf16")
+    q, out = values(2 * rows, 576, 69).to(DTYPES[dtype]), torch.zeros(2 * rows, 576, dtype=DTYPES[dtype], device=DEV)
+    workspace = torch.zeros(mp.kv8_prefill_workspace(cache.c, 9), dtype=torch.uint8, device=DEV)
+    offsets = torch.tensor([0, rows, 2 * rows], dtype=torch.int32, device=DEV)
+    starts = torch.tensor([333 - rows, 0], dtype=torch.int32, device=DEV)
+    mp.kv8_attention_prefill(cache.c, mp.Kv8PrefillArgs(
+        q=q.data_ptr(), out=out.data_ptr(), q_stride=576, out_stride=576, tables=tables.data_ptr(),
+        row_offsets=offsets.data_ptr(), starts=starts.data_ptr(), workspace=workspace.data_ptr(),
+        workspace_bytes=workspace.numel(), type=list(DTYPES).index(dtype), heads=9, table_stride=tables.stride(0),
+        count=2, rows=2 * rows, scale=scale), None, stream())
+    for i, n in enumerate(lengths):
+        part = slice(i * rows, (i + 1) * rows)
+        check_rows(cache, 9, q[part], out[part], tables[i].tolist(), n, scale, dtype == "bf16")
+
+
+def test_prefill_graph_replays_with_other_chunks(built):
+    """A captured call follows its metadata buffers: other chunks, other positions, sequences without rows."""
+    cache = Cache(300, 3, 64, 16, "e4m3")
+    tables = tables_for([1200, 1200, 1200], 16, 300, 70)
+    fill(cache, tables, [1200] * 3, 71)
+    rows = 600
+    q, out = values(rows, 576, 72), torch.zeros(rows, 576, device=DEV)
+    workspace = torch.zeros(mp.kv8_prefill_workspace(cache.c, 9), dtype=torch.uint8, device=DEV)
+    offsets, starts = torch.zeros(4, dtype=torch.int32, device=DEV), torch.zeros(3, dtype=torch.int32, device=DEV)
+    word = torch.zeros(1, dtype=torch.int32, device=DEV)
+    args = mp.Kv8PrefillArgs(q=q.data_ptr(), out=out.data_ptr(), q_stride=576, out_stride=576, tables=tables.data_ptr(),
+                             row_offsets=offsets.data_ptr(), starts=starts.data_ptr(), workspace=workspace.data_ptr(),
+                             workspace_bytes=workspace.numel(), type=0, heads=9, table_stride=tables.stride(0), count=3,
+                             rows=rows, scale=0.125)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        mp.kv8_attention_prefill(cache.c, args, word.data_ptr(), stream())
+    for counts, first in (([100, 0, 500], [1100, 7, 0]), ([0, 0, 0], [0, 0, 0]), ([1, 1, 1], [0, 1199, 600]),
+                          ([0, 600, 0], [0, 600, 0])):
+        offsets.copy_(torch.tensor([sum(counts[:i]) for i in range(4)], dtype=torch.int32))
+        starts.copy_(torch.tensor(first, dtype=torch.int32))
+        out.fill_(7.0)
+        graph.replay()
+        assert mp.kv8_status(word.data_ptr(), stream()) == mp.MP_OK
+        at = 0
+        for i, (c, s) in enumerate(zip(counts, first)):
+            if c:
+                check_rows(cache, 9, q[at: at + c], out[at: at + c], tables[i].tolist(), s + c, 0.125, False)
+            at += c
+        assert bool((out[at:] == 7).all())

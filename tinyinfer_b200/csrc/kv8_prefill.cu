@@ -8,6 +8,8 @@
 // outputs), so a long context with few rows is shared like many short ones; the device plans
 // this itself from row_offsets and starts.
 //
+// Calls with few rows go to kv8_decode.cu's kernel (launch_prefill below).
+//
 // Roles of a CTA (three more warps idle):
 //  * warps 8-11 widen K and V codes to FP16 tiles in shared memory (exact; K token-major,
 //    V token-major too: the tensor core reads it transposed), with their blocks' scales. The codes
@@ -32,8 +34,13 @@
 // every 128 tokens and is added up in FP32 registers, and the small halves' products go
 // first.
 //
-// Bound by the tensor core, exp2 and the softmax's other instructions alike: per 256
-// vectors x 128 tokens of FP32 at head_dim 64 each takes about 2050 cycles.
+// Bound by the softmax's chain of instructions: of the 6100 cycles that 256 vectors x 128 tokens
+// take in FP32 at head_dim 64 (16 x 512 rows of 9 / 3 heads at position 3584: 245 us), a thread
+// spends 900 on the maximum, 2900 on the weights, 640 on O and 700 waiting; an item's start and
+// end cost 700 more per tile. exp2 alone would take 2050, the products 2050 (3100 measured: P V is
+// 64 wide). At head_dim 128 BF16 (8 x 1024 rows of 32 / 8 heads at position 1000: 382 us, 460
+// TFLOP/s) it is 8000 cycles: 3600 of softmax, 2800 of waiting for S, whose place is free only after
+// the tile's own P V, 1500 of items' starts and ends.
 #include <algorithm>
 
 #include "kv8.cuh"
