@@ -4,8 +4,7 @@
 // A work item is (block of rows of one sequence, kv head): rows x query heads of the group
 // fill two 128-vector tiles (vector v of a tile: row v / group, head v % group), and its
 // context is a run of 128-token K/V tiles. All items' tiles, in order, are dealt out in
-// equal runs to one CTA per SM (an item counts kSetup tiles more, for its queries and
-// outputs), so a long context with few rows is shared like many short ones; the device plans
+// runs of equal cost to one CTA per SM (an item's queries and outputs count too), so a long context with few rows is shared like many short ones; the device plans
 // this itself from row_offsets and starts.
 //
 // Calls with few rows go to kv8_decode.cu's kernel (launch_prefill below).
@@ -35,10 +34,10 @@
 // first.
 //
 // Bound by the softmax's chain of instructions: of the 6100 cycles that 256 vectors x 128 tokens
-// take in FP32 at head_dim 64 (16 x 512 rows of 9 / 3 heads at position 3584: 245 us), a thread
+// take in FP32 at head_dim 64 (16 x 512 rows of 9 / 3 heads at position 3584: 243 us), a thread
 // spends 900 on the maximum, 2900 on the weights, 640 on O and 700 waiting; an item's start and
 // end cost 700 more per tile. exp2 alone would take 2050, the products 2050 (3100 measured: P V is
-// 64 wide). At head_dim 128 BF16 (8 x 1024 rows of 32 / 8 heads at position 1000: 382 us, 460
+// 64 wide). At head_dim 128 BF16 (8 x 1024 rows of 32 / 8 heads at position 1000: 377 us, 538
 // TFLOP/s) it is 8000 cycles: 3600 of softmax, 2800 of waiting for S, whose place is free only after
 // the tile's own P V, 1500 of items' starts and ends.
 #include <algorithm>
@@ -56,7 +55,10 @@ constexpr int kN = 128;       // tokens of a K/V tile
 // Scale rows in flight. Row j + 4 is written after P V of tile j + 1 completed (its V slot
 // was needed for tile j + 3), so every thread has read row j by then.
 constexpr int kScaleSlots = 4;
-constexpr int kSetup = 2;     // an item's start and end cost about this many tiles
+// Costs that runs are dealt out by: a K/V tile for both tiles of vectors, an item's start and end (8 and
+// 12 within 1 % of 10), and kAloneCost, a K/V tile for one tile of vectors: items of one take 0.73 to
+// 0.75 of the time of two at head_dim 128, 0.81 (FP32) and 0.93 (BF16) at 64.
+constexpr int kPairCost = 4, kSetup = 10;
 constexpr int kGroupTokens = 16;  // tokens that share a block's scales at least
 constexpr int kGroups = kN / kGroupTokens;
 // A weight times V scale of `unit` is 2^8 in FP16, and may grow to 2^15 before the reference
@@ -87,6 +89,7 @@ struct Shape {
     // registers a thread of each role: together those of the launch, 512 x 128
     static constexpr int kSoftmaxRegs = 184, kWidenRegs = 72;
     static constexpr int kProductRegs = 512 - 2 * kSoftmaxRegs - kWidenRegs;
+    static constexpr int kAloneCost = D == 128 ? 3 : 4;
     static constexpr uint32_t kTmemCols = 512;                          // S: kBuffers x 128, O: 2 x D
 };
 static_assert(Shape<float, 128>::kAlloc <= 232448 && Shape<__nv_bfloat16, 128>::kAlloc <= 232448);
@@ -246,27 +249,34 @@ __device__ __forceinline__ void widen_word(uint4 w, float (&x)[8]) {
 
 // One item's tiles k0 .. k1 - 1 (of `tiles`), and what it covers.
 struct Segment {
-    int seq, row0, rows, position, head, k0, k1, tiles;
-    int64_t first;  // device-wide index of the item's first unit (its tiles follow kSetup units)
+    int seq, row0, rows, position, head, k0, k1, tiles, cost;
+    int64_t first;  // device-wide index of the item's first unit of cost (its tiles follow kSetup units)
 };
 
 // The blocks of rows of all sequences in order, and a run of their tiles.
-struct Cursor {
+template <int kAloneCost>
+struct RunCursor {
     const AttentionParams* p;
     int block_rows;  // rows of a full item
-    int seq, block, head, k;  // k: unit of the item, kSetup + tile
+    int seq, block, head, k;  // k: unit of the item
     int64_t at;               // device-wide index of the next unit
     int left;
     int begin, start, rows;   // of sequence `seq`
 
+    static __device__ __forceinline__ int tiles_of(int start, int rows, int block, int block_rows) {
+        return (start + min((block + 1) * block_rows, rows) + kN - 1) / kN;
+    }
+    static __device__ __forceinline__ int cost_of(int rows, int block, int block_rows) {
+        return 2 * (rows - block * block_rows) <= block_rows ? kAloneCost : kPairCost;
+    }
     static __device__ __forceinline__ int units_of(int start, int rows, int block, int block_rows) {
-        return kSetup + (start + min((block + 1) * block_rows, rows) + kN - 1) / kN;
+        return kSetup + cost_of(rows, block, block_rows) * tiles_of(start, rows, block, block_rows);
     }
     // The next segment; false when the run is done.
     __device__ __forceinline__ bool next(Segment& s) {
         do
             if (!advance(s)) return false;
-        while (s.k0 >= s.k1);  // the run ends within an item's set-up units
+        while (s.k0 >= s.k1);  // no tile of the item begins in the run
         return true;
     }
     __device__ __forceinline__ bool advance(Segment& s) {
@@ -279,9 +289,11 @@ struct Cursor {
         s.row0 = begin + block * block_rows;
         s.rows = min(block_rows, rows - block * block_rows);
         s.position = start + block * block_rows;
-        const int units = units_of(start, rows, block, block_rows), end = min(units, k + left);
-        s.tiles = units - kSetup;
-        s.k0 = max(k - kSetup, 0), s.k1 = end - kSetup;
+        const int tiles = tiles_of(start, rows, block, block_rows), cost = cost_of(rows, block, block_rows);
+        const int end = min(kSetup + cost * tiles, k + left);
+        s.tiles = tiles, s.cost = cost;
+        // the tiles whose first unit is in the run
+        s.k0 = max(k - kSetup + cost - 1, 0) / cost, s.k1 = max(end - kSetup + cost - 1, 0) / cost;
         s.first = at - k;
         left -= end - k, at += end - k;
         k = 0;
@@ -293,6 +305,7 @@ struct Cursor {
 template <class T, int F, int D>
 __global__ void __launch_bounds__(kThreads, 1) prefill_kernel(const AttentionParams p) {
     using S = Shape<T, D>;
+    using Cursor = RunCursor<S::kAloneCost>;
     constexpr int kHalves = S::kHalves, kStages = S::kStages;
     extern __shared__ unsigned char smem_raw[];
     unsigned char* sm = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -386,7 +399,8 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_kernel(const AttentionPar
     }
     const int heads = p.cache.kv_heads;
     const int64_t total = units_before[kThreads] * heads;
-    const int ctas = int(total < int64_t(gridDim.x) ? total : int64_t(gridDim.x));
+    // every run holds a tile's first unit wherever it lies in an item
+    const int ctas = int(min(total / kPairCost, int64_t(gridDim.x)));
     const int64_t base = ctas ? (total >> 32 ? total / ctas : int64_t(uint32_t(total) / uint32_t(ctas))) : 0;
     const int extra = int(total - base * ctas);
     auto cta_of = [&](int64_t unit) {
@@ -740,7 +754,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_kernel(const AttentionPar
                 return ok;
             };
             if (!meet()) break;
-            const int c0 = cta_of(seg.first + kSetup), n = cta_of(seg.first + kSetup + seg.tiles - 1) - c0 + 1;
+            const int c0 = cta_of(seg.first + kSetup), n = cta_of(seg.first + kSetup + seg.cost * (seg.tiles - 1)) - c0 + 1;
             if (v == 0) {
                 const bool mine_last = atomicAdd(counters + 2 * c0 + w, 1u) == unsigned(n - 1);
                 if (mine_last) counters[2 * c0 + w] = 0;
