@@ -13,16 +13,16 @@
 // 64 bits measured 24 us for 8192 rows of 9 + 3 + 3 heads x 64 FP32, and 290 us for 20447 rows of
 // 32 + 8 + 8 heads x 128 BF16: its conversions bound it.)
 //
-// A CTA takes up to 8 packed rows: all its threads rotate their q, and its warps write the
-// tiles of the blocks that begin among its rows (a tile's first appended row is in one CTA
-// only). A tile is (block, kv head, K or V); its scale needs the largest magnitude of all
+// A CTA takes up to 8 packed rows: its warps write the tiles of the blocks that begin among
+// its rows (a tile's first appended row is in one CTA only), or all its threads rotate
+// their q; one CTA does both, or two share the rows (launch_append). A tile is (block, kv head, K or V); its scale needs the largest magnitude of all
 // its new tokens, so one warp takes it whole, 16 tokens (8 of head_dim 128) in registers at
 // a time, twice: magnitude, then codes. Fewer rows per CTA when there are few (one for a
 // decode step), so that all SMs take part.
 //
-// Measured: 8192 rows of 9 + 3 + 3 heads x 64 FP32 16.8 us (3.2 TB/s), 20447 of 32 + 8 + 8 heads x
-// 128 BF16 155 us (3.2 TB/s), half of the copy rate: a warp's loads, magnitude and codes follow
-// one another, and the 20 warps of an SM hide part of that.
+// Measured: 8192 rows of 9 + 3 + 3 heads x 64 FP32 15.0 us (3.6 TB/s), 20447 of 32 + 8 + 8 heads x
+// 128 BF16 128 us (3.9 TB/s), 0.55 to 0.6 of the copy rate: a warp's loads, magnitude and codes
+// follow one another, and the 20 warps of an SM hide part of that.
 #include "kv8.cuh"
 
 namespace mpb {
@@ -377,7 +377,7 @@ __global__ void __launch_bounds__(kThreads, kThreads == 128 ? 5 : 2) append_kern
     // ---- tiles of the blocks whose first appended row is here
     const int bt = p.cache.block_tokens, tiles = 2 * p.cache.kv_heads;
     int turn = warp;  // tiles go round the warps
-    for (int i = 0; i < rows; ++i) {
+    for (int i = 0; i < (blockIdx.y == 0 ? rows : 0); ++i) {
         const Place at = places[i];
         const int slot = at.position % bt;
         if (at.seq < 0) continue;
@@ -395,8 +395,8 @@ __global__ void __launch_bounds__(kThreads, kThreads == 128 ? 5 : 2) append_kern
         turn -= tiles;
     }
     // ---- q: a chunk of a head of a row per thread, kFly of them in flight
-    if (!p.q) return;
-    constexpr int kFly = 4;
+    if (!p.q || blockIdx.y + 1 != gridDim.y) return;
+    constexpr int kFly = kThreads == 128 ? 8 : 4;  // 20447 rows: 136 us with 4, 128 with 8; 256 single rows: 5.1 and 5.4
     const int per_row = p.heads * kChunks, total = rows * per_row;
     const Chunk ch = chunk_of<kInterleaved>(tid % kChunks, p.rotary_dim);  // kThreads is a multiple of kChunks
     const Angles angles{p.cos, p.sin, p.rotary_dim / 2};
@@ -442,9 +442,13 @@ cudaError_t launch_append(const AppendParams& p, int type, int format, int head_
         const uint32_t per_row = p.heads * (kDim / 8), inverse = uint32_t(((uint64_t(1) << 32) + per_row - 1) / per_row);
         // A row alone: 8 warps, so that its tiles are written side by side (5 rows, 256 rows: 4.1 and 5.1 us,
         // 5.3 and 5.9 with 4 warps). More rows: 4 warps, of which more CTAs overlap (8192 rows of FP32:
-        // 17 us, 20 with 8 warps).
+        // 17 us, 20 with 8 warps). The tiles' CTAs come before the queries' (of which more bytes are in
+        // flight): 8192 rows 15.0 us against 16.7 with one CTA for both (17.7 in turn, 17.5 queries
+        // first), 20447 rows of BF16 128 against 157, 5 rows 3.5 against 3.9. Single rows that fill
+        // the SMs without are not split: 256 rows 5.1 us, 5.6 split.
+        const int parts = p.q && (each > 1 || 2 * p.rows <= 148) ? 2 : 1;
         auto launch = [&](auto kernel, int threads) {
-            return launch_pdl(kernel, dim3((p.rows + each - 1) / each), dim3(threads), 0, stream, p, each, inverse);
+            return launch_pdl(kernel, dim3((p.rows + each - 1) / each, parts), dim3(threads), 0, stream, p, each, inverse);
         };
         if (each == 1)
             return p.interleaved ? launch(append_kernel<T, kFormat, kDim, true, 256>, 256)
