@@ -435,7 +435,7 @@ __global__ void __launch_bounds__(kThreads, kThreads == 128 ? 5 : 2) append_kern
 
 cudaError_t launch_append(const AppendParams& p, int type, int format, int head_dim, cudaStream_t stream) {
     return dispatch(type, format, head_dim, [&](auto t, auto f, auto d) {
-        const int each = std::clamp(p.rows / (2 * 148), 1, kMaxRows);
+        const int each = std::clamp(p.rows / (2 * kCtas), 1, kMaxRows);
         using T = decltype(t);
         constexpr int kFormat = decltype(f)::value, kDim = decltype(d)::value;
         // x / per_row = high half of x * inverse while x * per_row < 2^32: x < 8 * per_row, per_row <= 2^14
@@ -446,7 +446,7 @@ cudaError_t launch_append(const AppendParams& p, int type, int format, int head_
         // flight): 8192 rows 15.0 us against 16.7 with one CTA for both (17.7 in turn, 17.5 queries
         // first), 20447 rows of BF16 128 against 157, 5 rows 3.5 against 3.9. Single rows that fill
         // the SMs without are not split: 256 rows 5.1 us, 5.6 split.
-        const int parts = p.q && (each > 1 || 2 * p.rows <= 148) ? 2 : 1;
+        const int parts = p.q && (each > 1 || 2 * p.rows <= kCtas) ? 2 : 1;
         auto launch = [&](auto kernel, int threads) {
             return launch_pdl(kernel, dim3((p.rows + each - 1) / each, parts), dim3(threads), 0, stream, p, each, inverse);
         };
