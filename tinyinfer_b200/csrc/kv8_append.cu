@@ -282,7 +282,8 @@ __device__ __forceinline__ void append_tile(const AppendParams& p, const T* rows
         __syncwarp();
     }
     if (lane == 0) *scale = pow2(power);
-    const float inv = pow2(-power);
+    // a held scale may be 2^127: its inverse is subnormal (a new scale is at most 2^122)
+    const float inv = power == 127 ? 5.877471754e-39f : pow2(-power);
     for (int first = 0; first < n; first += kUnitTokens) {
         if (n > kUnitTokens) {  // else still there
             load(first);
