@@ -25,3 +25,27 @@ def test_append_under_the_largest_scale(built, fmt, rotary):
         x = values(5, 960, 82, 0.0)
         x[:, 576:] *= 2e38 / x[:, 576:].abs().amax()  # rotated magnitudes stay below 2.9e38
         run(tables, [5], [3], x)
+
+
+@pytest.mark.parametrize("first,late,gap", [(0.0, 2.0 ** 10, 140), (2.0 ** -100, 2.0 ** 20, 140),
+                                            (0.0, 2.0 ** 100, 120), (2.0 ** -100, 2.0 ** 100, 100), (1.0, 2.0 ** 60, 90)])
+def test_faint_tokens_with_large_value_scales(built, first, late, gap):
+    """Tokens whose weights are 2^-gap of the others', with V scales far above theirs, turn about with them; decode and
+    prefill row by row. Weights below 2^-126 of a row's largest count as zero (FP32's smallest normal number), so that
+    many times the largest V value comes on top of the bound."""
+    n = 4096
+    cache = Cache(n // 16, 3, 64, 16, "int8")
+    tables = tables_for([n], 16, n // 16, 83, spare=0)
+    fill(cache, tables, [n], 84, (0, 0))
+    faint = tables[0, torch.arange(n // 16, device=DEV) % 4 >= 2].long()  # every other 32 tokens
+    loud = tables[0, torch.arange(n // 16, device=DEV) % 4 < 2].long()
+    cache.pages[:, :, 0] = 0
+    cache.pages[faint, :, 0, :, 0] = -64
+    cache.scales[loud, :, 1], cache.scales[faint, :, 1] = first, late
+    q = torch.zeros(1, 576, device=DEV)
+    q.view(9, 64)[:, 0] = gap * math.log(2) / 8  # the faint tokens' score is -gap ln 2
+    want, weight, size, top = ref.attend(q.view(1, 9, 64), cache.pages, cache.scales, "int8", tables[0].tolist(), n, 0.125)
+    limit = ref.bound(want, weight, size, top, n, 64, False) + n * 2.0 ** -126 * late * 127
+    for _, out in (decode(cache, 9, tables, [n], "f32", q=q), prefill(cache, 9, tables, [1], [n - 1], "f32", q=q)):
+        assert bool(torch.isfinite(out).all())
+        assert bool(((out.view(1, 9, 64).double() - want).abs() <= limit).all())

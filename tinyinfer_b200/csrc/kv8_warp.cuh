@@ -37,6 +37,9 @@ constexpr int kChain = 4;                  // units per chain of tensor-op sums 
 constexpr float kWeightTop = 256.f;        // a weight of `unit` is 2^8 in FP16
 constexpr float kSlack = 6.f;              // a score may pass m by this (weights up to 2^6)
 constexpr float kUnitFloor = 7.70371977754894e-34f;  // 2^-110: below every scale the append makes
+// 2^-118: `unit` is at least that much of a scale in use (so far as reach < 2 unit: 2^-119), so that
+// kWeightTop * scale / unit stays below 2^127 when the tokens under a large scale have faint weights
+constexpr float kScaleFloor = 3.0092655e-36f;
 
 template <class T, int F, int D>
 struct WarpRow {
@@ -194,6 +197,7 @@ struct WarpRow {
         float reach = 0.f;  // largest weight times scale of the unit
 #pragma unroll
         for (int u = 0; u < kTiles; ++u) {
+            reach = fmaxf(reach, scale[u].y * kScaleFloor);
             const float tops = fmaxf(fmaxf(t[u][0][0], t[u][0][1]), fmaxf(t[u][1][0], t[u][1][1]));
             if (tops != -INFINITY) reach = fmaxf(reach, scale[u].y * ex2(tops - m_new));
         }
