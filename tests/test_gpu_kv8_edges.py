@@ -49,3 +49,20 @@ def test_faint_tokens_with_large_value_scales(built, first, late, gap):
     for _, out in (decode(cache, 9, tables, [n], "f32", q=q), prefill(cache, 9, tables, [1], [n - 1], "f32", q=q)):
         assert bool(torch.isfinite(out).all())
         assert bool(((out.view(1, 9, 64).double() - want).abs() <= limit).all())
+
+
+@pytest.mark.parametrize("rows", [5, 100])
+@pytest.mark.parametrize("scale", [2.0 ** 127, 3.4028234663852886e38])
+def test_value_scales_at_the_top_of_the_range(built, scale, rows):
+    """V scales up to FP32's largest number, under codes of 0 and of E4M3's smallest step: outputs are the values."""
+    cache = Cache(8, 3, 64, 16, "e4m3")
+    tables = tables_for([100], 16, 8, 85)
+    fill(cache, tables, [100], 86, (-6, -6))
+    cache.pages[:, :, 1] = torch.arange(64, device=DEV).to(torch.int8) % 2  # codes 0 and 2^-9 by turns
+    cache.scales[:, :, 1] = scale
+    want = (torch.arange(64, device=DEV) % 2).double() * 2.0 ** -9 * scale
+    # scores, weights and the joined sums have FP32's roundings in common with the normaliser but for their order: 100
+    # terms on each side, 2^-24 each, and a few roundings of the result
+    for _, out in (prefill(cache, 9, tables, [rows], [100 - rows], "f32"), decode(cache, 9, tables, [100], "f32")):
+        off = (out.view(-1, 9, 64).double() - want).abs()
+        assert bool(torch.isfinite(out).all()) and bool((off <= want * 210 * 2.0 ** -24).all())

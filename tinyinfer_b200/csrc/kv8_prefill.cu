@@ -618,7 +618,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_kernel(const AttentionPar
                             const float decay = m == -INFINITY ? 0.f : ex2(m - m_new);
                             // the largest so far, in whole powers of two; within the exponents of floats
                             const float most = fmaxf(m == -INFINITY ? -110.f : float(unit_log) + (m - m_new), reach - m_new);
-                            const int next = int(floorf(fminf(fmaxf(most, -110.f), 120.f)));
+                            const int next = int(floorf(fminf(fmaxf(most, -110.f), 126.f)));
                             moved = m == -INFINITY ? 0.f : ex2(m - m_new + float(unit_log - next));
                             l *= decay;
                             m = m_new, unit_log = next;
