@@ -66,3 +66,46 @@ def test_value_scales_at_the_top_of_the_range(built, scale, rows):
     for _, out in (prefill(cache, 9, tables, [rows], [100 - rows], "f32"), decode(cache, 9, tables, [100], "f32")):
         off = (out.view(-1, 9, 64).double() - want).abs()
         assert bool(torch.isfinite(out).all()) and bool((off <= want * 210 * 2.0 ** -24).all())
+
+
+def test_long_bf16_prefill_does_not_fade(built):
+    """2^20 tokens of one V value under random scores: the value comes back. (The tensor core cuts its sums by up to
+    2^-23 a product; an output added up in one chain over 65536 of them came out 0.5 % small.)"""
+    n, rows, count = 1 << 20, 256, 152
+    cache = Cache(n // 256, 1, 64, 256, "int8")
+    tables = tables_for([n], 256, n // 256, 87, spare=0).repeat(count, 1).contiguous()  # enough items that none is cut
+    g = torch.Generator(DEV).manual_seed(88)
+    cache.pages[:, :, 0] = torch.randint(-100, 101, cache.pages[:, :, 0].shape, generator=g, device=DEV, dtype=torch.int8)
+    cache.pages[:, :, 1] = 100
+    cache.scales.fill_(2.0 ** -6)
+    _, out = prefill(cache, 1, tables, [rows] * count, [n - rows] * count, "bf16")
+    assert bool((out == 100 * 2.0 ** -6).all()), out.unique()
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+def test_bf16_prefill_chains_with_rising_scores_and_scales(built, dim):
+    """Contexts of three chains of sums and a rest; scores that rise, stay or fall along them (by head), V scales that
+    rise 2^12 times, so that the reference and the unit move within and between chains."""
+    n, rows, count, heads = 100000, 100, 150, 4
+    cache = Cache(n // 32, 1, dim, 32, "int8")
+    table = tables_for([n], 32, n // 32, 95, spare=0)
+    fill(cache, table, [n], 96, (0, 0))
+    blocks, at = table[0].long(), torch.arange(n // 32, device=DEV)
+    keys = torch.zeros(n, dim, dtype=torch.int8, device=DEV)
+    marked = torch.arange(0, n, 997, device=DEV)  # every 997th token has a score, from 0 up to 16
+    keys[marked, 0] = (marked * 127 // n).to(torch.int8)
+    cache.pages[blocks, 0, 0] = keys.view(-1, 32, dim)
+    cache.scales[blocks, 0, 1] = torch.exp2((at * 12 // len(at) - 6).float())
+    starts = [n - rows - 61 * i for i in range(count)]
+    q = torch.zeros(rows * count, heads, dim, device=DEV)
+    q[..., 0] = torch.tensor([1.0, 0.5, 0.0, -1.0], device=DEV) * (dim ** 0.5 / 8)
+    q, out = prefill(cache, heads, table.repeat(count, 1).contiguous(), [rows] * count, starts, "bf16", q=q.flatten(1))
+    for i in (0, 75, 149):
+        part = slice(i * rows, (i + 1) * rows)
+        want, weight, _, top = ref.attend(q[part].view(rows, heads, dim), cache.pages, cache.scales, "int8",
+                                          table[0].tolist(), starts[i] + rows, dim ** -0.5)
+        # a weight is one FP16 half (2^-11), its score has two roundings (|score| < 2^5 in powers of two: 2^-18), the
+        # chains cut 2^-12, the normaliser adds 2^-12 at most; a rounding of the result; FP16's smallest steps
+        limit = weight * (2 ** -11 + 2 ** -17 + 2 ** -11) + want.abs() * 2 ** -8 + top * n * 2 ** -33
+        off = (out[part].view(rows, heads, dim).double() - want).abs()
+        assert bool((off <= limit).all()), float((off / limit).max())

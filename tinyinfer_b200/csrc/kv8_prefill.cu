@@ -24,7 +24,7 @@
 // turn by both tiles: with three, a tile's next S is ready before its threads ask for it.
 //
 // Outputs: FP32 ones are added up in registers, tile by tile; BF16 ones stay in tensor
-// memory over an item's tiles.
+// memory over kChainTiles of an item's tiles, and chains are added up in the workspace.
 //
 // FP32 precision: the query is two FP16 halves (each row scaled by a power of two towards
 // FP16's top), so S is two products per useful one; the weights, with V's scales folded
@@ -66,6 +66,10 @@ constexpr int kGroups = kN / kGroupTokens;
 // 2^2 some row of a warp asked for one in most tiles. FP16's smallest half step, 2^-25, is
 // 2^-33 of the largest.
 constexpr int kTopLog = 8;
+// K/V tiles of one chain of sums in tensor memory (BF16 outputs): 2048 products, each of which may cut 2^-23
+// of the sum, 2.4e-4 in all, an eighth of BF16's half step. (An uncut item of 2^20 tokens came out 5e-3
+// small in one chain.)
+constexpr int kChainTiles = 256;
 constexpr float kRoom = 7.f;
 
 template <class T, int D>
@@ -553,6 +557,31 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_kernel(const AttentionPar
                     }
                 }
             };
+            // a part of the item in the workspace, vectors side by side. Slot 0 of a CTA: the item began
+            // earlier, slot 1: it begins here. A segment's own slot is free until its end: chains go there
+            constexpr int64_t kPart = int64_t(kM) * (D + 2);
+            float* parts = reinterpret_cast<float*>(static_cast<unsigned char*>(p.workspace) + kCounterBytes);
+            auto part = [&](int cta, int which) { return parts + ((int64_t(cta) * 2 + which) * 2 + w) * kPart; };
+            [[maybe_unused]] float chain_m = -INFINITY;  // reference score of the finished chains
+            // BF16: a chain of outputs, in plain units, out of tensor memory
+            [[maybe_unused]] auto end_chain = [&](bool first) {
+                const float unit = pow2(unit_log - kTopLog), decay = chain_m == m ? 1.f : ex2(chain_m - m);
+                float* mine = part(blockIdx.x, seg.k0 == 0) + v * 4;
+#pragma unroll 1
+                for (int i = 0; i < D; i += 16) {
+                    float x[16];
+                    tmem_load(o_at + i, x);
+#pragma unroll
+                    for (int c = 0; c < 16; c += 4) {
+                        float4* at = reinterpret_cast<float4*>(mine + (i + c) * kM);
+                        float4 sum = first ? make_float4(0.f, 0.f, 0.f, 0.f) : *at;
+                        sum.x = fmaf(x[c], unit, sum.x * decay), sum.y = fmaf(x[c + 1], unit, sum.y * decay);
+                        sum.z = fmaf(x[c + 2], unit, sum.z * decay), sum.w = fmaf(x[c + 3], unit, sum.w * decay);
+                        *at = sum;
+                    }
+                }
+                chain_m = m;
+            };
             for (int j = 0; j < tiles; ++j) {
                 // S places in order: j = 0 of both tiles, j = 1, ..., each as far as it goes
                 const int place = used + (w ? min(j + 1, n0) + j : j + min(j, n1));
@@ -688,6 +717,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_kernel(const AttentionPar
                 if (!ok || !wait_outputs()) break;
                 if (S::kAdd && j) add_outputs(moved);
                 tmem_wait_store();
+                if (!S::kAdd && j && j % kChainTiles == 0) end_chain(j == kChainTiles);
                 tmem_fence_before();
                 arrive(p_full + w);
             }
@@ -701,6 +731,16 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_kernel(const AttentionPar
             slot += most;
             if (!ok) break;
             const float u = pow2(unit_log - kTopLog);
+            if (!S::kAdd && tiles > kChainTiles) {
+                const float* mine = part(blockIdx.x, seg.k0 == 0) + v * 4;
+                const float by = (chain_m == m ? 1.f : ex2(chain_m - m)) / u;
+#pragma unroll
+                for (int d = 0; d < D; d += 4) {
+                    const float4 x = *reinterpret_cast<const float4*>(mine + d * kM);
+                    o[d] = fmaf(x.x, by, o[d]), o[d + 1] = fmaf(x.y, by, o[d + 1]);
+                    o[d + 2] = fmaf(x.z, by, o[d + 2]), o[d + 3] = fmaf(x.w, by, o[d + 3]);
+                }
+            }
             // rows out through this tile's query buffer (its products are done): the warp's 32 rows,
             // 16-byte words XOR-ed by the row against bank conflicts, then word by word
             auto write_rows = [&](float r) {
@@ -731,12 +771,8 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_kernel(const AttentionPar
                 arrive(q_free + w);
                 continue;
             }
-            // ---- a part of the item: to the workspace; the last CTA to arrive joins them. Slot 0 of
-            // a CTA: the item began earlier, slot 1: it begins here. Vectors side by side.
-            constexpr int64_t kPart = int64_t(kM) * (D + 2);
+            // ---- a part of the item: to the workspace; the last CTA to arrive joins them
             unsigned* counters = static_cast<unsigned*>(p.workspace);
-            float* parts = reinterpret_cast<float*>(static_cast<unsigned char*>(p.workspace) + kCounterBytes);
-            auto part = [&](int cta, int which) { return parts + ((int64_t(cta) * 2 + which) * 2 + w) * kPart; };
             auto state = [&](int cta, int which) { return parts + (((int64_t(cta) * 2 + which) * 2 + w) * kPart + D * kM + v * 2); };
             {
                 float* mine = part(blockIdx.x, seg.k0 == 0);
@@ -914,7 +950,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_kernel(const AttentionPar
                         tmem_fence_after();
                         const uint32_t s_at = tmem + place * kN, o_at = tmem + S::kBuffers * kN + o.w * D;
                         const uint64_t vd = v_desc + uint64_t(stage * (S::kTileBytes >> 4));
-                        const bool keep = !S::kAdd && o.j > 0, leave = o.w || o.j >= n1;  // leave: V's last use
+                        const bool keep = !S::kAdd && o.j % kChainTiles != 0, leave = o.w || o.j >= n1;  // leave: V's last use
                         if (elect()) {
 #pragma unroll
                             for (int half = kHalves - 1; half >= 0; --half)
