@@ -109,3 +109,20 @@ def test_bf16_prefill_chains_with_rising_scores_and_scales(built, dim):
         limit = weight * (2 ** -11 + 2 ** -17 + 2 ** -11) + want.abs() * 2 ** -8 + top * n * 2 ** -33
         off = (out[part].view(rows, heads, dim).double() - want).abs()
         assert bool((off <= limit).all()), float((off / limit).max())
+
+
+def test_long_bf16_decode_does_not_fade(built):
+    """2^20 tokens per row and a row per warp: values of 64 and 65 whose mean lies just above the border of two BF16
+    numbers (64 and 64.5), under random scores. Sums that lost 2^-10 on the way fall on the other side of it."""
+    n, rows = 1 << 20, 2 * 148 * 16
+    cache = Cache(n // 256, 1, 64, 256, "int8")
+    tables = tables_for([n], 256, n // 256, 97, spare=0).repeat(rows, 1).contiguous()
+    g = torch.Generator(DEV).manual_seed(98)
+    cache.pages[:, :, 0] = torch.randint(-100, 101, cache.pages[:, :, 0].shape, generator=g, device=DEV, dtype=torch.int8)
+    cache.pages[:, :, 1] = (64 + (torch.rand(cache.pages[:, :, 1].shape, generator=g, device=DEV) < 0.27)).to(torch.int8)
+    cache.scales[..., 0], cache.scales[..., 1] = 2.0 ** -8, 1.0
+    q, out = decode(cache, 1, tables, [n] * rows, "bf16")
+    for i in range(0, rows, 599):
+        want, weight, _, _ = ref.attend(q[i: i + 1].view(1, 1, 64), cache.pages, cache.scales, "int8", tables[i].tolist(), n, 0.125)
+        # half a step of the result (0.25), and 2^-13 for the sums
+        assert bool(((out[i].double() - want.view(-1)).abs() <= 0.25 + weight.view(-1) * 2 ** -13).all())

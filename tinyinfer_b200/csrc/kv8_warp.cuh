@@ -15,8 +15,9 @@
 // V's block scale is folded into the weights.
 //
 // Tensor-op sums are cut, not rounded: each added tile loses about 2^-25.7 of the sum
-// (measured: 1.8e-5 after 1000 tiles). FP32 outputs therefore add the products up in
-// chains of kChain units and the chains in FP32 registers.
+// (measured: 1.8e-5 after 1000 tiles; up to 2^-23). Outputs are therefore added up in chains of
+// kChain units, and the chains in FP32 registers: 128 tokens a chain for FP32 outputs, 32768
+// (2048 tiles, at most 2.4e-4) for BF16 ones, which came out 6e-3 small after one chain of 2^20.
 //
 // The state is a running softmax: m (the reference score), l (sum of weights), and outputs
 // in units of `unit`, a power of two at most the largest weight times scale so far, so that
@@ -33,7 +34,6 @@ namespace kv8 {
 constexpr int kTile = 16;                  // tokens of a tile: the K of one product
 constexpr int kTiles = 2;                  // tiles of a unit: their products overlap, and votes and shuffles halve
 constexpr int kUnit = kTile * kTiles;
-constexpr int kChain = 4;                  // units per chain of tensor-op sums (FP32 outputs)
 constexpr float kWeightTop = 256.f;        // a weight of `unit` is 2^8 in FP16
 constexpr float kSlack = 6.f;              // a score may pass m by this (weights up to 2^6)
 constexpr float kUnitFloor = 7.70371977754894e-34f;  // 2^-110: below every scale the append makes
@@ -45,9 +45,10 @@ template <class T, int F, int D>
 struct WarpRow {
     static constexpr int kHalves = D / 64;
     static constexpr bool kSplit = sizeof(T) == 4;  // BF16 outputs: weights as one FP16 half (2^-12 relative)
+    static constexpr int kChain = kSplit ? 4 : 1024;  // units per chain of tensor-op sums
     uint32_t qa[D / 16][4];
     // outputs: lane (n, c) holds head n's dims 16 i / 2 + 4 c + i % 2 + {0, 2} in o[i][0, 1]
-    // (weights' hi halves) and o[i][2, 3] (lo)
+    // (weights' hi halves) and o[i][2, 3] (lo; BF16: finished chains, to which the products add zeros)
     float o[D / 8][4];
     float sum[kSplit ? D / 8 : 1][2];  // finished chains
     float m, l, unit, inv_unit, k_factor;
@@ -182,11 +183,9 @@ struct WarpRow {
                 }
             }
         }
-        if constexpr (kSplit) {
-            if (++chain == kChain) {
-                close();
-                chain = 0;
-            }
+        if (++chain == kChain) {
+            close();
+            chain = 0;
         }
     }
 
@@ -218,12 +217,19 @@ struct WarpRow {
         m = m_new, unit = pow2(exponent), inv_unit = kWeightTop * pow2(-exponent);
     }
 
+    // Ends a chain.
     __device__ __forceinline__ void close() {
 #pragma unroll
         for (int i = 0; i < D / 8; ++i) {
-            sum[i][0] += o[i][0] + o[i][2];
-            sum[i][1] += o[i][1] + o[i][3];
-            o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
+            if constexpr (kSplit) {
+                sum[i][0] += o[i][0] + o[i][2];
+                sum[i][1] += o[i][1] + o[i][3];
+                o[i][2] = o[i][3] = 0.f;
+            } else {
+                o[i][2] += o[i][0];
+                o[i][3] += o[i][1];
+            }
+            o[i][0] = o[i][1] = 0.f;
         }
     }
 
