@@ -126,3 +126,41 @@ def test_long_bf16_decode_does_not_fade(built):
         want, weight, _, _ = ref.attend(q[i: i + 1].view(1, 1, 64), cache.pages, cache.scales, "int8", tables[i].tolist(), n, 0.125)
         # half a step of the result (0.25), and 2^-13 for the sums
         assert bool(((out[i].double() - want.view(-1)).abs() <= 0.25 + weight.view(-1) * 2 ** -13).all())
+
+
+@pytest.mark.parametrize("rows", [10, 900])
+@pytest.mark.parametrize("fault", ["table", "rotation", "rows", "order"])
+def test_append_leaves_a_bad_sequence_out(built, fault, rows):
+    """A sequence that begins in range and ends behind its table, the rotation tables or the call's rows, or whose
+    offsets fall: reported, and none of its rows is written; the others are."""
+    bt, heads, kh, d = 16, 4, 2, 64
+    table = 2 * rows // bt + 3
+    cache = Cache(3 * table + 3, kh, d, bt, "int8")
+    tables = tables_for([table * bt] * 3, bt, cache.c.max_blocks, 89, spare=0)
+    positions = table * bt - (20 if fault == "rotation" else 0)
+    run = Appender(cache, heads, "f32", d, "half", positions)
+    starts, offsets = [5, 0, 3], [0, rows, 2 * rows, 3 * rows]
+    fill(cache, tables, starts, 90)
+    good = [0, 2]
+    if fault == "rows":
+        good, offsets[3] = [0, 1], 3 * rows + 1
+    elif fault == "order":
+        good, offsets[2:] = [0], [rows - 2, rows]  # the third sequence names rows of the first
+    else:
+        starts[1] = positions - rows + 3
+    x = values(3 * rows, (heads + 2 * kh) * d, 91)
+    q_out = torch.full((3 * rows, heads * d), 7.0, device=DEV)
+    pages, scales = cache.store.clone(), cache.scale_store.clone()
+    off, first = (torch.tensor(a, dtype=torch.int32, device=DEV) for a in (offsets, starts))
+    mp.kv8_append(cache.c, run.args(x, q_out, tables, off, first), run.error.data_ptr(), stream())
+    assert mp.kv8_status(run.error.data_ptr(), stream()) == mp.MP_ERR_BOUNDS
+    for i in good:
+        part = slice(i * rows, (i + 1) * rows)
+        assert bool((q_out[part] != 7).any(1).all())
+        k, v = (x[part, a: a + kh * d].double().view(rows, kh, d) for a in (heads * d, (heads + kh) * d))
+        at = torch.arange(rows, device=DEV) + starts[i]
+        k = ref.rotate(k, run.cos[at].double(), run.sin[at].double(), d, "half")
+        ref.append(pages[:, 0], scales[:, 0], "int8", k, v, [tables[i].tolist()], [0, rows], [starts[i]])
+        q_out[part] = 7
+    assert bool((q_out == 7).all()), "rows of a sequence that was to be left out"
+    assert torch.equal(pages, cache.store) and torch.equal(scales.view(torch.int32), cache.scale_store.view(torch.int32))

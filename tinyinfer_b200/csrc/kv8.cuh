@@ -99,16 +99,20 @@ __device__ __forceinline__ int block_id(const Cache& c, const int32_t* table, in
     return checked_id(c, page < table_stride ? table[page] : -1, error);
 }
 
-// Rows of a prefill's sequence i, 0 for one whose metadata is out of range.
-__device__ __forceinline__ int sequence_rows(const AttentionParams& p, int i, int& begin, int& start) {
-    begin = p.row_offsets[i], start = p.starts[i];
-    const int end = p.row_offsets[i + 1];
-    if (begin < 0 || end < begin || end > p.rows || (end > begin && start < 0) ||
-        int64_t(start) + (end - begin) > int64_t(p.table_stride) * p.cache.block_tokens) {
-        if (end != begin) raise_error(p.error, kErrBounds);
+// Rows of a sequence at row_offsets begin .. end of a call with `rows` packed ones, 0 if its metadata is out
+// of range: offsets that fall or leave the call's rows, or positions outside 0 .. limit - 1.
+__device__ __forceinline__ int checked_rows(int begin, int end, int start, int rows, int64_t limit, unsigned* error) {
+    if (begin < 0 || end < begin || end > rows || (end > begin && start < 0) || int64_t(start) + (end - begin) > limit) {
+        if (end != begin) raise_error(error, kErrBounds);
         return 0;
     }
     return end - begin;
+}
+
+// Rows of a prefill's sequence i.
+__device__ __forceinline__ int sequence_rows(const AttentionParams& p, int i, int& begin, int& start) {
+    begin = p.row_offsets[i], start = p.starts[i];
+    return checked_rows(begin, p.row_offsets[i + 1], start, p.rows, int64_t(p.table_stride) * p.cache.block_tokens, p.error);
 }
 
 // 2^x as a float, x in -126 .. 127.

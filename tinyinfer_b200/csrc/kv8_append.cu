@@ -326,10 +326,16 @@ __device__ __forceinline__ void append_tile(const AppendParams& p, const T* rows
     if (odd && lane == 0) raise_error(p.error, kErrValue);
 }
 
-// A packed row's place: its sequence (-1: behind the last, or out of range) and position.
+// A packed row's place: its sequence (-1: behind the last, or of one that is out of range) and position.
 struct Place {
     int seq, position, end;  // end: the sequence's last row + 1
 };
+
+// Positions that a sequence may have: those of its table and of the rotation tables.
+__device__ __forceinline__ int64_t position_limit(const AppendParams& p) {
+    const int64_t tokens = int64_t(p.table_stride) * p.cache.block_tokens;
+    return p.rotary_dim ? min(tokens, int64_t(p.max_positions)) : tokens;
+}
 
 // By one warp, a row per lane from `row0` on (rows <= 32): a row's sequence is the first that
 // ends behind it. With sequences of one length it is known for row0; else it is found 32
@@ -354,13 +360,8 @@ __device__ __forceinline__ Place find_rows(const AppendParams& p, int row0, int 
     while (low < p.count && (end = p.row_offsets[low + 1]) <= row) ++low;
     if (low >= p.count) return {-1, 0, 0};
     const int begin = p.row_offsets[low], start = low == guess ? start_there : p.starts[low];
-    const int64_t position = int64_t(start) + row - begin;
-    if (row < begin || start < 0 || position >= int64_t(p.table_stride) * p.cache.block_tokens ||
-        (p.rotary_dim && position >= p.max_positions)) {
-        raise_error(p.error, kErrBounds);
-        return {-1, 0, 0};
-    }
-    return {low, int(position), min(end, p.rows)};
+    if (row < begin || checked_rows(begin, end, start, p.rows, position_limit(p), nullptr) == 0) return {-1, 0, 0};
+    return {low, start + row - begin, end};
 }
 
 template <class T, int F, int D, bool kInterleaved, int kThreads>
@@ -373,6 +374,9 @@ __global__ void __launch_bounds__(kThreads, kThreads == 128 ? 5 : 2) append_kern
     if (warp == 0) {
         const Place at = find_rows(p, row0, rows, lane);
         if (lane < rows) places[lane] = at;
+    } else if (blockIdx.y == 0) {  // meanwhile: sequences that are out of range report themselves
+        for (int i = blockIdx.x * (kThreads - 32) + tid - 32; i < p.count; i += gridDim.x * (kThreads - 32))
+            checked_rows(p.row_offsets[i], p.row_offsets[i + 1], p.starts[i], p.rows, position_limit(p), p.error);
     }
     __syncthreads();
     // ---- tiles of the blocks whose first appended row is here
@@ -385,8 +389,7 @@ __global__ void __launch_bounds__(kThreads, kThreads == 128 ? 5 : 2) append_kern
         if (slot && row0 + i != p.row_offsets[at.seq]) continue;
         const int row = row0 + i;
         const int32_t* entry = p.tables + int64_t(at.seq) * p.table_stride + at.position / bt;
-        int n = min(bt - slot, at.end - row);
-        if (p.rotary_dim) n = min(n, p.max_positions - at.position);  // rows past the tables report themselves
+        const int n = min(bt - slot, at.end - row);
         for (; turn < tiles; turn += kThreads / 32) {
             const int head = turn >> 1, part = turn & 1;
             const T* x = static_cast<const T*>(part ? p.v : p.k);
