@@ -274,8 +274,9 @@ int mp_paged_attention_status(void* stream);
  * and clears it): bit 1 = a block id outside [0, max_blocks) (an append leaves the
  * block's rows out, an attention reads block 0 instead); a length past the table (a row of
  * zeros); row_offsets that fall or leave `rows`, or positions outside the table or the
- * rotation tables (that sequence is left out whole: none of its rows is written); more than
- * 2^30 pieces of work for one SM (the call is left out); bit 2 = a wait inside the
+ * rotation tables (that sequence is left out whole: none of its rows is written; where offsets
+ * fall, others may be left out too); more than 2^30 pieces of work for one SM (the call is left
+ * out); bit 2 = a wait inside the
  * prefill kernel expired (its outputs are incomplete);
  * bit 4 = an appended value was NaN or infinite, or the scale of a block that already
  * held tokens was no power of two. */

@@ -164,3 +164,27 @@ def test_append_leaves_a_bad_sequence_out(built, fault, rows):
         q_out[part] = 7
     assert bool((q_out == 7).all()), "rows of a sequence that was to be left out"
     assert torch.equal(pages, cache.store) and torch.equal(scales.view(torch.int32), cache.scale_store.view(torch.int32))
+
+
+def test_prefill_refuses_offsets_that_fall(built):
+    """Offsets that fall name rows more than once, more of them than the plan's indexes count: the call is left out."""
+    cache = Cache(30, 3, 64, 16, "int8")
+    tables = tables_for([100] * 4, 16, 30, 92, spare=0)
+    fill(cache, tables, [100] * 4, 93)
+    q, out = values(100, 576, 94), torch.full((100, 576), 7.0, device=DEV)
+    workspace = torch.zeros(mp.kv8_prefill_workspace(cache.c, 9), dtype=torch.uint8, device=DEV)
+    off, first = (torch.tensor(a, dtype=torch.int32, device=DEV) for a in ([0, 100, 0, 100, 0], [0] * 4))
+    word = torch.zeros(1, dtype=torch.int32, device=DEV)
+    args = mp.Kv8PrefillArgs(q=q.data_ptr(), out=out.data_ptr(), q_stride=576, out_stride=576, tables=tables.data_ptr(),
+                             row_offsets=off.data_ptr(), starts=first.data_ptr(), workspace=workspace.data_ptr(),
+                             workspace_bytes=workspace.numel(), type=0, heads=9, table_stride=tables.stride(0), count=4,
+                             rows=100, scale=0.125)
+    mp.kv8_attention_prefill(cache.c, args, word.data_ptr(), stream())
+    assert mp.kv8_status(word.data_ptr(), stream()) == mp.MP_ERR_BOUNDS
+    assert bool((out == 7).all())
+    off.copy_(torch.tensor([0, 40, 40, 95, 100], dtype=torch.int32))  # the workspace serves the next call
+    mp.kv8_attention_prefill(cache.c, args, word.data_ptr(), stream())
+    assert mp.kv8_status(word.data_ptr(), stream()) == mp.MP_OK
+    for i, (lo, hi) in enumerate(((0, 40), (40, 40), (40, 95), (95, 100))):
+        if hi > lo:
+            check_rows(cache, 9, q[lo:hi], out[lo:hi], tables[i].tolist(), hi - lo, 0.125, False)

@@ -362,13 +362,17 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_kernel(const AttentionPar
     };
     int begin, start;
     {
-        int mine = 0;
-        for (int i = 0; i < share; ++i)
-            if (tid * share + i < p.count)
-                mine += (sequence_rows(p, tid * share + i, begin, start) + block_rows - 1) / block_rows;
+        int mine = 0, falls = 0;
+        for (int i = tid * share; i < min((tid + 1) * share, p.count); ++i) {
+            mine += (sequence_rows(p, i, begin, start) + block_rows - 1) / block_rows;
+            falls |= p.row_offsets[i + 1] < begin;
+        }
         const int before = int(scan(mine, sums));
         blocks_before[tid] = before;
         if (tid == kThreads - 1) blocks_before[kThreads] = before + mine;
+        // offsets that fall may rise again and name rows many times over, up to 2^44 blocks of them, past
+        // the indexes below: such a call is left out (reported above)
+        if (__syncthreads_or(falls) && tid == kThreads - 1) blocks_before[kThreads] = 0;
         __syncthreads();
     }
     const int blocks = blocks_before[kThreads], each = (blocks + kThreads - 1) / kThreads;
