@@ -388,6 +388,10 @@ int mp_kv8_attention_prefill(const mp_kv8_cache* cache, const mp_kv8_prefill_arg
  * MP_ERR_TIMEOUT or MP_ERR_NONFINITE (the first that applies in the order timeout,
  * bounds, nonfinite). */
 int mp_kv8_status(uint32_t* device_error, void* stream);
+/* Failure-path tests: the process's next mp_kv8_attention_prefill, if it goes as tiles, gets no V
+ * tiles and bounds its waits at `wait_us` microseconds (1 us .. 1 s). They run out, the kernel
+ * sets the timeout bit, waits for its products and copies, releases its tensor memory and returns. */
+int mp_kv8_inject_wait_timeout(int32_t wait_us);
 
 #ifdef __cplusplus
 }

@@ -188,3 +188,35 @@ def test_prefill_refuses_offsets_that_fall(built):
     for i, (lo, hi) in enumerate(((0, 40), (40, 40), (40, 95), (95, 100))):
         if hi > lo:
             check_rows(cache, 9, q[lo:hi], out[lo:hi], tables[i].tolist(), hi - lo, 0.125, False)
+
+
+@pytest.mark.parametrize("heads,kv_heads,dim,dtype", [(9, 3, 64, "f32"), (32, 8, 128, "bf16")])
+def test_prefill_waits_that_run_out(built, heads, kv_heads, dim, dtype):
+    """Waits that expire end the kernel with the timeout bit within their bound; the next call, over a workspace that
+    was zeroed again, is as ever."""
+    cache = Cache(60, kv_heads, dim, 16, "int8")
+    tables = tables_for([400, 300], 16, 60, 99)
+    fill(cache, tables, [400, 300], 100)
+    q = values(170, heads * dim, 101).to(DTYPES[dtype])
+    out = torch.zeros_like(q)
+    workspace = torch.zeros(mp.kv8_prefill_workspace(cache.c, heads), dtype=torch.uint8, device=DEV)
+    off, first = (torch.tensor(a, dtype=torch.int32, device=DEV) for a in ([0, 100, 170], [300, 230]))
+    word = torch.zeros(1, dtype=torch.int32, device=DEV)
+    args = mp.Kv8PrefillArgs(q=q.data_ptr(), out=out.data_ptr(), q_stride=q.stride(0), out_stride=out.stride(0),
+                             tables=tables.data_ptr(), row_offsets=off.data_ptr(), starts=first.data_ptr(),
+                             workspace=workspace.data_ptr(), workspace_bytes=workspace.numel(),
+                             type=list(DTYPES).index(dtype), heads=heads, table_stride=tables.stride(0), count=2, rows=170,
+                             scale=dim ** -0.5)
+    for _ in range(3):
+        begin, end = (torch.cuda.Event(enable_timing=True) for _ in range(2))
+        mp.kv8_inject_wait_timeout(1000)
+        begin.record()
+        mp.kv8_attention_prefill(cache.c, args, word.data_ptr(), stream())
+        end.record()
+        assert mp.kv8_status(word.data_ptr(), stream()) == mp.MP_ERR_TIMEOUT
+        assert begin.elapsed_time(end) < 500  # ms: not the 2 s of other calls
+        workspace.zero_()
+        mp.kv8_attention_prefill(cache.c, args, word.data_ptr(), stream())
+        assert mp.kv8_status(word.data_ptr(), stream()) == mp.MP_OK
+        for part, i, n in ((slice(0, 100), 0, 400), (slice(100, 170), 1, 300)):
+            check_rows(cache, heads, q[part], out[part], tables[i].tolist(), n, dim ** -0.5, dtype == "bf16")

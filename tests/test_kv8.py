@@ -160,3 +160,10 @@ def test_reference_rounding_and_scales(fmt):
 @pytest.mark.parametrize("op", list(CALLS))
 def test_tables_beyond_the_index_range_are_refused(built, op):
     refused(op, mp.MP_ERR_INVALID, table_stride=(1 << 26) // 16 + 1)
+
+
+@pytest.mark.parametrize("wait_us", [0, -1, 1000001])
+def test_wait_limits_out_of_range_are_refused(built, wait_us):
+    with pytest.raises(mp.DeviceError) as e:
+        mp.kv8_inject_wait_timeout(wait_us)
+    assert e.value.code == mp.MP_ERR_INVALID

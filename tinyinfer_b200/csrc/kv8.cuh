@@ -51,6 +51,7 @@ struct AttentionParams {
     int sequences;  // launch_packed: of the prefill; count is its rows
     float scale;
     unsigned* error;
+    unsigned stall_ns;  // failure-path tests: the prefill kernel's V tiles never come, and its waits end after this (0: none)
 };
 
 cudaError_t launch_append(const AppendParams& p, int type, int format, int head_dim, cudaStream_t stream);

@@ -1,11 +1,15 @@
 // Entry points of the 8-bit paged K/V cache operators: argument checks, then one
 // launch on the caller's stream. Nothing here allocates, copies or synchronises
 // (mp_kv8_status alone synchronises).
+#include <atomic>
+
 #include "kv8.cuh"
 
 namespace {
 
 using namespace mpb;
+
+std::atomic<unsigned> stall_next_ns{0};  // mp_kv8_inject_wait_timeout
 
 int refuse(int code, const char* message) {
     set_last_error(message);
@@ -191,7 +195,14 @@ extern "C" int mp_kv8_attention_prefill(const mp_kv8_cache* cache, const mp_kv8_
     p.heads = a->heads, p.table_stride = a->table_stride, p.count = a->count, p.rows = a->rows;
     p.scale = a->scale;
     p.error = device_error;
+    p.stall_ns = stall_next_ns.exchange(0, std::memory_order_relaxed);
     return finish(kv8::launch_prefill(p, a->type, cache->format, cache->head_dim, static_cast<cudaStream_t>(stream)));
+}
+
+extern "C" int mp_kv8_inject_wait_timeout(int32_t wait_us) {
+    if (wait_us < 1 || wait_us > 1000000) return refuse(MP_ERR_INVALID, "kv8: wait limit must be 1 us .. 1 s");
+    stall_next_ns.store(unsigned(wait_us) * 1000u, std::memory_order_relaxed);
+    return MP_OK;
 }
 
 extern "C" int mp_kv8_status(uint32_t* device_error, void* stream_ptr) {

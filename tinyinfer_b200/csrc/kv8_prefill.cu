@@ -321,6 +321,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_kernel(const AttentionPar
     uint64_t* done = bars + 25;                              // a segment's products
     uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(bars + 26);
     int* failed = reinterpret_cast<int*>(bars + 27);
+    uint64_t* drained = bars + 29;                           // products in flight after a wait that expired
     int* last = reinterpret_cast<int*>(bars + 28);  // [2] whether this CTA joins the parts, per tile
     int64_t* units_before = reinterpret_cast<int64_t*>(sm + S::kPlan);       // [kThreads + 1]
     int64_t* sums = units_before + kThreads + 1;                         // [32], [32]
@@ -337,7 +338,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_kernel(const AttentionPar
         }
         for (int i = 0; i < S::kBuffers; ++i) mbar_init(s_full + i, 1);
         for (int i = 0; i < kScaleSlots; ++i) mbar_init(scales_full + i, 1);
-        mbar_init(done, 1);
+        mbar_init(done, 1), mbar_init(drained, 1);
         *failed = 0;
         fence_barrier_init();
     }
@@ -452,8 +453,8 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_kernel(const AttentionPar
     auto wait_one = [&](uint64_t* bar, uint32_t parity) {
         for (int i = 0; i < 64; ++i)  // before the clock is read, which takes longer than most waits
             if (mbar_try_wait(bar, parity)) return true;
-        const uint64_t start = global_ns();
-        while (!*reinterpret_cast<volatile int*>(failed) && global_ns() - start < kWaitNanoseconds)
+        const uint64_t start = global_ns(), limit = p.stall_ns ? p.stall_ns : kWaitNanoseconds;
+        while (!*reinterpret_cast<volatile int*>(failed) && global_ns() - start < limit)
             if (mbar_try_wait(bar, parity)) return true;
         *reinterpret_cast<volatile int*>(failed) = 1;
         raise_error(p.error, kErrTimeout);
@@ -893,7 +894,8 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_kernel(const AttentionPar
                 if (t == 0) mbar_arrive(scales_full + slot % kScaleSlots);
 #pragma unroll
                 for (int part = 0; part < 2; ++part) {
-                    if (!(ok = wait((part ? v_empty : k_empty) + stage, parity))) break;
+                    if (part && p.stall_ns) ok = false;
+                    if (!ok || !(ok = wait((part ? v_empty : k_empty) + stage, parity))) break;
                     if (part) wait_copies<2 * S::kRing - 1>();
                     unsigned char* tile = sm + (part ? S::kV : S::kK) + stage * S::kTileBytes;
 #pragma unroll
@@ -1003,6 +1005,11 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_kernel(const AttentionPar
     tmem_fence_before();
     __syncthreads();
     if (warp == kProductWarp) {
+        if (*failed) {  // the roles left in mid-work: products may still be using the tiles and tensor memory
+            if (elect()) mma_commit(drained);
+            __syncwarp();
+            mbar_wait_bounded(drained, 0);
+        }
         tmem_fence_after();
         tmem_dealloc(tmem, S::kTmemCols);
     }

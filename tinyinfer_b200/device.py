@@ -152,6 +152,7 @@ def library() -> C.CDLL:
             getattr(lib, name).argtypes = [C.POINTER(Kv8Cache), C.c_int32]
             getattr(lib, name).restype = C.c_size_t
         lib.mp_kv8_status.argtypes = [C.c_void_p, C.c_void_p]
+        lib.mp_kv8_inject_wait_timeout.argtypes = [C.c_int32]
         _lib = lib
     return _lib
 
@@ -406,3 +407,8 @@ def kv8_prefill_workspace(cache: Kv8Cache, heads: int) -> int:
 def kv8_status(device_error: int, stream: int | None = None) -> int:
     """Synchronises `stream`, reads and clears the error word: an MP_* code (see mp_kv8_status)."""
     return library().mp_kv8_status(device_error, stream)
+
+
+def kv8_inject_wait_timeout(wait_us: int) -> None:
+    """Failure-path tests: the next prefill attention's bounded waits run out (see mp_kv8_inject_wait_timeout)."""
+    check(library().mp_kv8_inject_wait_timeout(wait_us))
