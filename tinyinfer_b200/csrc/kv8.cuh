@@ -101,9 +101,10 @@ __device__ __forceinline__ int block_id(const Cache& c, const int32_t* table, in
 }
 
 // Rows of a sequence at row_offsets begin .. end of a call with `rows` packed ones, 0 if its metadata is out
-// of range: offsets that fall or leave the call's rows, or positions outside 0 .. limit - 1.
-__device__ __forceinline__ int checked_rows(int begin, int end, int start, int rows, int64_t limit, unsigned* error) {
-    if (begin < 0 || end < begin || end > rows || (end > begin && start < 0) || int64_t(start) + (end - begin) > limit) {
+// of range: offsets that fall or leave the call's rows, or positions past the `pages` times `tokens` there are.
+__device__ __forceinline__ int checked_rows(int begin, int end, int start, int rows, int pages, int tokens, unsigned* error) {
+    if (begin < 0 || end < begin || end > rows || (end > begin && start < 0) ||
+        int64_t(start) + (end - begin) > int64_t(pages) * tokens) {
         if (end != begin) raise_error(error, kErrBounds);
         return 0;
     }
@@ -113,7 +114,7 @@ __device__ __forceinline__ int checked_rows(int begin, int end, int start, int r
 // Rows of a prefill's sequence i.
 __device__ __forceinline__ int sequence_rows(const AttentionParams& p, int i, int& begin, int& start) {
     begin = p.row_offsets[i], start = p.starts[i];
-    return checked_rows(begin, p.row_offsets[i + 1], start, p.rows, int64_t(p.table_stride) * p.cache.block_tokens, p.error);
+    return checked_rows(begin, p.row_offsets[i + 1], start, p.rows, p.table_stride, p.cache.block_tokens, p.error);
 }
 
 // 2^x as a float, x in -126 .. 127.

@@ -331,10 +331,10 @@ struct Place {
     int seq, position, end;  // end: the sequence's last row + 1
 };
 
-// Positions that a sequence may have: those of its table and of the rotation tables.
-__device__ __forceinline__ int64_t position_limit(const AppendParams& p) {
-    const int64_t tokens = int64_t(p.table_stride) * p.cache.block_tokens;
-    return p.rotary_dim ? min(tokens, int64_t(p.max_positions)) : tokens;
+// Positions that a sequence may have: those of its table (at most kMostTokens) and of the rotation tables.
+__device__ __forceinline__ int position_limit(const AppendParams& p) {
+    const int tokens = p.table_stride * p.cache.block_tokens;
+    return p.rotary_dim ? min(tokens, p.max_positions) : tokens;
 }
 
 // By one warp, a row per lane from `row0` on (rows <= 32): a row's sequence is the first that
@@ -360,7 +360,7 @@ __device__ __forceinline__ Place find_rows(const AppendParams& p, int row0, int 
     while (low < p.count && (end = p.row_offsets[low + 1]) <= row) ++low;
     if (low >= p.count) return {-1, 0, 0};
     const int begin = p.row_offsets[low], start = low == guess ? start_there : p.starts[low];
-    if (row < begin || checked_rows(begin, end, start, p.rows, position_limit(p), nullptr) == 0) return {-1, 0, 0};
+    if (row < begin || checked_rows(begin, end, start, p.rows, position_limit(p), 1, nullptr) == 0) return {-1, 0, 0};
     return {low, start + row - begin, end};
 }
 
@@ -374,9 +374,6 @@ __global__ void __launch_bounds__(kThreads, kThreads == 128 ? 5 : 2) append_kern
     if (warp == 0) {
         const Place at = find_rows(p, row0, rows, lane);
         if (lane < rows) places[lane] = at;
-    } else if (blockIdx.y == 0) {  // meanwhile: sequences that are out of range report themselves
-        for (int i = blockIdx.x * (kThreads - 32) + tid - 32; i < p.count; i += gridDim.x * (kThreads - 32))
-            checked_rows(p.row_offsets[i], p.row_offsets[i + 1], p.starts[i], p.rows, position_limit(p), p.error);
     }
     __syncthreads();
     // ---- tiles of the blocks whose first appended row is here
@@ -398,6 +395,10 @@ __global__ void __launch_bounds__(kThreads, kThreads == 128 ? 5 : 2) append_kern
         }
         turn -= tiles;
     }
+    // ---- sequences that are out of range report themselves (here: before the tiles, beside the search for
+    // the rows, this cost 8192 rows of 32 / 8 heads x 128 FP32 30 %)
+    for (int i = blockIdx.x * kThreads + tid; blockIdx.y == 0 && i < p.count; i += gridDim.x * kThreads)
+        checked_rows(p.row_offsets[i], p.row_offsets[i + 1], p.starts[i], p.rows, position_limit(p), 1, p.error);
     // ---- q: a chunk of a head of a row per thread, kFly of them in flight
     if (!p.q || blockIdx.y + 1 != gridDim.y) return;
     constexpr int kFly = kThreads == 128 ? 8 : 4;  // 20447 rows: 136 us with 4, 128 with 8; 256 single rows: 5.1 and 5.4
