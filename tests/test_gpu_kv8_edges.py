@@ -128,6 +128,26 @@ def test_long_bf16_decode_does_not_fade(built):
         assert bool(((out[i].double() - want.view(-1)).abs() <= 0.25 + weight.view(-1) * 2 ** -13).all())
 
 
+@pytest.mark.parametrize("dim,heads,kv_heads", [(64, 9, 3), (128, 8, 2)])
+def test_short_contexts_in_long_tables(built, dim, heads, kv_heads):
+    """Tables that could hold more than a chain of sums (32768 tokens) beside ones that could not: the same outputs."""
+    counts, starts = [70, 0, 130, 9], [500, 3, 0, 1200]
+    lengths = [s + c if c else 0 for s, c in zip(starts, counts)]
+    cache = Cache(sum(-(-n // 16) for n in lengths), kv_heads, dim, 16, "int8")
+    outs = []
+    for spare in (0, 2049):
+        tables = tables_for(lengths, 16, cache.c.max_blocks, 102, spare=spare)
+        fill(cache, tables, lengths, 103)
+        q, out = prefill(cache, heads, tables, counts, starts, "bf16")
+        outs.append(out)
+        at = 0
+        for i, (c, n) in enumerate(zip(counts, lengths)):
+            if c:
+                check_rows(cache, heads, q[at: at + c], out[at: at + c], tables[i].tolist(), n, dim ** -0.5, True)
+            at += c
+    assert torch.equal(*outs)
+
+
 @pytest.mark.parametrize("rows", [10, 900])
 @pytest.mark.parametrize("fault", ["table", "rotation", "rows", "order"])
 def test_append_leaves_a_bad_sequence_out(built, fault, rows):

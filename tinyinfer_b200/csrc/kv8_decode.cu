@@ -375,6 +375,7 @@ __global__ void __launch_bounds__(warps_of<T, D>() * 32, 1)
                 } else {
                     w.template step<true>(load_k, load_v, scale, len - unit * kUnit, lane);
                 }
+                if (!WarpRow<T, F, D>::kSplit && (unit + 1) % WarpRow<T, F, D>::kChain == 0) w.close();
                 __syncwarp();
                 issue(stage);
                 if (++stage == lay.stages) stage = 0;

@@ -306,7 +306,8 @@ struct RunCursor {
     }
 };
 
-template <class T, int F, int D>
+// kLong: BF16 outputs of contexts that may pass one chain (launch_prefill)
+template <class T, int F, int D, bool kLong>
 __global__ void __launch_bounds__(kThreads, 1) prefill_kernel(const AttentionParams p) {
     using S = Shape<T, D>;
     using Cursor = RunCursor<S::kAloneCost>;
@@ -722,7 +723,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_kernel(const AttentionPar
                 if (!ok || !wait_outputs()) break;
                 if (S::kAdd && j) add_outputs(moved);
                 tmem_wait_store();
-                if (!S::kAdd && j && j % kChainTiles == 0) end_chain(j == kChainTiles);
+                if (kLong && j && j % kChainTiles == 0) end_chain(j == kChainTiles);
                 tmem_fence_before();
                 arrive(p_full + w);
             }
@@ -736,7 +737,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_kernel(const AttentionPar
             slot += most;
             if (!ok) break;
             const float u = pow2(unit_log - kTopLog);
-            if (!S::kAdd && tiles > kChainTiles) {
+            if (kLong && tiles > kChainTiles) {
                 const float* mine = part(blockIdx.x, seg.k0 == 0) + v * 4;
                 const float by = (chain_m == m ? 1.f : ex2(chain_m - m)) / u;
 #pragma unroll
@@ -956,7 +957,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_kernel(const AttentionPar
                         tmem_fence_after();
                         const uint32_t s_at = tmem + place * kN, o_at = tmem + S::kBuffers * kN + o.w * D;
                         const uint64_t vd = v_desc + uint64_t(stage * (S::kTileBytes >> 4));
-                        const bool keep = !S::kAdd && o.j % kChainTiles != 0, leave = o.w || o.j >= n1;  // leave: V's last use
+                        const bool keep = !S::kAdd && (kLong ? o.j % kChainTiles : o.j) != 0, leave = o.w || o.j >= n1;  // leave: V's last use
                         if (elect()) {
 #pragma unroll
                             for (int half = kHalves - 1; half >= 0; --half)
@@ -1031,11 +1032,21 @@ cudaError_t launch_prefill(const AttentionParams& p, int type, int format, int h
     if (int64_t(p.rows) * p.cache.kv_heads * ((p.heads / p.cache.kv_heads + 7) / 8) <= kPackedItems)
         return launch_packed(p, type, format, head_dim, stream);
     return dispatch(type, format, head_dim, [&](auto t, auto f, auto d) {
-        using S = Shape<decltype(t), decltype(d)::value>;
-        auto kernel = prefill_kernel<decltype(t), decltype(f)::value, decltype(d)::value>;
-        const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kAlloc);
-        if (e != cudaSuccess) return e;
-        return launch_pdl(kernel, dim3(kCtas), dim3(kThreads), S::kAlloc, stream, p);
+        using T = decltype(t);
+        constexpr int kFormat = decltype(f)::value, kDim = decltype(d)::value;
+        using S = Shape<T, kDim>;
+        auto launch = [&](auto kernel) {
+            const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kAlloc);
+            if (e != cudaSuccess) return e;
+            return launch_pdl(kernel, dim3(kCtas), dim3(kThreads), S::kAlloc, stream, p);
+        };
+        // Ending chains takes registers from the loop over tiles (BF16: 16 x 512 rows of 9 / 3 heads x 64 at position
+        // 3584 200 us, 185 without; 8 x 1024 of 32 / 8 heads x 128 at 1000 387, 380): tables that cannot hold a
+        // context longer than a chain go without.
+        if constexpr (!S::kAdd)
+            if (int64_t(p.table_stride) * p.cache.block_tokens > int64_t(kChainTiles) * kN)
+                return launch(prefill_kernel<T, kFormat, kDim, true>);
+        return launch(prefill_kernel<T, kFormat, kDim, false>);
     });
 }
 

@@ -45,7 +45,7 @@ template <class T, int F, int D>
 struct WarpRow {
     static constexpr int kHalves = D / 64;
     static constexpr bool kSplit = sizeof(T) == 4;  // BF16 outputs: weights as one FP16 half (2^-12 relative)
-    static constexpr int kChain = kSplit ? 4 : 1024;  // units per chain of tensor-op sums
+    static constexpr int kChain = kSplit ? 4 : 1024;  // units per chain of tensor-op sums (the caller ends BF16's)
     uint32_t qa[D / 16][4];
     // outputs: lane (n, c) holds head n's dims 16 i / 2 + 4 c + i % 2 + {0, 2} in o[i][0, 1]
     // (weights' hi halves) and o[i][2, 3] (lo; BF16: finished chains, to which the products add zeros)
@@ -183,9 +183,11 @@ struct WarpRow {
                 }
             }
         }
-        if (++chain == kChain) {
-            close();
-            chain = 0;
+        if constexpr (kSplit) {
+            if (++chain == kChain) {
+                close();
+                chain = 0;
+            }
         }
     }
 
