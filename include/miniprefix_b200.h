@@ -258,7 +258,8 @@ int mp_paged_attention_status(void* stream);
  *   mp_kv8_attention_prefill  causal attention of packed chunks of rows.
  * A value is code * scale. Codes are INT8 (-127..127) or E4M3 (bytes of the 8-bit
  * float with 4 exponent and 3 mantissa bits, largest 448). The append chooses scales
- * that are powers of two; the attentions take any finite scale that is not negative.
+ * that are powers of two; the attentions take any finite scale that is not negative (a K scale
+ * times a row's largest |q| times |scale| has to stay in FP32's range).
  *
  * All arrays are device memory of the current device unless stated, and the metadata
  * (tables, lengths, row_offsets, starts) is read by the kernels only: no call copies
@@ -329,17 +330,17 @@ typedef struct {
     const void *q, *k, *v; /* q optional */
     void* q_out;           /* with q */
     int64_t q_stride, k_stride, v_stride, q_out_stride;
-    const float *cos, *sin;
+    const float *cos, *sin;     /* 16-byte aligned */
     const int32_t* tables;      /* [count][table_stride] block ids */
     const int32_t* row_offsets; /* [count + 1] */
     const int32_t* starts;      /* [count] */
     int32_t type;               /* MP_TYPE_* of q, k, v, q_out */
-    int32_t heads;              /* query heads, a multiple of kv_heads */
+    int32_t heads;              /* query heads: 1 .. 64 per kv head, at most 1024 */
     int32_t rotary_dim;         /* a multiple of 8, 0 .. head_dim */
     int32_t rope_layout;        /* MP_ROPE_* */
     int32_t max_positions;
     int32_t table_stride;       /* table_stride * block_tokens <= 2^26 */
-    int32_t count; /* 1 .. 65536 */
+    int32_t count;              /* 1 .. 65536 */
     int32_t rows;
 } mp_kv8_append_args;
 int mp_kv8_append(const mp_kv8_cache* cache, const mp_kv8_append_args* args, uint32_t* device_error, void* stream);
@@ -348,7 +349,10 @@ int mp_kv8_append(const mp_kv8_cache* cache, const mp_kv8_append_args* args, uin
  * query head h reading kv head h / (heads / kv_heads). A length of 0 gives a row of
  * zeros. Sums, maxima and weights are FP32; products run on the tensor cores as FP16
  * halves (FP32-level: the codes are exact in FP16, an FP32 query and weight is two
- * halves). The rows' tokens are cut into equal runs over the device and joined. */
+ * halves; of a BF16 call's weights the high half alone). Counted as zero are weights below
+ * 2^-126 of a row's largest, and weights times V scales below 2^-33 of the largest such
+ * product. The rows' tokens are cut into equal runs over the device and joined. The limits on
+ * heads, count and table_stride are the append's; rows are 16-byte aligned here, too. */
 typedef struct {
     const void* q;
     void* out;

@@ -7,22 +7,24 @@
 // A k code is the nearest multiple of the block's scale to the exact rotated value, so a
 // value next to the border of two codes must not be rounded on the way. The FP32 value
 // a c - (b s) is off by at most e = 2^-23 (|b s| + |value|), far below a code (|b s| is at most
-// the rotated pair's length); where value - e and value + e have the same code, that is the code. Where not (one value in some 10^4)
-// the lane computes its codes again in 64 bits, in which the products are exact; likewise
-// for the scale, and for tiles with values outside the range in which e holds. (Everything in
-// 64 bits measured 24 us for 8192 rows of 9 + 3 + 3 heads x 64 FP32, and 290 us for 20447 rows of
-// 32 + 8 + 8 heads x 128 BF16: its conversions bound it.)
+// the rotated pair's length); where value - e and value + e have the same code, that is the
+// code. Where not (one value in some 10^4) the lane computes its codes again in 64 bits, in
+// which the products are exact; likewise for the scale, and for tiles with values outside the
+// range in which e holds. (Everything in 64 bits measured 24 us for 8192 rows of 9 + 3 + 3 heads
+// x 64 FP32, and 290 us for 20447 rows of 32 + 8 + 8 heads x 128 BF16: its conversions bound it.)
 //
 // A CTA takes up to 8 packed rows: its warps write the tiles of the blocks that begin among
 // its rows (a tile's first appended row is in one CTA only), or all its threads rotate
-// their q; one CTA does both, or two share the rows (launch_append). A tile is (block, kv head, K or V); its scale needs the largest magnitude of all
-// its new tokens, so one warp takes it whole, 16 tokens (8 of head_dim 128) in registers at
-// a time, twice: magnitude, then codes. Fewer rows per CTA when there are few (one for a
-// decode step), so that all SMs take part.
+// their q; one CTA does both, or two share the rows (launch_append). A tile is (block, kv head,
+// K or V); its scale needs the largest magnitude of all its new tokens, so one warp takes it
+// whole, 16 tokens (8 of head_dim 128) in registers at a time, twice: magnitude, then codes.
+// Fewer rows per CTA when there are few (one for a decode step), so that all SMs take part.
 //
-// Measured: 8192 rows of 9 + 3 + 3 heads x 64 FP32 15.0 us (3.6 TB/s), 20447 of 32 + 8 + 8 heads x
-// 128 BF16 128 us (3.9 TB/s), 0.55 to 0.6 of the copy rate: a warp's loads, magnitude and codes
-// follow one another, and the 20 warps of an SM hide part of that.
+// Measured with buffers that pass through L2: 8192 rows of 9 + 3 + 3 heads x 64 FP32 17.8 us (3.1
+// TB/s; 15.4 where they stay in it), 20447 of 32 + 8 + 8 heads x 128 BF16 130 us (3.9 TB/s), 0.47
+// and 0.59 of the copy rate: a warp's loads, magnitude and codes follow one another, and the 20
+// warps of an SM hide part of that. Large blocks leave most warps without a tile: the 8192 rows
+// take 31 us with blocks of 64 tokens and 87 with 256.
 #include "kv8.cuh"
 
 namespace mpb {

@@ -7,16 +7,19 @@
 // long the sequences are, or a CTA takes an item whole. The lengths are device memory,
 // so every CTA adds them up itself (a block scan) and finds where its warps' runs begin.
 //
-// A warp is a pipeline of its own: a ring of units in shared memory that cp.async fills
-// (rows swizzled against bank conflicts) and the warp-level tensor ops of kv8_warp.cuh
-// empty. 16 warps keep up to 192 KB in flight per SM, and no two warps wait for one another
-// before the end. (The copy engine's tiles, issued by a lane, cost the warp more instructions
-// than 16-byte copies by all lanes: 74 us against 52 for 256 rows of 2048 tokens.)
+// A warp works on its own: cp.async fills its ring of 1 to 3 units in shared memory (rows
+// swizzled against bank conflicts), the warp-level tensor ops of kv8_warp.cuh empty it, and no
+// two warps wait for one another before the end. At head_dim 64 16 warps keep up to 192 KB in
+// flight per SM; FP32 at 128 has 8 warps with two units or more; BF16 at 128 12 warps, whose
+// partials leave room for one unit each from 3 query heads per kv head on: nothing is then in
+// flight while such a warp computes, the others cover for it. (The copy engine's tiles, issued by
+// a lane, cost the warp more instructions than 16-byte copies by all lanes: 74 us against 52 for
+// 256 rows of 2048 tokens.)
 //
-// Bound by instructions: about 480 a unit on a scheduler with 4 warps (2 or 3 for head_dim 128),
-// where the ring without arithmetic takes 40 us for 256 x 2048 tokens of 9 / 3 heads x 64; with it
-// 53 us in FP32 (3.8 TB/s), 48 in BF16. Wider heads come nearer to HBM: 64 x 4096 tokens of
-// 32 / 8 heads x 128 100 us (5.4 TB/s).
+// Bound by instructions at head_dim 64: about 480 a unit on a scheduler with 4 warps, where the
+// ring without arithmetic takes 40 us for 256 x 2048 tokens of 9 / 3 heads; with it 55 us in FP32
+// (3.7 TB/s), 49 in BF16. At 128, 64 x 4096 tokens of 32 / 8 heads take 101 us in FP32 (5.3 TB/s),
+// nearer to HBM, and 110 in BF16 (4.9 TB/s), with the one-unit rings.
 //
 // An item that ends in a later run leaves partials (max, sum, outputs): a CTA's warps join theirs
 // through shared memory, CTAs through the workspace: the last CTA to arrive on the counter of

@@ -4,8 +4,9 @@
 // A work item is (block of rows of one sequence, kv head): rows x query heads of the group
 // fill two 128-vector tiles (vector v of a tile: row v / group, head v % group), and its
 // context is a run of 128-token K/V tiles. All items' tiles, in order, are dealt out in
-// runs of equal cost to one CTA per SM (an item's queries and outputs count too), so a long context with few rows is shared like many short ones; the device plans
-// this itself from row_offsets and starts.
+// runs of equal cost to one CTA per SM (an item's queries and outputs count too), so a long
+// context with few rows is shared like many short ones; the device plans this itself from
+// row_offsets and starts.
 //
 // Calls with few rows go to kv8_decode.cu's kernel (launch_prefill below).
 //
@@ -34,10 +35,10 @@
 // first.
 //
 // Bound by the softmax's chain of instructions: of the 6100 cycles that 256 vectors x 128 tokens
-// take in FP32 at head_dim 64 (16 x 512 rows of 9 / 3 heads at position 3584: 243 us), a thread
+// take in FP32 at head_dim 64 (16 x 512 rows of 9 / 3 heads at position 3584: 246 us), a thread
 // spends 900 on the maximum, 2900 on the weights, 640 on O and 700 waiting; an item's start and
 // end cost 700 more per tile. exp2 alone would take 2050, the products 2050 (3100 measured: P V is
-// 64 wide). At head_dim 128 BF16 (8 x 1024 rows of 32 / 8 heads at position 1000: 377 us, 538
+// 64 wide). At head_dim 128 BF16 (8 x 1024 rows of 32 / 8 heads at position 1000: 380 us, 534
 // TFLOP/s) it is 8000 cycles: 3600 of softmax, 2800 of waiting for S, whose place is free only after
 // the tile's own P V, 1500 of items' starts and ends.
 #include <algorithm>
@@ -1025,8 +1026,8 @@ size_t prefill_workspace(int group, int head_dim) {
 cudaError_t launch_prefill(const AttentionParams& p, int type, int format, int head_dim, cudaStream_t stream) {
     // Few rows go one by one, as decode's do, while there is an SM for each (row, kv head, 8 query
     // heads): their tokens are read once per row, but no tile of vectors has to be filled. 9 / 3
-    // heads, FP32, beside the tiles: 37 rows 7.4 us against 13.4 (at position 500 11.5 / 19.8);
-    // 49 rows 8.0 / 14.8, at 2000 17.0 / 30.0, at 16000 62.7 / 67.9. Twice as many would
+    // heads, FP32, beside the tiles: 37 rows 7.6 us against 13.4 (at position 500 11.6 / 19.8);
+    // 49 rows 8.0 / 14.8, at 2000 17.0 / 30.0, at 16000 63 / 67.9. Twice as many would
     // still gain a little on short contexts (98 rows 14.6 / 15.0, at 2000 27.2 / 31.6), and lose
     // on long ones, where the time is the tokens that an SM passes over.
     if (int64_t(p.rows) * p.cache.kv_heads * ((p.heads / p.cache.kv_heads + 7) / 8) <= kPackedItems)

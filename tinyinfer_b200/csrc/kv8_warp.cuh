@@ -20,11 +20,12 @@
 // (2048 tiles, at most 2.4e-4) for BF16 ones, which came out 6e-3 small after one chain of 2^20.
 //
 // The state is a running softmax: m (the reference score), l (sum of weights), and outputs
-// in units of `unit`, a power of two at most the largest weight times scale so far, so that
-// the weights fill FP16's range. FP16 has room for weights 2^7 times 2^8 (`unit` is below the
-// largest by up to 2), so m and unit move only when a score passes m by 6 (in powers of
-// two) or a scale reaches twice the unit: moving them every time that the maximum grew cost a
-// fifth of the instructions. FP16's smallest half step, 2^-25, is 2^-33 of the largest.
+// in units of `unit`, a power of two at most the largest weight times scale so far (but see
+// kUnitFloor and kScaleFloor), so that the weights fill FP16's range. FP16 has room for weights
+// 2^7 times 2^8 (`unit` is below the largest by up to 2), so m and unit move only when a score
+// passes m by 6 (in powers of two) or a scale reaches twice the unit: moving them every time that
+// the maximum grew cost a fifth of the instructions. FP16's smallest half step, 2^-25, is 2^-33
+// of the largest.
 #pragma once
 #include "kv8.cuh"
 
@@ -88,10 +89,10 @@ struct WarpRow {
     }
 
     // One unit. load_k(u, i, h): the 16-byte word c of 64-byte half h of token(i, n)'s row in
-    // tile u (bytes behind the last token may be NaN codes: they become zero); load_v(u, q, r): dims 32 q .. 32 q + 31 of V's tile u as four transposed
-    // matrices, r[2 a + i] = chunk 2 q + a of the tokens of half i; scale[u]: the K and V
-    // scales. kLast: tokens at or past `valid` (1 .. 32) are masked (a tile without tokens
-    // has scales 0); else all 32 are there.
+    // tile u (bytes behind the last token may be NaN codes: they become zero); load_v(u, q, r):
+    // dims 32 q .. 32 q + 31 of V's tile u as four transposed matrices, r[2 a + i] = chunk 2 q + a
+    // of the tokens of half i; scale[u]: the K and V scales. kLast: tokens at or past `valid`
+    // (1 .. 32) are masked (a tile without tokens has scales 0); else all 32 are there.
     template <bool kLast, class LoadK, class LoadV>
     __device__ __forceinline__ void step(LoadK load_k, LoadV load_v, const float2 (&scale)[kTiles], int valid, int lane) {
         const int n = lane >> 2, c = lane & 3;
