@@ -240,3 +240,29 @@ def test_prefill_waits_that_run_out(built, heads, kv_heads, dim, dtype):
         assert mp.kv8_status(word.data_ptr(), stream()) == mp.MP_OK
         for part, i, n in ((slice(0, 100), 0, 400), (slice(100, 170), 1, 300)):
             check_rows(cache, heads, q[part], out[part], tables[i].tolist(), n, dim ** -0.5, dtype == "bf16")
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("dim,heads,kv_heads", [(64, 9, 3), (128, 8, 2)])
+def test_queries_that_are_not_finite_stay_alone(built, dim, heads, kv_heads, dtype):
+    """A NaN or an infinity in one row's head makes that output NaN and no other; decode, row by row and as tiles."""
+    n = 400
+    cache = Cache(n // 16, kv_heads, dim, 16, "int8")
+    tables = tables_for([n], 16, n // 16, 104)
+    fill(cache, tables, [n], 105)
+    for rows in (5, 100):
+        q = values(rows, heads * dim, 106).to(DTYPES[dtype]).view(rows, heads, dim)
+        q[1, 2, 7], q[3, 0, 0], q[rows - 1, heads - 1, dim - 1] = float("nan"), float("inf"), -float("inf")
+        bad = ~torch.isfinite(q).all(-1)
+        good = torch.where(bad[..., None], torch.zeros_like(q), q)
+        want, weight, size, top = ref.attend(good, cache.pages, cache.scales, "int8", tables[0].tolist(), n, dim ** -0.5)
+        limit = ref.bound(want, weight, size, top, n, dim, dtype == "bf16")
+        _, out = prefill(cache, heads, tables, [rows], [n - rows], dtype, q=q.flatten(1))
+        outs = [out]
+        if rows == 5:
+            lengths = [n - rows + 1 + i for i in range(rows)]
+            outs.append(decode(cache, heads, tables.repeat(rows, 1).contiguous(), lengths, dtype, q=q.flatten(1))[1])
+        for out in outs:
+            out = out.view(rows, heads, dim)
+            assert bool(torch.isnan(out[bad]).all())
+            assert bool(((out[~bad].double() - want[~bad]).abs() <= limit[~bad]).all())

@@ -5,7 +5,9 @@ import random
 import pytest
 import torch
 
-from test_gpu_kv8 import DEV, Appender, Cache, check_prefill, fill, tables_for, values
+import kv8_reference as ref
+from test_gpu_kv8 import DEV, Appender, Cache, check_prefill, check_rows, decode, fill, stream, tables_for, values
+from tinyinfer_b200 import device as mp
 
 pytestmark = pytest.mark.gpu
 
@@ -46,3 +48,62 @@ def test_prefill_many_heads_per_kv_head(built, heads, kv_heads, dim, dtype):
     lengths = [s + c if c else 0 for s, c in zip(starts, counts)]
     cache = Cache(sum(-(-n // 16) for n in lengths), kv_heads, dim, 16, "int8")
     check_prefill(cache, heads, tables_for(lengths, 16, cache.c.max_blocks, 113), counts, starts, dtype)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("heads,kv_heads,dim", [(256, 256, 64), (1024, 256, 128), (1024, 16, 64)])
+def test_largest_head_counts(built, heads, kv_heads, dim, dtype):
+    counts, starts = [3, 0, 21], [30, 0, 2]
+    lengths = [s + c if c else 0 for s, c in zip(starts, counts)]
+    cache = Cache(sum(-(-n // 16) for n in lengths), kv_heads, dim, 16, "e4m3")
+    tables = tables_for(lengths, 16, cache.c.max_blocks, 114)
+    check_prefill(cache, heads, tables, counts, starts, dtype)
+    q, out = decode(cache, heads, tables, lengths, dtype)
+    for i, n in enumerate(lengths):
+        if n:
+            check_rows(cache, heads, q[i: i + 1], out[i: i + 1], tables[i].tolist(), n, dim ** -0.5, dtype == "bf16")
+    run = Appender(cache, heads, dtype, dim, "half", 64)
+    run(tables, [1, 0, 2], [32, 0, 14], values(3, (heads + 2 * kv_heads) * dim, 115))
+
+
+def test_largest_count(built):
+    """65536 sequences of 0 to 17 tokens or rows; every operator, checked at some of them."""
+    n, heads, kv_heads, dim = 65536, 2, 1, 64
+    r = random.Random(116)
+    lengths = [r.choice([0, 1, 1, 2, 17]) for _ in range(n)]
+    cache = Cache(sum(-(-x // 16) for x in lengths), kv_heads, dim, 16, "int8")
+    tables = tables_for(lengths, 16, cache.c.max_blocks, 117, spare=0)
+    total = sum(lengths)
+    run = Appender(cache, heads, "f32", dim, "half", 32)
+    qkv = values(total, (heads + 2 * kv_heads) * dim, 118)
+    q_out = torch.full((total, heads * dim), 7.0, device=DEV)
+    offsets = [0]
+    for x in lengths:
+        offsets.append(offsets[-1] + x)
+    off, first = torch.tensor(offsets, dtype=torch.int32, device=DEV), torch.zeros(n, dtype=torch.int32, device=DEV)
+    mp.kv8_append(cache.c, run.args(qkv, q_out, tables, off, first), run.error.data_ptr(), stream())
+    out = torch.full((total, heads * dim), 7.0, device=DEV)
+    workspace = torch.zeros(mp.kv8_prefill_workspace(cache.c, heads), dtype=torch.uint8, device=DEV)
+    common = dict(tables=tables.data_ptr(), workspace=workspace.data_ptr(), workspace_bytes=workspace.numel(), type=0,
+                  heads=heads, table_stride=tables.stride(0), count=n, scale=0.125, q_stride=heads * dim,
+                  out_stride=heads * dim)
+    mp.kv8_attention_prefill(cache.c, mp.Kv8PrefillArgs(q=q_out.data_ptr(), out=out.data_ptr(), row_offsets=off.data_ptr(),
+                             starts=first.data_ptr(), rows=total, **common), run.error.data_ptr(), stream())
+    q, last = values(n, heads * dim, 119), torch.full((n, heads * dim), 7.0, device=DEV)
+    lens = torch.tensor(lengths, dtype=torch.int32, device=DEV)
+    mp.kv8_attention_decode(cache.c, mp.Kv8DecodeArgs(q=q.data_ptr(), out=last.data_ptr(), lengths=lens.data_ptr(), **common),
+                            run.error.data_ptr(), stream())
+    assert mp.kv8_status(run.error.data_ptr(), stream()) == mp.MP_OK
+    assert bool((last[lens == 0] == 0).all())
+    for i in [0, 1, 511, 512, n - 1] + [r.randrange(n) for _ in range(60)]:
+        x, at = lengths[i], offsets[i]
+        if not x:
+            continue
+        pages, scales = cache.store[:, 0].clone(), cache.scale_store[:, 0].clone()
+        y, pos = qkv[at: at + x].double(), torch.arange(x, device=DEV)
+        c, s = run.cos[pos].double(), run.sin[pos].double()
+        k = ref.rotate(y[:, heads * dim: (heads + 1) * dim].reshape(x, 1, dim), c, s, dim, "half")
+        ref.append(pages, scales, "int8", k, y[:, (heads + 1) * dim:].reshape(x, 1, dim), [tables[i].tolist()], [0, x], [0])
+        assert torch.equal(pages, cache.store[:, 0]) and torch.equal(scales.view(torch.int32), cache.scale_store[:, 0].view(torch.int32))
+        check_rows(cache, heads, q_out[at: at + x], out[at: at + x], tables[i].tolist(), x, 0.125, False)
+        check_rows(cache, heads, q[i: i + 1], last[i: i + 1], tables[i].tolist(), x, 0.125, False)
