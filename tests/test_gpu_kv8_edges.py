@@ -148,6 +148,32 @@ def test_short_contexts_in_long_tables(built, dim, heads, kv_heads):
     assert torch.equal(*outs)
 
 
+@pytest.mark.parametrize("log2n", [17, 20])
+@pytest.mark.parametrize("dim", [64, 128])
+def test_long_sums_of_like_weights(built, dim, log2n):
+    """FP32 rows over 2^17 and 2^20 tokens of one value, all but the first of one weight: a sum that is rounded n times
+    on its way up is off by at most n / 2 times 2^-24 of it, all errors alike, and the outputs' chains and the
+    normaliser have n = tokens / 128 such sums each (2^-18: those within a chain, and the halves)."""
+    n = 1 << log2n
+    cache = Cache(n // 256, 1, dim, 256, "int8")
+    table = tables_for([n], 256, n // 256, 107, spare=0)
+    cache.pages.zero_()
+    cache.pages[:, :, 0, :, 0] = -1
+    cache.pages[int(table[0, 0]), 0, 0, 0, 0] = 0
+    cache.pages[:, :, 1], cache.scales[...] = 100, 2.0 ** -6
+    limit = 100 * 2.0 ** -6 * (n / 128 * 2.0 ** -24 + 2.0 ** -18)
+    for weight in (0.7, 0.61, 0.9, 0.53):
+        rows = 148 * (16 if dim == 64 else 8)  # a row per warp
+        q = torch.zeros(rows, dim, device=DEV)
+        q[:, 0] = -math.log(weight) * 2.0 ** 6 * dim ** 0.5
+        _, out = decode(cache, 1, table.repeat(rows, 1).contiguous(), [n] * rows, "f32", q=q)
+        assert float((out.double() - 100 * 2.0 ** -6).abs().max()) <= limit
+        count = 152  # items enough that none is cut
+        q = q[:1].repeat(256 * count, 1)
+        _, out = prefill(cache, 1, table.repeat(count, 1).contiguous(), [256] * count, [n - 256] * count, "f32", q=q)
+        assert float((out.double() - 100 * 2.0 ** -6).abs().max()) <= limit
+
+
 @pytest.mark.parametrize("rows", [10, 900])
 @pytest.mark.parametrize("fault", ["table", "rotation", "rows", "order"])
 def test_append_leaves_a_bad_sequence_out(built, fault, rows):

@@ -681,6 +681,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_kernel(const AttentionPar
                     const float unit = pow2(unit_log);
                     [[maybe_unused]] const Pair minus_one = pair(-1.f, -1.f);
                     const float least = fmaxf(unit * 8.6736174e-19f, 1.17549435e-38f);
+                    float tile_l = 0.f;  // the tile's weights first: fewer additions to a long sum
                     each_group(Some{}, [&](float (&x)[16], int g) {
                         const float4 sc = scale[g];
                         const bool small = sc.y < least;
@@ -709,11 +710,12 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_kernel(const AttentionPar
                             }
                         }
                         const float2 both = unpair(sum);
-                        l = fmaf(both.x + both.y, kCut && g * 16 >= visible ? 0.f : back, l);
+                        tile_l = fmaf(both.x + both.y, kCut && g * 16 >= visible ? 0.f : back, tile_l);
                         // over the scores just read: 16 columns hold 8 of high halves, 8 of low
                         tmem_store8(s_at + g * 16, hi);
                         if constexpr (kHalves == 2) tmem_store8(s_at + g * 16 + 8, lo);
                     });
+                    l += tile_l;
                 };
                 if (cut) {
                     weigh(std::true_type{});

@@ -18,6 +18,7 @@
 // (measured: 1.8e-5 after 1000 tiles; up to 2^-23). Outputs are therefore added up in chains of
 // kChain units, and the chains in FP32 registers: 128 tokens a chain for FP32 outputs, 32768
 // (2048 tiles, at most 2.4e-4) for BF16 ones, which came out 6e-3 small after one chain of 2^20.
+// The sum of weights goes by the same chains (in one, 2^20 weights of 0.7 were 1e-3 off).
 //
 // The state is a running softmax: m (the reference score), l (sum of weights), and outputs
 // in units of `unit`, a power of two at most the largest weight times scale so far (but see
@@ -52,7 +53,7 @@ struct WarpRow {
     // (weights' hi halves) and o[i][2, 3] (lo; BF16: finished chains, to which the products add zeros)
     float o[D / 8][4];
     float sum[kSplit ? D / 8 : 1][2];  // finished chains
-    float m, l, unit, inv_unit, k_factor;
+    float m, l, chain_l, unit, inv_unit, k_factor;  // chain_l: of the sum of weights, the chain's part
     int chain;
 
     // Token of column x of 8 in half `i` of a tile. 128-byte rows: columns 2i and 2i + 1 are
@@ -85,7 +86,7 @@ struct WarpRow {
         for (int i = 0; i < D / 8; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
 #pragma unroll
         for (int i = 0; i < (kSplit ? D / 8 : 1); ++i) sum[i][0] = sum[i][1] = 0.f;
-        m = -INFINITY, l = 0.f, unit = kUnitFloor, inv_unit = kWeightTop / kUnitFloor, chain = 0;
+        m = -INFINITY, l = chain_l = 0.f, unit = kUnitFloor, inv_unit = kWeightTop / kUnitFloor, chain = 0;
     }
 
     // One unit. load_k(u, i, h): the 16-byte word c of 64-byte half h of token(i, n)'s row in
@@ -156,7 +157,7 @@ struct WarpRow {
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
                 const float p0 = ex2(t[u][i][0] - base), p1 = ex2(t[u][i][1] - base);
-                l += p0 + p1;
+                chain_l += p0 + p1;
                 if constexpr (kSplit) {
                     split_pair(p0 * w, p1 * w, a[2 * i], a[2 * i + 1]);
                 } else {
@@ -210,7 +211,7 @@ struct WarpRow {
         const float largest = fminf(fmaxf(fmaxf(unit * decay, reach), kUnitFloor), 8.507059e37f);
         const int exponent = (__float_as_int(largest) >> 23) - 127;  // rounded down to a power of two
         const float by = decay * (unit * pow2(-exponent));
-        l *= decay;
+        l *= decay, chain_l *= decay;
 #pragma unroll
         for (int i = 0; i < D / 8; ++i) {
 #pragma unroll
@@ -222,6 +223,7 @@ struct WarpRow {
 
     // Ends a chain.
     __device__ __forceinline__ void close() {
+        l += chain_l, chain_l = 0.f;
 #pragma unroll
         for (int i = 0; i < D / 8; ++i) {
             if constexpr (kSplit) {
@@ -239,14 +241,14 @@ struct WarpRow {
     // Sum of weights over the head's lanes; o[i][0, 1] become the head's outputs in plain
     // units (unnormalised).
     __device__ __forceinline__ void end() {
+        close();
         l += __shfl_xor_sync(0xffffffffu, l, 1);
         l += __shfl_xor_sync(0xffffffffu, l, 2);
         const float u = unit * (1.f / kWeightTop);
-        if constexpr (kSplit) close();
 #pragma unroll
         for (int i = 0; i < D / 8; ++i) {
-            o[i][0] = (kSplit ? sum[i][0] : o[i][0] + o[i][2]) * u;
-            o[i][1] = (kSplit ? sum[i][1] : o[i][1] + o[i][3]) * u;
+            o[i][0] = (kSplit ? sum[i][0] : o[i][2]) * u;
+            o[i][1] = (kSplit ? sum[i][1] : o[i][3]) * u;
         }
     }
 
