@@ -18,7 +18,7 @@
 //
 // Bound by instructions at head_dim 64: about 480 a unit on a scheduler with 4 warps, where the
 // ring without arithmetic takes 40 us for 256 x 2048 tokens of 9 / 3 heads; with it 55 us in FP32
-// (3.7 TB/s), 49 in BF16. At 128, 64 x 4096 tokens of 32 / 8 heads take 101 us in FP32 (5.3 TB/s),
+// (3.7 TB/s), 50 in BF16. At 128, 64 x 4096 tokens of 32 / 8 heads take 102 us in FP32 (5.3 TB/s),
 // nearer to HBM, and 110 in BF16 (4.9 TB/s), with the one-unit rings.
 //
 // An item that ends in a later run leaves partials (max, sum, outputs): a CTA's warps join theirs

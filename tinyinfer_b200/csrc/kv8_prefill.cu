@@ -35,10 +35,10 @@
 // first.
 //
 // Bound by the softmax's chain of instructions: of the 6100 cycles that 256 vectors x 128 tokens
-// take in FP32 at head_dim 64 (16 x 512 rows of 9 / 3 heads at position 3584: 246 us), a thread
+// take in FP32 at head_dim 64 (16 x 512 rows of 9 / 3 heads at position 3584: 247 us), a thread
 // spends 900 on the maximum, 2900 on the weights, 640 on O and 700 waiting; an item's start and
 // end cost 700 more per tile. exp2 alone would take 2050, the products 2050 (3100 measured: P V is
-// 64 wide). At head_dim 128 BF16 (8 x 1024 rows of 32 / 8 heads at position 1000: 380 us, 534
+// 64 wide). At head_dim 128 BF16 (8 x 1024 rows of 32 / 8 heads at position 1000: 382 us, 531
 // TFLOP/s) it is 8000 cycles: 3600 of softmax, 2800 of waiting for S, whose place is free only after
 // the tile's own P V, 1500 of items' starts and ends.
 #include <algorithm>
