@@ -167,3 +167,8 @@ def test_wait_limits_out_of_range_are_refused(built, wait_us):
     with pytest.raises(mp.DeviceError) as e:
         mp.kv8_inject_wait_timeout(wait_us)
     assert e.value.code == mp.MP_ERR_INVALID
+
+
+def test_rotation_in_place_with_another_stride_is_refused(built):
+    """Rows would be overwritten before they are read."""
+    refused("append", mp.MP_ERR_INVALID, q_out_stride=640)

@@ -118,6 +118,8 @@ extern "C" int mp_kv8_append(const mp_kv8_cache* cache, const mp_kv8_append_args
     if (a->q) {
         MPB_TRY(check_buffer(a->q, a->q_stride, a->heads * d, a->type));
         MPB_TRY(check_buffer(a->q_out, a->q_out_stride, a->heads * d, a->type));
+        if (a->q_out == a->q && a->q_out_stride != a->q_stride)
+            return refuse(MP_ERR_INVALID, "kv8: q rotated in place with another row stride");
     }
     MPB_TRY(check_words(a->tables));
     MPB_TRY(check_words(a->row_offsets));
